@@ -174,7 +174,7 @@ def _plain_train(s):
         dz = dy * h * (sg * (1.0 + z * torch.sigmoid(-z)))
         dy = dy * (z * sg)
     if s["dlast"] is not None:
-        dy[:, -1] += s["dlast"]
+        dy = torch.cat((dy[:, :-1], dy[:, -1:] + s["dlast"].unsqueeze(1)), 1)  # dy can be the state's own tensor
     after = torch.cat((a[:, 1:], torch.zeros_like(a[:, :1])), 1)
     g = _recurrence(after.flip(1), dy.flip(1)).flip(1)
     first = torch.zeros_like(h[:, 0]) if s["init_state"] is None else s["init_state"]
