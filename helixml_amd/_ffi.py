@@ -92,6 +92,11 @@ SIGNATURES = {
     "hx_selective_scan_fwd_ws": [_i64, _i64, _i64, _i64, _int, _int] + [_p] * 11 + [_p, _sz, _p],
     "hx_selective_scan_fwd_noalloc": [_i64, _i64, _i64, _i64, _int, _int] + [_p] * 11 + [_p],
     "hx_selective_state_update": [_i64, _i64, _i64, _int, _int] + [_p] * 10 + [_p],
+    "hx_gated_scan_workspace_size": [_i64, _i64, _i64, _int],
+    "hx_gated_scan_fwd": [_i64, _i64, _i64, _int] + [_p] * 7 + [_p, _sz, _p],
+    "hx_gated_scan_bwd_workspace_size": [_i64, _i64, _i64, _int],
+    "hx_gated_scan_bwd": [_i64, _i64, _i64, _int] + [_p] * 10 + [_p, _sz, _p],
+    "hx_gated_state_update": [_i64, _i64, _int] + [_p] * 6,
     "hx_s4_discretize": [_i64, _f, _p, _p, _p],
     "hx_s4_ref_workspace_size": [_i64, _i64, _i64],
     "hx_s4_ref_fwd": [_i64, _i64, _i64, _f] + [_p] * 7 + [_p, _sz, _p],
@@ -105,6 +110,8 @@ SIGNATURES = {
                      _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p],
     "hx_gemm_bf16_splitk": [_i64, _i64, _i64, _p, _i64, _p, _i64, _p, _int, _int,
                             _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _int, _p, _sz, _p],
+    "hx_w4_quantize": [_i64, _i64, _p, _p, _p],
+    "hx_linear_w4": [_i64, _i64, _i64, _p, _i64, _p, _p, _p, _int, _int, _p, _i64, _p],
     "hx_conv1d_silu": [_i64, _i64, _i64, _i64, _int, _p, _i64, _p, _p, _p, _p],
     "hx_selective_scan_dtproj_fwd": [_i64, _i64, _i64, _i64] + [_p] * 12,
     "hx_mamba_block_workspace_size": [_i64, _i64, _i64, _i64, _i64],
@@ -115,6 +122,8 @@ SIGNATURES = {
     "hx_mamba_layer_workspace_size": [_i64] * 6,
     "hx_mamba_layer_fwd": [_i64] * 7 + [_p, _p, _f] + [_p] * 11 + [_p, _sz, _p],
     "hx_mamba_layer_decode": [_i64] * 6 + [_p, _p, _f] + [_p] * 11 + [_p, _sz, _p],
+    "hx_logits_adjust": [_i64, _i64, _int, _p, _i64, _p, _i64, _i64] + [_p] * 6 +
+                        [_i64, _p, _i64, _p, _i64, _p],
     "hx_binary_f32": [_int, _i64, _p, _p, _p, _p],
     "hx_unary_f32": [_int, _i64, _p, _f, _p, _p],
     "hx_mean_axis_f32": [_i64, _i64, _i64, _int, _p, _p, _p],

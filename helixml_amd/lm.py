@@ -21,7 +21,7 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _ffi
-from .ssm import _ptr, _stream, keep_for_stream, on_launch_stream
+from .ssm import _STORAGE, _need, _on_stream_device, _ptr, _stream, keep_for_stream, on_launch_stream
 
 _F32, _BF16 = _ffi.HX_F32, _ffi.HX_BF16
 
@@ -64,6 +64,73 @@ def conv1d_step(x, weight, bias, state, out=None, stream=None):
     dt = _F32 if x.dtype == torch.float32 else _BF16
     _ffi.call("hx_conv1d_step", bt, dim, width, dt, _ptr(x), x.stride(0), _ptr(weight), _ptr(bias),
               _ptr(state), _ptr(out), _stream(stream))
+    return out
+
+
+def _rows(t, name, shape, dtype):
+    """Checks a [batch, n] device tensor with unit column stride; its row stride (n for a single row)."""
+    if not t.is_cuda:
+        raise _ffi.InvalidInput(f"{name} must be a device tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise _ffi.ShapeMismatch(f"{name}: expected {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise _ffi.DTypeMismatch(f"{name}: expected {dtype}, got {t.dtype}")
+    if shape[1] > 1 and t.stride(1) != 1:
+        raise _ffi.InvalidInput(f"{name} needs unit column stride")
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+@on_launch_stream
+def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repetition=None, frequency=None,
+                  presence=None, bias=None, allowed=None, out=None, stream=None):
+    """What a decode step does to its logits [batch, vocab] (fp32 or bf16) before a token is chosen
+    (hx_logits_adjust): penalties for the tokens of ``history`` int32 [batch, n] (its first ``lengths[b]``
+    entries, all when None; entries outside the vocabulary are skipped), a bias, a grammar mask.
+
+      l = l / repetition if l > 0 else l * repetition     tokens anywhere in the history
+      l -= frequency * count + presence * (count > 0)     counted from ``prompt_lengths[b]`` on (0 when None)
+      l += bias                                           fp32 [vocab] or [batch, vocab]
+      l = -inf unless allowed                             int32 words, bit v % 32 of word v // 32:
+                                                          [ceil(vocab / 32)] or [batch, ceil(vocab / 32)]
+
+    repetition, frequency, presence: fp32 [batch]; lengths, prompt_lengths: int32 [batch]. Rows may be strided.
+    ``out``: where the result goes (``logits`` itself for in place); a new tensor when None."""
+    if logits.dim() != 2:
+        raise _ffi.ShapeMismatch(f"logits: expected [batch, vocab], got {list(logits.shape)}")
+    if logits.dtype not in _STORAGE:
+        raise _ffi.DTypeMismatch(f"logits: {logits.dtype} is neither float32 nor bfloat16")
+    bt, V = shape = logits.shape
+    ldl = _rows(logits, "logits", shape, logits.dtype)
+    ldh = n = 0
+    if history is not None:
+        if history.dim() != 2:
+            raise _ffi.ShapeMismatch(f"history: expected [batch, n], got {list(history.shape)}")
+        n = history.shape[1]
+        ldh = _rows(history, "history", (bt, n), torch.int32)
+    for name, t, dtype in (("lengths", lengths, torch.int32), ("prompt_lengths", prompt_lengths, torch.int32),
+                           ("repetition", repetition, torch.float32), ("frequency", frequency, torch.float32),
+                           ("presence", presence, torch.float32)):
+        _need(t, name, (bt,), dtype)
+    words = -(-V // 32)
+    ldb = lda = 0
+    if bias is not None:
+        if bias.dim() == 1:
+            _need(bias, "bias", (V,), torch.float32)
+        else:
+            ldb = _rows(bias, "bias", shape, torch.float32)
+    if allowed is not None:
+        if allowed.dim() == 1:
+            _need(allowed, "allowed", (words,), torch.int32)
+        else:
+            lda = _rows(allowed, "allowed", (bt, words), torch.int32)
+    if out is None:
+        out = torch.empty((bt, V), device=logits.device, dtype=logits.dtype)
+    ldo = _rows(out, "out", shape, logits.dtype)
+    _on_stream_device(stream, logits=logits, history=history, lengths=lengths, prompt_lengths=prompt_lengths,
+                      repetition=repetition, frequency=frequency, presence=presence, bias=bias, allowed=allowed, out=out)
+    _ffi.call("hx_logits_adjust", bt, V, _STORAGE[logits.dtype], _ptr(logits), ldl, _ptr(history), ldh, n,
+              _ptr(lengths), _ptr(prompt_lengths), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias), ldb,
+              _ptr(allowed), lda, _ptr(out), ldo, _stream(stream))
     return out
 
 

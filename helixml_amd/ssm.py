@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from . import _ffi
-from ._ffi import DTypeMismatch, InvalidInput, ShapeMismatch
+from ._ffi import DeviceMismatch, DTypeMismatch, InvalidInput, ShapeMismatch
 
 _STORAGE = {torch.float32: _ffi.HX_F32, torch.bfloat16: _ffi.HX_BF16}
 
@@ -51,6 +51,8 @@ def on_launch_stream(fn):
     @functools.wraps(fn)
     def run(*args, stream=None, **kwargs):
         ts = _torch_stream(stream)
+        if stream is None:  # the current stream: nothing to switch
+            return fn(*args, stream=ts, **kwargs)
         with torch.cuda.stream(ts):
             return fn(*args, stream=ts, **kwargs)
     run.on_launch_stream = True
@@ -75,6 +77,13 @@ def _need(t: Optional[torch.Tensor], name: str, shape, dtype) -> None:
         raise DTypeMismatch(f"{name}: expected {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise InvalidInput(f"{name} must be contiguous")
+
+
+def _on_stream_device(launch, **tensors) -> None:
+    """Raises DeviceMismatch unless every tensor lives on the device whose stream the kernels are launched on."""
+    for name, t in tensors.items():
+        if t is not None and t.device != launch.device:
+            raise DeviceMismatch(f"{name} is on {t.device}, the launch stream on {launch.device}")
 
 
 def selective_scan_workspace_size(batch, seqlen, dim, dstate, dtype=torch.float32):
@@ -175,6 +184,105 @@ def selective_state_update(state, u, delta, A, B, C, D=None, z=None, dt_bias=Non
     _ffi.call("hx_selective_state_update", bt, dim, N, _STORAGE[st], int(bool(delta_softplus)),
               _ptr(state), _ptr(u), _ptr(delta), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z),
               _ptr(dt_bias), _ptr(out), _stream(stream))
+    return out
+
+
+# steps between the states that gated_scan_fwd keeps for its backward pass
+GATED_CHUNK = 128
+
+
+def _gated_workspace(name, given, batch, seqlen, dim, dtype, device):
+    need = int(getattr(_ffi.lib(), name)(batch, seqlen, dim, _STORAGE[dtype]))
+    if need and given is None:
+        given = torch.empty(need, device=device, dtype=torch.uint8)
+    return (None, 0) if given is None else (given, given.numel() * given.element_size())
+
+
+@on_launch_stream
+def gated_scan_fwd(x, f, z=None, init_state=None, return_last_state=False, return_states=False, out=None,
+                   workspace=None, stream=None):
+    """Gated linear recurrence (hx_gated_scan_fwd): a = sigmoid(f), h_t = a_t h_{t-1} + (1 - a_t) x_t,
+    out = h, times silu(z) where z is given. x, f, z: [batch, L, dim] fp32 or bf16; init_state: [batch, dim]
+    fp32. Returns out, followed by the last state [batch, dim] fp32 and by the states that gated_scan_bwd
+    needs ([batch, ceil(L / GATED_CHUNK), dim] fp32) where asked for. ``workspace``: a uint8 device tensor of
+    at least gated_scan_workspace_size(...) bytes; allocated here when not given."""
+    if x.dim() != 3:
+        raise ShapeMismatch(f"x: expected 3 dims [batch, seqlen, dim], got {list(x.shape)}")
+    bt, L, dim = shape = x.shape
+    st = x.dtype
+    if st not in _STORAGE:
+        raise DTypeMismatch(f"x: storage dtype {st} is neither float32 nor bfloat16")
+    _need(x, "x", shape, st)
+    _need(f, "f", shape, st)
+    _need(z, "z", shape, st)
+    _need(init_state, "init_state", (bt, dim), torch.float32)
+    _need(out, "out", shape, st)
+    _on_stream_device(stream, x=x, f=f, z=z, init_state=init_state, out=out, workspace=workspace)
+    if out is None:
+        out = torch.empty_like(x)
+    f32 = torch.float32
+    last = torch.empty((bt, dim), device=x.device, dtype=f32) if return_last_state else None
+    states = torch.empty((bt, -(-L // GATED_CHUNK), dim), device=x.device, dtype=f32) if return_states else None
+    workspace, nbytes = _gated_workspace("hx_gated_scan_workspace_size", workspace, bt, L, dim, st, x.device)
+    _ffi.call("hx_gated_scan_fwd", bt, L, dim, _STORAGE[st], _ptr(x), _ptr(f), _ptr(z), _ptr(init_state), _ptr(out),
+              _ptr(last), _ptr(states), _ptr(workspace), nbytes, _stream(stream))
+    if not (return_last_state or return_states):
+        return out
+    return (out,) + ((last,) if return_last_state else ()) + ((states,) if return_states else ())
+
+
+@on_launch_stream
+def gated_scan_bwd(x, f, dout, states, z=None, dlast=None, workspace=None, stream=None):
+    """Gradients of gated_scan_fwd (hx_gated_scan_bwd): (dx, df, dz, dinit) from dout [batch, L, dim] and
+    dlast [batch, dim] fp32 (the last state's gradient; None: zero). x, f, z: the forward's inputs, states: what
+    it returned with return_states. dx, df, dz have x's type, dinit [batch, dim] fp32; dz is None without z."""
+    if x.dim() != 3:
+        raise ShapeMismatch(f"x: expected 3 dims [batch, seqlen, dim], got {list(x.shape)}")
+    bt, L, dim = shape = x.shape
+    st = x.dtype
+    if st not in _STORAGE:
+        raise DTypeMismatch(f"x: storage dtype {st} is neither float32 nor bfloat16")
+    _need(x, "x", shape, st)
+    _need(f, "f", shape, st)
+    _need(z, "z", shape, st)
+    _need(dout, "dout", shape, st)
+    _need(states, "states", (bt, -(-L // GATED_CHUNK), dim), torch.float32)
+    _need(dlast, "dlast", (bt, dim), torch.float32)
+    _on_stream_device(stream, x=x, f=f, z=z, dout=dout, states=states, dlast=dlast, workspace=workspace)
+    dx, df = torch.empty_like(x), torch.empty_like(x)
+    dz = None if z is None else torch.empty_like(x)
+    dinit = torch.empty((bt, dim), device=x.device, dtype=torch.float32)
+    workspace, nbytes = _gated_workspace("hx_gated_scan_bwd_workspace_size", workspace, bt, L, dim, st, x.device)
+    _ffi.call("hx_gated_scan_bwd", bt, L, dim, _STORAGE[st], _ptr(x), _ptr(f), _ptr(z), _ptr(states), _ptr(dout),
+              _ptr(dlast), _ptr(dx), _ptr(df), _ptr(dz), _ptr(dinit), _ptr(workspace), nbytes, _stream(stream))
+    return dx, df, dz, dinit
+
+
+def gated_scan_workspace_size(batch, seqlen, dim, dtype=torch.float32, backward=False) -> int:
+    """Bytes of scratch that gated_scan_fwd (or gated_scan_bwd) needs."""
+    name = "hx_gated_scan_bwd_workspace_size" if backward else "hx_gated_scan_workspace_size"
+    return int(getattr(_ffi.lib(), name)(batch, seqlen, dim, _STORAGE[dtype]))
+
+
+@on_launch_stream
+def gated_state_update(state, x, f, z=None, out=None, stream=None):
+    """One token of the gated recurrence (hx_gated_state_update); advances ``state`` [batch, dim] fp32 in
+    place. x, f, z, out: [batch, dim] fp32 or bf16."""
+    if x.dim() != 2:
+        raise ShapeMismatch(f"x: expected 2 dims [batch, dim], got {list(x.shape)}")
+    shape, st = x.shape, x.dtype
+    if st not in _STORAGE:
+        raise DTypeMismatch(f"x: storage dtype {st} is neither float32 nor bfloat16")
+    _need(state, "state", shape, torch.float32)
+    _need(x, "x", shape, st)
+    _need(f, "f", shape, st)
+    _need(z, "z", shape, st)
+    _need(out, "out", shape, st)
+    _on_stream_device(stream, state=state, x=x, f=f, z=z, out=out)
+    if out is None:
+        out = torch.empty_like(x)
+    _ffi.call("hx_gated_state_update", shape[0], shape[1], _STORAGE[st], _ptr(state), _ptr(x), _ptr(f), _ptr(z),
+              _ptr(out), _stream(stream))
     return out
 
 
@@ -309,6 +417,66 @@ def gemm_bf16(X, W, bias=None, act=0, out_dtype=torch.bfloat16, splits=None, str
     else:
         _ffi.call("hx_gemm_bf16", *args, _stream(stream))
     return outs[0] if len(outs) == 1 else tuple(outs)
+
+
+W4_GROUP = 32
+
+
+def _w4_rows(K):
+    """Bytes of one packed row and of one row of scales (include/helix_hip.h, "4-bit weights")."""
+    groups = -(-K // W4_GROUP)
+    return 16 * groups, 16 * -(-groups // 16)
+
+
+def w4_quantize(W, device=None):
+    """Rounds a weight [N, K] to 4 bits with group scales (hx_w4_quantize, OCP MXFP4): (packed, scales), uint8
+    tensors [N, 16 ceil(K / 32)] and [N, 16 ceil(K / 512)] on ``device`` (W's own when None). Runs on the
+    host, once per weight; W is read back if it lives on the device."""
+    if W.dim() != 2:
+        raise ShapeMismatch(f"W: expected [N, K], got {list(W.shape)}")
+    N, K = W.shape
+    w = np.ascontiguousarray(W.detach().float().cpu().numpy())
+    pr, sr = _w4_rows(K)
+    packed, scales = np.empty((N, pr), np.uint8), np.empty((N, sr), np.uint8)
+    _ffi.call("hx_w4_quantize", N, K, w.ctypes.data, packed.ctypes.data, scales.ctypes.data)
+    device = W.device if device is None else device
+    return torch.from_numpy(packed).to(device), torch.from_numpy(scales).to(device)
+
+
+@on_launch_stream
+def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=None):
+    """Y = X . W^T (+ bias)(, SiLU) with 4-bit weights (hx_linear_w4). X [M, K] bf16 (rows may be strided);
+    packed, scales: what w4_quantize gives for W [N, K]; bias [N] fp32. act: bit 0 SiLU, bit 1 adds to
+    ``out`` [M, N] (rows may be strided), which has to be given then."""
+    if X.dim() != 2 or packed.dim() != 2:
+        raise ShapeMismatch(f"X, packed: expected 2 dims, got {list(X.shape)}, {list(packed.shape)}")
+    M, K = X.shape
+    N = packed.shape[0]
+    if X.dtype != torch.bfloat16:
+        raise DTypeMismatch("linear_w4: X must be bfloat16")
+    if K > 1 and X.stride(1) != 1:
+        raise InvalidInput("linear_w4: X needs unit column stride")
+    pr, sr = _w4_rows(K)
+    _need(packed, "packed", (N, pr), torch.uint8)
+    _need(scales, "scales", (N, sr), torch.uint8)
+    _need(bias, "bias", (N,), torch.float32)
+    if out is None:
+        if act & 2:
+            raise InvalidInput("linear_w4: act bit 1 adds to out, which is not given")
+        if out_dtype not in _STORAGE:
+            raise DTypeMismatch(f"out_dtype {out_dtype} is neither float32 nor bfloat16")
+        out = torch.empty((M, N), device=X.device, dtype=out_dtype)
+    elif tuple(out.shape) != (M, N):
+        raise ShapeMismatch(f"out: expected {[M, N]}, got {list(out.shape)}")
+    elif out.dtype not in _STORAGE:
+        raise DTypeMismatch(f"out: {out.dtype} is neither float32 nor bfloat16")
+    elif N > 1 and out.stride(1) != 1:
+        raise InvalidInput("linear_w4: out needs unit column stride")
+    _on_stream_device(stream, X=X, packed=packed, scales=scales, bias=bias, out=out)
+    # a single row has no stride: torch may report any
+    _ffi.call("hx_linear_w4", M, N, K, _ptr(X), X.stride(0) if M > 1 else K, _ptr(packed), _ptr(scales), _ptr(bias),
+              int(act), _STORAGE[out.dtype], _ptr(out), out.stride(0) if M > 1 else N, _stream(stream))
+    return out
 
 
 def set_scan_variant(v: int) -> None:

@@ -152,6 +152,44 @@ int hx_selective_state_update(int64_t batch, int64_t dim, int64_t dstate,
                               const void* z, const float* dt_bias, void* out,
                               void* stream);
 
+/* ------------------------------------------------------------------ gated linear recurrence */
+/* A linear recurrence with one state per channel and a forget gate per token, over whole sequences:
+ *   a = sigmoid(f);  h_t = a_t * h_{t-1} + (1 - a_t) * x_t;  out_t = h_t (* silu(z_t) if z != NULL)
+ * (1 - a is formed as sigmoid(-f), so closed and open gates keep their relative accuracy.)
+ * The reference's recurrences (crates/nn/src/ssm.rs:138-186, :474-483) carry dstate states and no
+ * gate per token; this is the elementwise member of the family and the only one with a gradient.
+ * x, f, z, out: [batch, seqlen, dim] of `dtype`; init_state, last_state: [batch, dim] fp32.
+ * init_state (nullable) seeds h; last_state (nullable) receives h after the last step (init_state,
+ * or zero, where seqlen is 0).
+ * states (nullable): [batch, ceil(seqlen / HX_GATED_CHUNK), dim] fp32, receives h BEFORE steps 0,
+ * HX_GATED_CHUNK, 2 * HX_GATED_CHUNK, ...: what hx_gated_scan_bwd forms h from again.
+ * workspace: hx_gated_scan_workspace_size(...) bytes of device memory (0: none needed), 16-byte
+ * aligned; it holds nothing between calls, and one call uses it at a time. */
+#define HX_GATED_CHUNK 128
+size_t hx_gated_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype);
+int hx_gated_scan_fwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, const void* x,
+                      const void* f, const void* z, const float* init_state, void* out,
+                      float* last_state, float* states, void* workspace, size_t workspace_bytes,
+                      void* stream);
+/* Its backward pass. With dh = dout * silu(z) (dout without a gate), dh_{L-1} += dlast, and
+ *   g_t = dh_t + a_{t+1} * g_{t+1}:
+ *   dx = (1 - a) * g;  df = g * a * (1 - a) * (h_{t-1} - x);  dz = dout * h * silu'(z);
+ *   dinit = a_0 * g_0  (the gradient of the entry state; dlast, or zero, where seqlen is 0)
+ * x, f, z and states: what hx_gated_scan_fwd took and gave (its init_state is states' first entry).
+ * dout, dx, df, dz: [batch, seqlen, dim] of `dtype`; dlast (nullable: zero), dinit (nullable: not
+ * wanted): [batch, dim] fp32. dz is required exactly where z is given. h is formed again in fp32
+ * from `states`, so nothing of `out`'s rounding enters a gradient. workspace as above, of
+ * hx_gated_scan_bwd_workspace_size(...) bytes. */
+size_t hx_gated_scan_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype);
+int hx_gated_scan_bwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, const void* x,
+                      const void* f, const void* z, const float* states, const void* dout,
+                      const float* dlast, void* dx, void* df, void* dz, float* dinit,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* One token of that recurrence for every sequence: state [batch, dim] fp32 is advanced in place;
+ * x, f, z (nullable), out: [batch, dim] of `dtype`. */
+int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, const void* x,
+                          const void* f, const void* z, void* out, void* stream);
+
 /* ------------------------------------------------------------------ S4 recurrences */
 /* nn::ssm::S4Block::discretize(dt)'s real decay (crates/nn/src/ssm.rs:113-120) on HOST arrays:
  * a[n] = expf(a_real[n]*dt) * cosf(a_imag[n]*dt), each product rounded to f32 first, with the
@@ -244,6 +282,31 @@ int hx_gemm_bf16_splitk(int64_t M, int64_t N, int64_t K, const void* X, int64_t 
                         int64_t split2, void* Y2, int64_t ld2, int splits, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* 4-bit weights with group scales, OCP Microscaling MXFP4: element k of row n is
+ *   w[n][k] = E2M1(code) * 2^(scale - 127),
+ * code = 4 bits (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), one scale byte
+ * per HX_W4_GROUP = 32 elements along k. Row n of `packed` starts at n * 16 * G bytes, G = ceil(K / 32):
+ * element 2j in the low and 2j + 1 in the high nibble of byte j, elements from K on unused. Row n of
+ * `scales` starts at n * 16 * ceil(G / 16) bytes, group g's byte at g, bytes from G on unused. Scale
+ * bytes 2..252 (2^-125 .. 2^125, what hx_w4_quantize writes) are exact; 255 is NaN; with 0, 1, 253 and
+ * 254 a weight can leave the normal range of bf16 and then is flushed or overflows there. */
+#define HX_W4_GROUP 32
+/* Rounds weights w [N, K] (the Linear layout, row stride K) to that format, all three on the HOST: a
+ * group's scale is the power of two that puts its largest magnitude into [4, 8) (clamped to the exact
+ * bytes; 2^-125 for a group of zeros), elements round to the nearest code, ties to the even code,
+ * magnitudes above 6 to 6. Unused elements and scale bytes are written as 0 and 127. A weight that
+ * is not finite is refused (HX_ERR_INVALID_INPUT). Done once per weight, as hx_s4_discretize is. */
+int hx_w4_quantize(int64_t N, int64_t K, const float* w, void* packed, void* scales);
+/* Y = X . W^T (+ bias)(, SiLU) with such weights, the nn::Linear layout (crates/nn/src/lib.rs:120-134):
+ * the weight-read-bound product of decode and of small batches. X [M, K] bf16 (row stride ldx),
+ * packed and scales as above (device, 16-byte aligned), bias [N] fp32 (nullable), Y [M, N] of
+ * out_dtype HX_F32 or HX_BF16 (row stride ldy); act as in hx_gemm_bf16 (bit 0 SiLU, bit 1 Y = Y + result).
+ * Weights are expanded to bf16 exactly and multiplied on the matrix core with fp32 accumulation. Any
+ * M, N, K; every X row gets the same arithmetic whatever M is. */
+int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const void* packed,
+                 const void* scales, const float* bias, int act, int out_dtype, void* Y,
+                 int64_t ldy, void* stream);
+
 /* Causal depthwise conv1d over time + bias + SiLU (the Mamba block's conv, kernel `width` <= 4):
  * y[b,t,d] = silu(bias[d] + sum_j weight[d,j] * x[b, t-width+1+j, d]) with zero padding.
  * x: [batch, seqlen, dim] with row stride ldx (so it can be the x half of in_proj's output);
@@ -331,6 +394,29 @@ int hx_mamba_layer_decode(int64_t batch, int64_t d_model, int64_t d_inner, int64
                           const float* A, const float* D, const void* w_out, float* ssm_state,
                           float* conv_state, void* workspace, size_t workspace_bytes,
                           void* stream);
+
+/* What a decode step does to its logits before a token is chosen. For row b and token v, with
+ *   seen  = v is among history[b][0 .. lengths[b]),
+ *   count = how often v is among history[b][prompt_lengths[b] .. lengths[b]):
+ *   l = logits[b][v];  if seen: l = l > 0 ? l / repetition[b] : l * repetition[b];
+ *   l = l - frequency[b] * count - presence[b] * (count > 0) + bias[b][v];
+ *   out[b][v] = allowed ? l : -inf
+ * so the repetition penalty covers prompt and answer, the other two the answer alone.
+ * logits, out: [batch, vocab] of `dtype` (row strides ldl, ldo; out may be logits itself with the same
+ * stride). history: int32 [batch, history_len] (row stride ldh; nullable with history_len 0); entries
+ * outside [0, vocab) are skipped. lengths (nullable: history_len), prompt_lengths (nullable: 0): int32
+ * [batch], clamped to [0, history_len]. repetition (nullable: 1), frequency, presence (nullable: 0):
+ * fp32 [batch]. bias (nullable): fp32, row stride ldb, 0 for one row shared by all. allowed
+ * (nullable): int32 words, bit v % 32 of word v / 32 set where token v is allowed; row stride lda words,
+ * 0 for one row shared by all. A row that allows nothing becomes -inf throughout; a NaN logit stays
+ * one unless it is masked. The reference has no sampling step (its byte LM stops at the logits,
+ * examples/ssm_byte_lm/src/main.rs:121-130). */
+int hx_logits_adjust(int64_t batch, int64_t vocab, int dtype, const void* logits, int64_t ldl,
+                     const int32_t* history, int64_t ldh, int64_t history_len,
+                     const int32_t* lengths, const int32_t* prompt_lengths,
+                     const float* repetition, const float* frequency, const float* presence,
+                     const float* bias, int64_t ldb, const int32_t* allowed, int64_t lda,
+                     void* out, int64_t ldo, void* stream);
 
 /* CpuTensor::matmul 2-D x 2-D (crates/backend-cpu/src/lib.rs:644-678): Y = A[M,K] . B[K,N]. */
 int hx_matmul_f32(int64_t M, int64_t K, int64_t N, const float* A, const float* B, float* Y,
