@@ -1,12 +1,10 @@
 // hx_gated.hip — the gated linear recurrence with one state per channel: forward, backward, one token.
 //   a = sigmoid(f), i = sigmoid(-f);  h_t = a_t h_{t-1} + i_t x_t;  out = h [silu(z)]
 #include "hx_common.h"
-#include "hx_wave.h"
+#include <initializer_list>
 
 namespace hx {
 namespace {
-
-constexpr int kChunk = HX_GATED_CHUNK;
 
 // Both gates from one exponential of -|f|, which is at most 1: neither overflows, and the smaller of
 // the two is a product, so it keeps its relative accuracy where the other rounds to 1. A state's decay
@@ -29,69 +27,382 @@ __device__ inline void silu_grad(float z, float& v, float& d) {
     d = s * fmaf(z, t, 1.0f);
 }
 
-// One thread per (batch, channel), in time order.
-template <typename T>
-__global__ __launch_bounds__(64) void gated_fwd_kernel(int64_t rows, int64_t L, int64_t D, const T* __restrict__ x,
-                                                       const T* __restrict__ f, const T* __restrict__ z,
-                                                       const float* __restrict__ init, T* __restrict__ out,
-                                                       float* __restrict__ last, float* __restrict__ states) {
-    const int64_t r = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (r >= rows) return;
-    const int64_t b = r / D, d = r - b * D, nc = (L + kChunk - 1) / kChunk;
-    float h = init ? init[r] : 0.0f;
-    for (int64_t t = 0; t < L; ++t) {
-        if (states && t % kChunk == 0) states[(b * nc + t / kChunk) * D + d] = h;
-        const int64_t o = (b * L + t) * D + d;
-        float a, i;
-        gates(Storage<T>::load(f + o), a, i);
-        h = fmaf(a, h, i * Storage<T>::load(x + o));
-        Storage<T>::store(out + o, z ? h * silu(Storage<T>::load(z + o)) : h);
+// ------------------------------------------------------------------ tiles
+// A block owns a tile of kTile steps x 64 channels of one sequence. Lane (half, c) of wave w holds channels
+// 2c and 2c+1 of the kSteps consecutive steps of part p = 2w + half, so a row of the tile is one 128-byte (bf16)
+// or 256-byte (fp32) run and every element is read once and stays in registers. A part is the affine map
+// h -> A h + H (A the product of its gates); the tile's parts are joined in LDS and the tiles of a sequence
+// through the workspace: a tile publishes its map as soon as it has it, then its exit state once it knows its
+// entry state, which it forms from the nearest exit state that is there and the maps after it.
+constexpr int kSteps = 8, kWaves = 8, kParts = 2 * kWaves, kTile = kParts * kSteps, kWidth = 64;
+static_assert(kTile == HX_GATED_CHUNK, "a tile's entry state is one of `states`");
+
+// Two neighbouring channels as they are stored.
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+    using raw = float2;
+    __device__ static inline raw wide(const float* p) { return *reinterpret_cast<const float2*>(p); }
+    __device__ static inline raw make(float a, float b) { return make_float2(a, b); }
+    __device__ static inline float lo(raw r) { return r.x; }
+    __device__ static inline float hi(raw r) { return r.y; }
+    __device__ static inline void store(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+};
+template <> struct Pair<uint16_t> {
+    using raw = uint32_t;
+    __device__ static inline raw wide(const uint16_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+    __device__ static inline raw make(uint16_t a, uint16_t b) { return (uint32_t)b << 16 | a; }
+    __device__ static inline float lo(raw r) { return __uint_as_float(r << 16); }
+    __device__ static inline float hi(raw r) { return __uint_as_float(r & 0xffff0000u); }
+    __device__ static inline void store(uint16_t* p, float a, float b) {
+        *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(a, b);
     }
-    if (last) last[r] = h;
+};
+
+// Where a lane's elements lie. VEC: even dim and pairs aligned to a wide load.
+template <typename T, bool VEC>
+struct Place {
+    int64_t row;   // of the wave's first step, its first channel (uniform)
+    int64_t D;
+    uint32_t off;  // the lane's part and channel from there
+    int steps;     // of this lane that lie inside the sequence, none for channels behind the last
+    bool second;   // the pair's second channel exists
+
+    __device__ Place(int64_t b, int64_t t0, int64_t c0, int wave, int lane, int64_t L, int64_t dim) : D(dim) {
+        const int half = lane >> 5, c = (lane & 31) * 2;
+        row = (b * L + t0 + wave * 2 * kSteps) * D + c0;
+        off = (uint32_t)(half * kSteps * D + c);
+        const int64_t left = L - t0 - (wave * 2 + half) * kSteps;
+        steps = c0 + c < D ? (int)(left < 0 ? 0 : left < kSteps ? left : kSteps) : 0;
+        second = c0 + c + 1 < D;
+    }
+    __device__ inline typename Pair<T>::raw load(const T* base, int j) const {
+        const T* p = base + (row + j * D);
+        if (VEC) return Pair<T>::wide(p + off);
+        return Pair<T>::make(p[off], second ? p[off + 1] : p[off]);
+    }
+    __device__ inline void store(T* base, int j, float a, float b) const {
+        T* p = base + (row + j * D);
+        if (VEC) {
+            Pair<T>::store(p + off, a, b);
+        } else {
+            Storage<T>::store(p + off, a);
+            if (second) Storage<T>::store(p + off + 1, b);
+        }
+    }
+    // All of the tile's loads of one operand, for the steps that exist.
+    __device__ inline void load_all(const T* base, typename Pair<T>::raw (&r)[kSteps]) const {
+        if (__all(steps == kSteps)) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) r[j] = load(base, j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) r[j] = j < steps ? load(base, j) : typename Pair<T>::raw{};
+        }
+    }
+};
+
+// The workspace: a ticket, then for each tile and channel its map (A, H) as one 64-bit word and its exit state as
+// one 32-bit word. A word of all ones is not there yet: every word is written once, whole, and carries its own
+// readiness, so no fence is needed, only that readers and writers meet beyond the L2 of their XCD (agent scope).
+struct Chain {
+    uint32_t* ticket;
+    unsigned long long* maps;
+    uint32_t* exits;
+    int tiles;       // of one sequence
+    uint32_t lanes;  // sequences x column tiles
+};
+constexpr uint32_t kAbsent = 0xffffffffu, kNaN = 0x7fc00000u;
+constexpr int kWindow = 8;  // tiles that one look back covers
+// A wait ends by itself where the workspace is misused (two calls at once): some 10^5 looks of about a microsecond.
+constexpr int kLooks = 1 << 17;
+
+__device__ inline uint32_t word_of(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return u == kAbsent ? kNaN : u;
+}
+// The first word of tile k in a column: uniform, so that a lane's part of an address is its number.
+__device__ inline size_t row_of(const Chain& c, int k, uint32_t col) { return ((size_t)k * c.lanes + col) * kWidth; }
+__device__ inline void publish_map(const Chain& c, int k, uint32_t col, int lane, float A, float H) {
+    __hip_atomic_store(c.maps + row_of(c, k, col) + lane, (unsigned long long)word_of(H) << 32 | word_of(A),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void publish_exit(const Chain& c, int k, uint32_t col, int lane, float v) {
+    __hip_atomic_store(c.exits + row_of(c, k, col) + lane, word_of(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// One thread per (batch, channel), chunks from the last: a chunk's states before each step are formed
-// again from the stored one and kept in LDS.
-template <typename T>
-__global__ __launch_bounds__(64) void gated_bwd_kernel(int64_t rows, int64_t L, int64_t D, const T* __restrict__ x,
-                                                       const T* __restrict__ f, const T* __restrict__ z,
-                                                       const float* __restrict__ states, const T* __restrict__ dout,
-                                                       const float* __restrict__ dlast, T* __restrict__ dx,
-                                                       T* __restrict__ df, T* __restrict__ dz, float* __restrict__ dinit) {
-    __shared__ float before[kChunk][64];
-    const int64_t r = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (r >= rows) return;
-    const int64_t b = r / D, d = r - b * D, nc = (L + kChunk - 1) / kChunk;
-    float carry = dlast ? dlast[r] : 0.0f;  // a_{t+1} g_{t+1}
-    for (int64_t c = nc - 1; c >= 0; --c) {
-        const int64_t t0 = c * kChunk;
-        const int n = (int)(L - t0 < kChunk ? L - t0 : kChunk);
-        float h = states[(b * nc + c) * D + d];
-        for (int k = 0; k < n; ++k) {
-            const int64_t o = (b * L + t0 + k) * D + d;
-            before[k][threadIdx.x] = h;
-            float a, i;
-            gates(Storage<T>::load(f + o), a, i);
-            h = fmaf(a, h, i * Storage<T>::load(x + o));
+// The state that tile k of a chain starts from; `first` is the chain's own. An exit state is its tile's map applied
+// to its entry state, whoever applies it, so the bits do not depend on which words were there.
+__device__ inline float entry_of(const Chain& c, int k, uint32_t col, int lane, float first) {
+    float e = first;
+    bool have = k == 0;
+    for (int look = 0; look < kLooks && !__all(have); ++look) {
+        if (look) __builtin_amdgcn_s_sleep(2);
+        uint32_t s[kWindow];
+        unsigned long long m[kWindow];
+#pragma unroll
+        for (int i = 0; i < kWindow; ++i) {
+            const int j = k - kWindow + i;
+            const size_t row = row_of(c, j < 0 ? 0 : j, col);
+            s[i] = __hip_atomic_load(c.exits + row + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            m[i] = __hip_atomic_load(c.maps + row + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        for (int k = n - 1; k >= 0; --k) {
-            const int64_t o = (b * L + t0 + k) * D + d;
-            const float xv = Storage<T>::load(x + o), hb = before[k][threadIdx.x], dy = Storage<T>::load(dout + o);
-            float a, i, dh = dy;
-            gates(Storage<T>::load(f + o), a, i);
-            if (z) {
-                float v, g;
-                silu_grad(Storage<T>::load(z + o), v, g);
-                Storage<T>::store(dz + o, dy * fmaf(a, hb, i * xv) * g);
-                dh = dy * v;
+        float v = first;
+        bool ok = k <= kWindow;  // the window reaches the chain's start
+#pragma unroll
+        for (int i = 0; i < kWindow; ++i) {
+            if (k - kWindow + i < 0) continue;
+            const float A = __uint_as_float((uint32_t)m[i]), H = __uint_as_float((uint32_t)(m[i] >> 32));
+            if (s[i] != kAbsent) {
+                v = __uint_as_float(s[i]);
+                ok = true;
+            } else {
+                v = fmaf(A, v, H);
+                ok = ok && m[i] != ~0ull;
             }
-            const float g = dh + carry, gi = g * i;
-            Storage<T>::store(dx + o, gi);
-            Storage<T>::store(df + o, gi * a * (hb - xv));
-            carry = g * a;
+        }
+        if (ok) {
+            e = v;
+            have = true;
         }
     }
-    if (dinit) dinit[r] = carry;
+    return have ? e : __uint_as_float(kNaN);
+}
+
+// Which tile this block takes: tickets are handed out in the order in which blocks start, tile 0 of every column
+// first, so what a block waits for is always held by a block that has started.
+__device__ inline bool take_unit(const Chain& c, uint32_t& shared_unit, int& k, uint32_t& col) {
+    uint32_t unit = blockIdx.x;
+    if (c.tiles > 1) {
+        if (threadIdx.x == 0) shared_unit = atomicAdd(c.ticket, 1u);
+        __syncthreads();
+        unit = __builtin_amdgcn_readfirstlane(shared_unit);
+    }
+    k = (int)(unit / c.lanes);
+    col = unit - (uint32_t)k * c.lanes;
+    return k < c.tiles;
+}
+
+struct FwdArgs {
+    int64_t L, D;
+    const void *x, *f, *z;
+    const float* init;
+    void* out;
+    float *last, *states;
+    uint32_t cols;  // column tiles of one sequence
+    Chain chain;
+};
+
+template <typename T, bool VEC, bool GATE>
+__global__ __launch_bounds__(64 * kWaves, 4) void gated_fwd_kernel(const FwdArgs p) {
+    __shared__ float2 maps[kParts][kWidth];
+    __shared__ float entries[kParts][kWidth];
+    __shared__ uint32_t shared_unit;
+    int k;
+    uint32_t col;
+    if (!take_unit(p.chain, shared_unit, k, col)) return;
+    const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Place<T, VEC> at(b, (int64_t)k * kTile, c0, wave, lane, p.L, p.D);
+    typename Pair<T>::raw rf[kSteps], rx[kSteps], rz[kSteps];
+    at.load_all((const T*)p.f, rf);
+    at.load_all((const T*)p.x, rx);
+    if (GATE) at.load_all((const T*)p.z, rz);
+
+    float a0[kSteps], a1[kSteps], b0[kSteps], b1[kSteps];
+    float A0 = 1.0f, A1 = 1.0f, H0 = 0.0f, H1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        float i0, i1;
+        gates(Pair<T>::lo(rf[j]), a0[j], i0);
+        gates(Pair<T>::hi(rf[j]), a1[j], i1);
+        b0[j] = i0 * Pair<T>::lo(rx[j]);
+        b1[j] = i1 * Pair<T>::hi(rx[j]);
+        if (j >= at.steps) {  // a step that is not there changes nothing
+            a0[j] = a1[j] = 1.0f;
+            b0[j] = b1[j] = 0.0f;
+        }
+        H0 = fmaf(a0[j], H0, b0[j]);
+        H1 = fmaf(a1[j], H1, b1[j]);
+        A0 *= a0[j];
+        A1 *= a1[j];
+    }
+    const int part = wave * 2 + (lane >> 5), c = (lane & 31) * 2;
+    *reinterpret_cast<float4*>(&maps[part][c]) = make_float4(A0, H0, A1, H1);
+    __syncthreads();
+    if (wave == 0) {
+        const bool in = c0 + lane < p.D;
+        const int64_t r = b * p.D + c0 + lane;
+        float A = 1.0f, H = 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < kParts; ++s) {
+            const float2 m = maps[s][lane];
+            H = fmaf(m.x, H, m.y);
+            A *= m.x;
+        }
+        float e = in && p.init ? p.init[r] : 0.0f;
+        if (p.chain.tiles > 1) {
+            if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, H);
+            e = entry_of(p.chain, k, col, lane, e);
+            if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, H));
+        }
+        if (in && p.states) p.states[(b * p.chain.tiles + k) * p.D + c0 + lane] = e;
+        if (in && p.last && k + 1 == p.chain.tiles) p.last[r] = fmaf(A, e, H);
+#pragma unroll 8
+        for (int s = 0; s < kParts; ++s) {
+            const float2 m = maps[s][lane];
+            entries[s][lane] = e;
+            e = fmaf(m.x, e, m.y);
+        }
+    }
+    __syncthreads();
+    const float2 e = *reinterpret_cast<const float2*>(&entries[part][c]);
+    float h0 = e.x, h1 = e.y;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        h0 = fmaf(a0[j], h0, b0[j]);
+        h1 = fmaf(a1[j], h1, b1[j]);
+        if (j < at.steps)
+            at.store((T*)p.out, j, GATE ? h0 * silu(Pair<T>::lo(rz[j])) : h0, GATE ? h1 * silu(Pair<T>::hi(rz[j])) : h1);
+    }
+}
+
+struct BwdArgs {
+    int64_t L, D;
+    const void *x, *f, *z, *dout;
+    const float *states, *dlast;
+    void *dx, *df, *dz;
+    float* dinit;
+    uint32_t cols;
+    Chain chain;
+};
+
+// The tiles from the last one back. The carry c_t = a_t g_t obeys c_t = a_t c_{t+1} + a_t dh_t, so parts and tiles
+// are affine maps again, with the same A. h is formed from `states` for the tile alone, without waiting.
+template <typename T, bool VEC, bool GATE>
+__global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs p) {
+    __shared__ float maps_a[kParts][kWidth], maps_h[kParts][kWidth], maps_g[kParts][kWidth];
+    __shared__ uint32_t shared_unit;
+    int k;
+    uint32_t col;
+    if (!take_unit(p.chain, shared_unit, k, col)) return;
+    const int tile = p.chain.tiles - 1 - k;
+    const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Place<T, VEC> at(b, (int64_t)tile * kTile, c0, wave, lane, p.L, p.D);
+    typename Pair<T>::raw rf[kSteps], rx[kSteps], rz[kSteps], rd[kSteps];
+    at.load_all((const T*)p.f, rf);
+    at.load_all((const T*)p.x, rx);
+    at.load_all((const T*)p.dout, rd);
+    if (GATE) at.load_all((const T*)p.z, rz);
+
+    float a0[kSteps], a1[kSteps], i0[kSteps], i1[kSteps];
+    float A0 = 1.0f, A1 = 1.0f, H0 = 0.0f, H1 = 0.0f, G0 = 0.0f, G1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        gates(Pair<T>::lo(rf[j]), a0[j], i0[j]);
+        gates(Pair<T>::hi(rf[j]), a1[j], i1[j]);
+        if (j >= at.steps) {
+            a0[j] = a1[j] = 1.0f;
+            i0[j] = i1[j] = 0.0f;
+        }
+        H0 = fmaf(a0[j], H0, i0[j] * Pair<T>::lo(rx[j]));
+        H1 = fmaf(a1[j], H1, i1[j] * Pair<T>::hi(rx[j]));
+        A0 *= a0[j];
+        A1 *= a1[j];
+    }
+#pragma unroll
+    for (int j = kSteps - 1; j >= 0; --j) {
+        float d0 = Pair<T>::lo(rd[j]), d1 = Pair<T>::hi(rd[j]);
+        if (GATE) {
+            d0 *= silu(Pair<T>::lo(rz[j]));
+            d1 *= silu(Pair<T>::hi(rz[j]));
+        }
+        G0 = a0[j] * (G0 + d0);
+        G1 = a1[j] * (G1 + d1);
+    }
+    const int part = wave * 2 + (lane >> 5), c = (lane & 31) * 2;
+    *reinterpret_cast<float2*>(&maps_a[part][c]) = make_float2(A0, A1);
+    *reinterpret_cast<float2*>(&maps_h[part][c]) = make_float2(H0, H1);
+    *reinterpret_cast<float2*>(&maps_g[part][c]) = make_float2(G0, G1);
+    __syncthreads();
+    // Wave 0 joins the carries and waits for the tiles after this one, wave 1 the states; each leaves its parts' entry
+    // values where the maps were that only it reads.
+    if (wave == 0) {
+        const bool in = c0 + lane < p.D;
+        const int64_t r = b * p.D + c0 + lane;
+        float A = 1.0f, G = 0.0f;
+#pragma unroll 8
+        for (int s = kParts - 1; s >= 0; --s) {
+            const float m = maps_a[s][lane];
+            G = fmaf(m, G, maps_g[s][lane]);
+            A *= m;
+        }
+        float e = in && p.dlast ? p.dlast[r] : 0.0f;
+        if (p.chain.tiles > 1) {
+            if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, G);
+            e = entry_of(p.chain, k, col, lane, e);
+            if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, G));
+        }
+        if (in && p.dinit && tile == 0) p.dinit[r] = fmaf(A, e, G);
+#pragma unroll 8
+        for (int s = kParts - 1; s >= 0; --s) {
+            const float g = maps_g[s][lane];
+            maps_g[s][lane] = e;
+            e = fmaf(maps_a[s][lane], e, g);
+        }
+    } else if (wave == 1) {
+        float h = c0 + lane < p.D ? p.states[(b * p.chain.tiles + tile) * p.D + c0 + lane] : 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < kParts; ++s) {
+            const float m = maps_h[s][lane];
+            maps_h[s][lane] = h;
+            h = fmaf(maps_a[s][lane], h, m);
+        }
+    }
+    __syncthreads();
+    const float2 eh = *reinterpret_cast<const float2*>(&maps_h[part][c]);
+    const float2 eg = *reinterpret_cast<const float2*>(&maps_g[part][c]);
+    // dout and z were kept as stored, and silu(z) is formed again with its derivative: 32 registers less at the wait
+    float h0[kSteps], h1[kSteps], d0[kSteps], d1[kSteps];  // the state before each step, dh
+    float n0 = eh.x, n1 = eh.y;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        h0[j] = n0;
+        h1[j] = n1;
+        n0 = fmaf(a0[j], n0, i0[j] * Pair<T>::lo(rx[j]));
+        n1 = fmaf(a1[j], n1, i1[j] * Pair<T>::hi(rx[j]));
+        d0[j] = Pair<T>::lo(rd[j]);
+        d1[j] = Pair<T>::hi(rd[j]);
+        if (GATE) {
+            float v0, v1, s0, s1;
+            silu_grad(Pair<T>::lo(rz[j]), v0, s0);
+            silu_grad(Pair<T>::hi(rz[j]), v1, s1);
+            if (j < at.steps) at.store((T*)p.dz, j, d0[j] * n0 * s0, d1[j] * n1 * s1);
+            d0[j] *= v0;
+            d1[j] *= v1;
+        }
+    }
+    float g0 = eg.x, g1 = eg.y;
+#pragma unroll
+    for (int j = kSteps - 1; j >= 0; --j) {
+        g0 += d0[j];
+        g1 += d1[j];
+        const float q0 = g0 * i0[j], q1 = g1 * i1[j];
+        if (j < at.steps) {
+            at.store((T*)p.dx, j, q0, q1);
+            at.store((T*)p.df, j, q0 * a0[j] * (h0[j] - Pair<T>::lo(rx[j])), q1 * a1[j] * (h1[j] - Pair<T>::hi(rx[j])));
+        }
+        g0 *= a0[j];
+        g1 *= a1[j];
+    }
+}
+
+// Every word of the workspace absent, the ticket at its start.
+__global__ __launch_bounds__(256) void gated_chain_clear_kernel(uint4* ws, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t v = i == 0 ? 0 : kAbsent;
+    ws[i] = make_uint4(v, v, v, v);
 }
 
 template <typename T>
@@ -116,10 +427,31 @@ __global__ __launch_bounds__(256) void gated_state_copy_kernel(int64_t n, const 
 
 constexpr int64_t kMaxBlocks = 0x7fffffff;  // of one grid axis
 
-// batch * seqlen * dim elements whose byte offsets fit 63 bits, rows that fit one grid axis.
-bool sizes_fit(int64_t batch, int64_t seqlen, int64_t dim) {
-    __int128 n = (__int128)batch * dim;
-    return n < (__int128)64 * kMaxBlocks && n * (seqlen > 0 ? seqlen : 1) < ((__int128)1 << 60);
+struct Shape {
+    int64_t batch, L, D, cols, tiles, units;
+    Shape(int64_t batch_, int64_t L_, int64_t D_)
+        : batch(batch_), L(L_), D(D_), cols((D_ + kWidth - 1) / kWidth), tiles((L_ + kTile - 1) / kTile),
+          units(fits() ? batch_ * cols * tiles : 0) {}
+    // Byte offsets of 63 bits, a lane's offset inside its wave's rows of 32, one block a tile.
+    bool fits() const {
+        return batch < kMaxBlocks && D < (1 << 26) && L < ((int64_t)1 << 37) &&
+               (__int128)batch * cols * (tiles > 0 ? tiles : 1) < kMaxBlocks && (__int128)batch * L * D < ((__int128)1 << 60);
+    }
+    // 16 bytes for the ticket, a map (8 bytes) and an exit state (4) per tile and channel; one tile waits for nobody
+    size_t workspace() const { return tiles > 1 ? 16 + (size_t)units * kWidth * 12 : 0; }
+    Chain chain(void* ws) const {
+        char* w = (char*)ws;
+        return Chain{(uint32_t*)w, (unsigned long long*)(w + 16), (uint32_t*)(w + 16 + (size_t)units * kWidth * 8), (int)tiles,
+                     (uint32_t)(batch * cols)};
+    }
+};
+
+int clear_chain(const Shape& g, void* ws, hipStream_t s) {
+    if (g.tiles <= 1) return HX_OK;
+    const int64_t n = (int64_t)(g.workspace() / 16);
+    hipLaunchKernelGGL(gated_chain_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (uint4*)ws, n);
+    HX_LAUNCH_CHECK();
+    return HX_OK;
 }
 
 int copy_state(int64_t rows, const float* src, float* dst, hipStream_t s) {
@@ -129,31 +461,50 @@ int copy_state(int64_t rows, const float* src, float* dst, hipStream_t s) {
     return HX_OK;
 }
 
+// Pairs can be loaded whole: even rows, every operand aligned to a pair.
 template <typename T>
-int fwd(int64_t batch, int64_t L, int64_t D, const void* x, const void* f, const void* z, const float* init, void* out,
-        float* last, float* states, hipStream_t s) {
-    const int64_t rows = batch * D;
-    hipLaunchKernelGGL(gated_fwd_kernel<T>, dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, s, rows, L, D, (const T*)x,
-                       (const T*)f, (const T*)z, init, (T*)out, last, states);
+bool pairs(int64_t D, std::initializer_list<const void*> ops) {
+    if (D % 2) return false;
+    for (const void* p : ops)
+        if (!aligned(p, 2 * sizeof(T))) return false;
+    return true;
+}
+
+template <typename T>
+int fwd(const Shape& g, const FwdArgs& p, hipStream_t s) {
+    const bool vec = pairs<T>(g.D, {p.x, p.f, p.z, p.out});
+    const auto k = vec ? (p.z ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
+                       : (p.z ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
+    hipLaunchKernelGGL(k, dim3((unsigned)g.units), dim3(64 * kWaves), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
 
 template <typename T>
-int bwd(int64_t batch, int64_t L, int64_t D, const void* x, const void* f, const void* z, const float* states,
-        const void* dout, const float* dlast, void* dx, void* df, void* dz, float* dinit, hipStream_t s) {
-    const int64_t rows = batch * D;
-    hipLaunchKernelGGL(gated_bwd_kernel<T>, dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, s, rows, L, D, (const T*)x,
-                       (const T*)f, (const T*)z, states, (const T*)dout, dlast, (T*)dx, (T*)df, (T*)dz, dinit);
+int bwd(const Shape& g, const BwdArgs& p, hipStream_t s) {
+    const bool vec = pairs<T>(g.D, {p.x, p.f, p.z, p.dout, p.dx, p.df, p.dz});
+    const auto k = vec ? (p.z ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
+                       : (p.z ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
+    hipLaunchKernelGGL(k, dim3((unsigned)g.units), dim3(64 * kWaves), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
+}
+
+size_t workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype) {
+    if (batch <= 0 || seqlen <= 0 || dim <= 0 || (dtype != HX_F32 && dtype != HX_BF16)) return 0;
+    const Shape g(batch, seqlen, dim);
+    return g.fits() ? g.workspace() : 0;
 }
 
 }  // namespace
 }  // namespace hx
 
-extern "C" size_t hx_gated_scan_workspace_size(int64_t, int64_t, int64_t, int) { return 0; }
-extern "C" size_t hx_gated_scan_bwd_workspace_size(int64_t, int64_t, int64_t, int) { return 0; }
+extern "C" size_t hx_gated_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype) {
+    return hx::workspace_size(batch, seqlen, dim, dtype);
+}
+extern "C" size_t hx_gated_scan_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype) {
+    return hx::workspace_size(batch, seqlen, dim, dtype);
+}
 
 extern "C" int hx_gated_scan_fwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, const void* x, const void* f,
                                  const void* z, const float* init_state, void* out, float* last_state, float* states,
@@ -162,15 +513,17 @@ extern "C" int hx_gated_scan_fwd(int64_t batch, int64_t seqlen, int64_t dim, int
     HX_REQUIRE(batch >= 0 && seqlen >= 0 && dim >= 0, HX_ERR_INVALID_DIMENSION, "gated_scan: negative size");
     HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, HX_ERR_DTYPE_MISMATCH, "gated_scan: dtype %d", dtype);
     if (batch == 0 || dim == 0) return HX_OK;
-    HX_REQUIRE(sizes_fit(batch, seqlen, dim), HX_ERR_UNSUPPORTED, "gated_scan: too many elements");
-    const size_t need = hx_gated_scan_workspace_size(batch, seqlen, dim, dtype);
+    const Shape g(batch, seqlen, dim);
+    HX_REQUIRE(g.fits(), HX_ERR_UNSUPPORTED, "gated_scan: too many elements");
+    const size_t need = g.workspace();
     hipStream_t s = as_stream(stream);
     if (seqlen == 0) return copy_state(batch * dim, init_state, last_state, s);
     HX_REQUIRE(x && f && out, HX_ERR_INVALID_INPUT, "gated_scan: x, f and out are required");
     HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), HX_ERR_INVALID_INPUT,
                "gated_scan: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
-    return dtype == HX_F32 ? fwd<float>(batch, seqlen, dim, x, f, z, init_state, out, last_state, states, s)
-                           : fwd<uint16_t>(batch, seqlen, dim, x, f, z, init_state, out, last_state, states, s);
+    if (int rc = clear_chain(g, workspace, s)) return rc;
+    const FwdArgs p{seqlen, dim, x, f, z, init_state, out, last_state, states, (uint32_t)g.cols, g.chain(workspace)};
+    return dtype == HX_F32 ? fwd<float>(g, p, s) : fwd<uint16_t>(g, p, s);
 }
 
 extern "C" int hx_gated_scan_bwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, const void* x, const void* f,
@@ -180,8 +533,9 @@ extern "C" int hx_gated_scan_bwd(int64_t batch, int64_t seqlen, int64_t dim, int
     HX_REQUIRE(batch >= 0 && seqlen >= 0 && dim >= 0, HX_ERR_INVALID_DIMENSION, "gated_scan_bwd: negative size");
     HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, HX_ERR_DTYPE_MISMATCH, "gated_scan_bwd: dtype %d", dtype);
     if (batch == 0 || dim == 0) return HX_OK;
-    HX_REQUIRE(sizes_fit(batch, seqlen, dim), HX_ERR_UNSUPPORTED, "gated_scan_bwd: too many elements");
-    const size_t need = hx_gated_scan_bwd_workspace_size(batch, seqlen, dim, dtype);
+    const Shape g(batch, seqlen, dim);
+    HX_REQUIRE(g.fits(), HX_ERR_UNSUPPORTED, "gated_scan_bwd: too many elements");
+    const size_t need = g.workspace();
     hipStream_t s = as_stream(stream);
     if (seqlen == 0) return copy_state(batch * dim, dlast, dinit, s);
     HX_REQUIRE(x && f && states && dout && dx && df, HX_ERR_INVALID_INPUT,
@@ -189,9 +543,9 @@ extern "C" int hx_gated_scan_bwd(int64_t batch, int64_t seqlen, int64_t dim, int
     HX_REQUIRE((z == nullptr) == (dz == nullptr), HX_ERR_INVALID_INPUT, "gated_scan_bwd: dz goes with z");
     HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), HX_ERR_INVALID_INPUT,
                "gated_scan_bwd: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
-    return dtype == HX_F32
-               ? bwd<float>(batch, seqlen, dim, x, f, z, states, dout, dlast, dx, df, dz, dinit, s)
-               : bwd<uint16_t>(batch, seqlen, dim, x, f, z, states, dout, dlast, dx, df, dz, dinit, s);
+    if (int rc = clear_chain(g, workspace, s)) return rc;
+    const BwdArgs p{seqlen, dim, x, f, z, dout, states, dlast, dx, df, dz, dinit, (uint32_t)g.cols, g.chain(workspace)};
+    return dtype == HX_F32 ? bwd<float>(g, p, s) : bwd<uint16_t>(g, p, s);
 }
 
 extern "C" int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, const void* x, const void* f,
@@ -200,7 +554,7 @@ extern "C" int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, floa
     HX_REQUIRE(batch >= 0 && dim >= 0, HX_ERR_INVALID_DIMENSION, "gated_state_update: negative size");
     HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, HX_ERR_DTYPE_MISMATCH, "gated_state_update: dtype %d", dtype);
     if (batch == 0 || dim == 0) return HX_OK;
-    HX_REQUIRE(sizes_fit(batch, 1, dim), HX_ERR_UNSUPPORTED, "gated_state_update: too many elements");
+    HX_REQUIRE((__int128)batch * dim < (__int128)256 * kMaxBlocks, HX_ERR_UNSUPPORTED, "gated_state_update: too many elements");
     HX_REQUIRE(state && x && f && out, HX_ERR_INVALID_INPUT, "gated_state_update: state, x, f and out are required");
     const int64_t n = batch * dim;
     dim3 grid((unsigned)((n + 255) / 256));

@@ -208,8 +208,15 @@ def test_closed_and_open_gates(dev, dtype):
     got = {k: None if v is None else v.float().cpu() for k, v in run(dev, x).items()}
     for v in got.values():
         assert v is None or torch.isfinite(v).all()
+    # Through the held steps the true state is one number h, that of step 99. Steps with a = 1 and i x = 0 multiply by
+    # one and add nothing, exactly, alone or grouped, so each output there is some grouping of the steps up to 99: within
+    # that step's bound of h (as step 99's own output is), plus half a step of storage each.
+    ref = {k: f64(x[k]) for k in ("x", "f", "z", "init")}
+    o = oracle_fwd(**{k: v if v is None or v.ndim < 3 else v[:, :100] for k, v in ref.items()})
     for c in (0, 2):
-        assert torch.equal(got["out"][0, 100:400, c], got["out"][0, 99, c].expand(300))
+        h = float(o["out"][0, 99, c])
+        tol = 2 * float(o["out_E"][0, 99, c]) + 2 * HALF[dtype] * abs(h)
+        assert (got["out"][0, 100:400, c] - got["out"][0, 99, c]).abs().max() <= tol
         assert (got["dx"][0, 100:400, c] == 0).all() and (got["df"][0, 100:400, c] == 0).all()
     for c in (1, 3):
         assert got["out"][0, 300, c] == x["x"][0, 300, c].float()
