@@ -9,12 +9,11 @@ namespace {
 // Both gates from one exponential of -|f|, which is at most 1: neither overflows, and the smaller of
 // the two is a product, so it keeps its relative accuracy where the other rounds to 1. A state's decay
 // over n steps is a product of n gates, in which the reciprocal's error of up to an ulp, always to the
-// same side for neighbouring values, would add up: one Newton step, with the rounding error d of 1 + e
-// (exact, as e <= 1), leaves that of the last rounding alone.
+// same side for neighbouring values, would add up: one Newton step leaves that of the last rounding.
 __device__ inline void gates(float f, float& a, float& i) {
     const float e = fast_exp2(-fabsf(f) * kLog2e);
-    const float u = 1.0f + e, d = e - (u - 1.0f), q = fast_rcp(u);
-    const float r = fmaf(q, fmaf(-u, q, 1.0f) - d * q, q), s = e * r;
+    const float u = 1.0f + e, q = fast_rcp(u);
+    const float r = fmaf(q, fmaf(-u, q, 1.0f), q), s = e * r;
     a = f >= 0.0f ? r : s;
     i = f >= 0.0f ? s : r;
 }
@@ -46,6 +45,7 @@ template <> struct Pair<float> {
     __device__ static inline float lo(raw r) { return r.x; }
     __device__ static inline float hi(raw r) { return r.y; }
     __device__ static inline void store(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+    __device__ static inline void hold(raw& r) { asm("" : "+v"(r.x), "+v"(r.y)); }
 };
 template <> struct Pair<uint16_t> {
     using raw = uint32_t;
@@ -56,6 +56,8 @@ template <> struct Pair<uint16_t> {
     __device__ static inline void store(uint16_t* p, float a, float b) {
         *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(a, b);
     }
+    // Keeps the stored form in registers: what was computed from it before is not carried along to be used again.
+    __device__ static inline void hold(raw& r) { asm("" : "+v"(r)); }
 };
 
 // Where a lane's elements lie. VEC: even dim and pairs aligned to a wide load.
@@ -112,7 +114,6 @@ struct Chain {
     uint32_t lanes;  // sequences x column tiles
 };
 constexpr uint32_t kAbsent = 0xffffffffu, kNaN = 0x7fc00000u;
-constexpr int kWindow = 8;  // tiles that one look back covers
 // A wait ends by itself where the workspace is misused (two calls at once): some 10^5 looks of about a microsecond.
 constexpr int kLooks = 1 << 17;
 
@@ -131,7 +132,9 @@ __device__ inline void publish_exit(const Chain& c, int k, uint32_t col, int lan
 }
 
 // The state that tile k of a chain starts from; `first` is the chain's own. An exit state is its tile's map applied
-// to its entry state, whoever applies it, so the bits do not depend on which words were there.
+// to its entry state, whoever applies it, so the bits do not depend on which words were there. One look covers
+// kWindow tiles, all of its words in flight at once.
+template <int kWindow>
 __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int lane, float first) {
     float e = first;
     bool have = k == 0;
@@ -242,7 +245,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_fwd_kernel(const FwdArgs
         float e = in && p.init ? p.init[r] : 0.0f;
         if (p.chain.tiles > 1) {
             if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, H);
-            e = entry_of(p.chain, k, col, lane, e);
+            e = entry_of<8>(p.chain, k, col, lane, e);
             if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, H));
         }
         if (in && p.states) p.states[(b * p.chain.tiles + k) * p.D + c0 + lane] = e;
@@ -338,9 +341,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
             A *= m;
         }
         float e = in && p.dlast ? p.dlast[r] : 0.0f;
+        // fp32 keeps twice the registers for its operands: a window of 8 would spill
         if (p.chain.tiles > 1) {
             if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, G);
-            e = entry_of(p.chain, k, col, lane, e);
+            e = entry_of<sizeof(T) == 4 ? 4 : 8>(p.chain, k, col, lane, e);
             if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, G));
         }
         if (in && p.dinit && tile == 0) p.dinit[r] = fmaf(A, e, G);
@@ -360,6 +364,12 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
         }
     }
     __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        Pair<T>::hold(rx[j]);
+        Pair<T>::hold(rd[j]);
+        if (GATE) Pair<T>::hold(rz[j]);
+    }
     const float2 eh = *reinterpret_cast<const float2*>(&maps_h[part][c]);
     const float2 eg = *reinterpret_cast<const float2*>(&maps_g[part][c]);
     // dout and z were kept as stored, and silu(z) is formed again with its derivative: 32 registers less at the wait
