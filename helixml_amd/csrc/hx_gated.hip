@@ -103,32 +103,33 @@ struct Place {
     }
 };
 
-// The workspace: a ticket, then for each tile and channel its map (A, H) as one 64-bit word and its exit state as
-// one 32-bit word. A word of all ones is not there yet: every word is written once, whole, and carries its own
-// readiness, so no fence is needed, only that readers and writers meet beyond the L2 of their XCD (agent scope).
+// The workspace: a ticket, then one 64-bit word for each tile and channel: all ones while there is nothing, then the
+// tile's map (A, H), then its exit state (kExit, h). Each word is written whole and says itself what it is, so no fence
+// is needed, only that readers and writers meet beyond the L2 of their XCD (agent scope).
 struct Chain {
     uint32_t* ticket;
-    unsigned long long* maps;
-    uint32_t* exits;
+    unsigned long long* words;
     int tiles;       // of one sequence
     uint32_t lanes;  // sequences x column tiles
 };
-constexpr uint32_t kAbsent = 0xffffffffu, kNaN = 0x7fc00000u;
+constexpr unsigned long long kAbsent = ~0ull;
+constexpr uint32_t kExit = 0xfffffffeu, kNaN = 0x7fc00000u;
 // A wait ends by itself where the workspace is misused (two calls at once): some 10^5 looks of about a microsecond.
 constexpr int kLooks = 1 << 17;
 
-__device__ inline uint32_t word_of(float v) {
-    const uint32_t u = __float_as_uint(v);
-    return u == kAbsent ? kNaN : u;
-}
 // The first word of tile k in a column: uniform, so that a lane's part of an address is its number.
-__device__ inline size_t row_of(const Chain& c, int k, uint32_t col) { return ((size_t)k * c.lanes + col) * kWidth; }
+__device__ inline unsigned long long* words_of(const Chain& c, int k, uint32_t col) {
+    return c.words + ((size_t)k * c.lanes + col) * kWidth;
+}
+__device__ inline void publish(unsigned long long* word, uint32_t lo, float hi) {
+    __hip_atomic_store(word, (unsigned long long)__float_as_uint(hi) << 32 | lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 __device__ inline void publish_map(const Chain& c, int k, uint32_t col, int lane, float A, float H) {
-    __hip_atomic_store(c.maps + row_of(c, k, col) + lane, (unsigned long long)word_of(H) << 32 | word_of(A),
-                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t u = __float_as_uint(A);
+    publish(words_of(c, k, col) + lane, u >= kExit ? kNaN : u, H);  // no NaN passes for a tag
 }
 __device__ inline void publish_exit(const Chain& c, int k, uint32_t col, int lane, float v) {
-    __hip_atomic_store(c.exits + row_of(c, k, col) + lane, word_of(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    publish(words_of(c, k, col) + lane, kExit, v);
 }
 
 // The state that tile k of a chain starts from; `first` is the chain's own. An exit state is its tile's map applied
@@ -139,29 +140,23 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int lane, 
     float e = first;
     bool have = k == 0;
     for (int look = 0; look < kLooks && !__all(have); ++look) {
-        if (look) __builtin_amdgcn_s_sleep(2);
-        uint32_t s[kWindow];
+        if (look) __builtin_amdgcn_s_sleep(1);
         unsigned long long m[kWindow];
 #pragma unroll
         for (int i = 0; i < kWindow; ++i) {
             const int j = k - kWindow + i;
-            const size_t row = row_of(c, j < 0 ? 0 : j, col);
-            s[i] = __hip_atomic_load(c.exits + row + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            m[i] = __hip_atomic_load(c.maps + row + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            m[i] = __hip_atomic_load(words_of(c, j < 0 ? 0 : j, col) + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         float v = first;
         bool ok = k <= kWindow;  // the window reaches the chain's start
 #pragma unroll
         for (int i = 0; i < kWindow; ++i) {
             if (k - kWindow + i < 0) continue;
-            const float A = __uint_as_float((uint32_t)m[i]), H = __uint_as_float((uint32_t)(m[i] >> 32));
-            if (s[i] != kAbsent) {
-                v = __uint_as_float(s[i]);
-                ok = true;
-            } else {
-                v = fmaf(A, v, H);
-                ok = ok && m[i] != ~0ull;
-            }
+            const uint32_t lo = (uint32_t)m[i];
+            const float H = __uint_as_float((uint32_t)(m[i] >> 32));
+            const bool exit = lo == kExit;
+            ok = exit || (ok && m[i] != kAbsent);
+            v = exit ? H : fmaf(__uint_as_float(lo), v, H);
         }
         if (ok) {
             e = v;
@@ -196,7 +191,7 @@ struct FwdArgs {
 };
 
 template <typename T, bool VEC, bool GATE>
-__global__ __launch_bounds__(64 * kWaves, 4) void gated_fwd_kernel(const FwdArgs p) {
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void gated_fwd_kernel(const FwdArgs p) {
     __shared__ float2 maps[kParts][kWidth];
     __shared__ float entries[kParts][kWidth];
     __shared__ uint32_t shared_unit;
@@ -245,7 +240,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_fwd_kernel(const FwdArgs
         float e = in && p.init ? p.init[r] : 0.0f;
         if (p.chain.tiles > 1) {
             if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, H);
-            e = entry_of<8>(p.chain, k, col, lane, e);
+            e = entry_of<GATE && sizeof(T) == 2 ? 6 : 8>(p.chain, k, col, lane, e);
             if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, H));
         }
         if (in && p.states) p.states[(b * p.chain.tiles + k) * p.D + c0 + lane] = e;
@@ -341,10 +336,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
             A *= m;
         }
         float e = in && p.dlast ? p.dlast[r] : 0.0f;
-        // fp32 keeps twice the registers for its operands: a window of 8 would spill
         if (p.chain.tiles > 1) {
             if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, G);
-            e = entry_of<sizeof(T) == 4 ? 4 : 8>(p.chain, k, col, lane, e);
+            e = entry_of<8>(p.chain, k, col, lane, e);
             if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, G));
         }
         if (in && p.dinit && tile == 0) p.dinit[r] = fmaf(A, e, G);
@@ -411,7 +405,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
 __global__ __launch_bounds__(256) void gated_chain_clear_kernel(uint4* ws, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    const uint32_t v = i == 0 ? 0 : kAbsent;
+    const uint32_t v = i == 0 ? 0 : 0xffffffffu;
     ws[i] = make_uint4(v, v, v, v);
 }
 
@@ -447,12 +441,10 @@ struct Shape {
         return batch < kMaxBlocks && D < (1 << 26) && L < ((int64_t)1 << 37) &&
                (__int128)batch * cols * (tiles > 0 ? tiles : 1) < kMaxBlocks && (__int128)batch * L * D < ((__int128)1 << 60);
     }
-    // 16 bytes for the ticket, a map (8 bytes) and an exit state (4) per tile and channel; one tile waits for nobody
-    size_t workspace() const { return tiles > 1 ? 16 + (size_t)units * kWidth * 12 : 0; }
+    // 16 bytes for the ticket, a word per tile and channel; one tile waits for nobody
+    size_t workspace() const { return tiles > 1 ? 16 + (size_t)units * kWidth * 8 : 0; }
     Chain chain(void* ws) const {
-        char* w = (char*)ws;
-        return Chain{(uint32_t*)w, (unsigned long long*)(w + 16), (uint32_t*)(w + 16 + (size_t)units * kWidth * 8), (int)tiles,
-                     (uint32_t)(batch * cols)};
+        return Chain{(uint32_t*)ws, (unsigned long long*)((char*)ws + 16), (int)tiles, (uint32_t)(batch * cols)};
     }
 };
 
