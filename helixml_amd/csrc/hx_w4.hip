@@ -2,6 +2,7 @@
 #include <cmath>
 
 #include "hx_common.h"
+#include "hx_wave.h"
 
 namespace hx {
 namespace {
@@ -15,9 +16,12 @@ __host__ __device__ inline int64_t scales_row(int64_t K) { return (groups_of(K) 
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWindow = 128;  // elements of K that one 16-byte load per lane covers for 16 rows
-constexpr int kAhead = 4;     // windows whose weights are in flight at once
+constexpr int kAhead = 4;     // windows whose weights are in flight at once, and whose scales one load covers
+constexpr int kRowsAtOnce = 32;  // rows of X that one block takes at most
+constexpr int kXRow = 2 * kWindow + 16;  // bytes from one staged row of X to the next
 
 struct W4Args {
     int64_t M, N, K, ldx, ldy;
@@ -25,7 +29,7 @@ struct W4Args {
     const uint8_t *W, *S;
     const float* bias;
     void* Y;
-    int act, windows, per;  // windows of K, and how many a wave takes
+    int act, windows, per, waves;  // windows of K, how many a wave takes, the waves of a block
 };
 
 // Eight codes of a group at its scale as bf16: exact (one significant bit and a power of two), two codes an instruction.
@@ -42,31 +46,45 @@ __device__ inline bf16x8 expand8(uint32_t q, float scale) {
     return u.v;
 }
 
-// A block computes 16 NT outputs of 16 MT rows of X, its waves a run of windows each. Lane (n, j) of a wave holds row n's
-// group j of a window, 32 codes in one 16-byte load under one scale; the matrix instruction i of four takes the codes
-// 8i..8i+7 of all four groups, and X's elements at the same places as its other operand (K may be summed in any order).
-// With the scale inside the expanded weights the groups need no sums of their own. XVEC: 16-byte aligned rows of X.
-template <int NT, int MT, bool XVEC, typename TO>
-__global__ __launch_bounds__(1024) void linear_w4_kernel(const W4Args p) {
-    extern __shared__ float sums[];  // [waves][NT][MT][16 m][16 n]
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+// A block takes 16 NT outputs of at most 4 XR rows of X, its waves a run of windows each. What a wave loads is laid out by
+// memory, since the L1 looks up one line a clock and lanes that each sit in a row of their own cost 64 looks a load (47 us
+// instead of 34.5 at 5 x 32768 x 8192, whatever the loads in flight), and brought to the matrix instruction's order:
+//   weights  lane 4n + j holds row n's group j of a window, 32 codes in 16 bytes. A lane permutation gives (n, j) its
+//            place 16j + n, four register swaps turn (lane j, word i) into (lane i, word j), after which instruction i
+//            of four takes group i, eight codes a lane under one scale (with the scale inside the expanded weights the
+//            groups need no sums of their own);
+//   X        16 lanes read a row's 256 bytes of the window and leave them in the wave's own LDS rows, 16 bytes apart
+//            from a power of two, so that 16 rows read at one place of theirs meet all banks.
+// XVEC: 16-byte aligned rows of X.
+template <int NT, int XR, bool XVEC, typename TO>
+__global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
+    constexpr int MT = XR < 4 ? 1 : XR / 4, kRows = 4 * XR;  // column tiles of 16, rows of X that are staged
+    extern __shared__ float lds[];  // first the waves' rows of X, then [waves][NT][MT][16 m][16 n] sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, j = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * kRows;
     const int64_t G = groups_of(p.K), pr = packed_row(p.K), sr = scales_row(p.K);
-    // rows behind the last read the last one; what they give is not stored
-    const uint8_t *w[NT], *s[NT];
+    // Rows behind the last read the last one; what they give is not stored. A lane's part of an address is a 32-bit offset
+    // from a uniform place.
+    const uint8_t *const wb = p.W + n0 * pr, *const sb = p.S + n0 * sr;
+    uint32_t w[NT], s[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int64_t n = n0 + 16 * t + r < p.N ? n0 + 16 * t + r : p.N - 1;
-        w[t] = p.W + n * pr + 16 * j;
-        s[t] = p.S + n * sr + j;
+        const int64_t row = 16 * t + lane / 4, inside = n0 + row < p.N ? row : p.N - 1 - n0;
+        w[t] = (uint32_t)(inside * pr) + 16 * (lane % 4);
+        s[t] = (uint32_t)(inside * sr);
     }
-    const uint16_t* x[MT];
+    const int place = (4 * r + j) * 4;  // the lane that loaded (r, j), in bytes
+    char* const xrow = (char*)lds + wave * (kRows * kXRow);
+    const int64_t rows = p.M - m0 < kRows ? p.M - m0 : kRows;
+    const int rows_in = (int)rows;
+    const uint16_t* const xb = p.X + m0 * p.ldx;
+    uint32_t x[XR];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int64_t m = m0 + 16 * t + r < p.M ? m0 + 16 * t + r : p.M - 1;
-        x[t] = p.X + m * p.ldx + 32 * j;
-    }
+    for (int t = 0; t < XR; ++t) x[t] = (uint32_t)((4 * t + j < rows_in ? 4 * t + j : rows_in - 1) * p.ldx) + 8 * r;
+    const char* xread[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xread[t] = xrow + (16 * t + r < rows_in ? 16 * t + r : rows_in - 1) * kXRow + 16 * j;
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int a = 0; a < NT; ++a)
@@ -74,39 +92,75 @@ __global__ __launch_bounds__(1024) void linear_w4_kernel(const W4Args p) {
         for (int b = 0; b < MT; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
     uint32_t top[NT] = {};  // the largest scale byte of each row: 255 is not a number
 
-    const auto load_x = [&](int t, int64_t k, int i, bool whole) {
-        const uint16_t* at = x[t] + k + 8 * i;
-        union {
-            uint4 v;
-            uint16_t e[8];
-        } u;
-        if (XVEC && whole) {
-            u.v = *reinterpret_cast<const uint4*>(at);
-        } else {
-            const int64_t left = p.K - (k + 32 * j + 8 * i);  // elements from K on count as zero
+    const auto load_x = [&](int at, u32x4 (&o)[XR]) {
+        const uint16_t* from = xb + (int64_t)at * kWindow;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u.e[e] = whole || e < left ? at[e] : 0;
-        }
-        return __builtin_bit_cast(bf16x8, u.v);
+        for (int t = 0; t < XR; ++t) o[t] = *reinterpret_cast<const u32x4*>(from + x[t]);
     };
-    const auto window = [&](int64_t k, const uint4 (&q)[NT], const uint32_t (&sb)[NT], bool whole) {
-        float scale[NT];
+    // A wave's own rows, and its LDS accesses keep their order: no barrier, and the registers are free for the next window.
+    const auto stage = [&](const u32x4 (&xs)[XR]) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            scale[t] = __uint_as_float(sb[t] << 23);
-            top[t] = sb[t] > top[t] ? sb[t] : top[t];
+        for (int t = 0; t < XR; ++t) *reinterpret_cast<u32x4*>(xrow + (4 * t + j) * kXRow + 16 * r) = xs[t];
+    };
+    // Element by element: rows of any alignment, and the window that K ends in, elements from K on as zero.
+    const auto stage_any = [&](int at) {
+        const int64_t left = p.K - (int64_t)at * kWindow - 8 * r;
+        for (int row = j; row < rows_in; row += 4) {
+            const uint16_t* from = xb + row * p.ldx + (int64_t)at * kWindow + 8 * r;
+            union {
+                u32x4 v;
+                uint16_t e[8];
+            } u;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u.e[e] = e < left ? from[e] : 0;
+            *reinterpret_cast<u32x4*>(xrow + row * kXRow + 16 * r) = u.v;
+        }
+    };
+    const auto load_w = [&](int at, bool in, u32x4 (&o)[NT]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            o[t] = in ? *reinterpret_cast<const u32x4*>(wb + (int64_t)at * (kWindow / 2) + w[t]) : u32x4{0, 0, 0, 0};
+    };
+    // lane 4n + u: the four scale bytes of row n's window at + u
+    const int last = (int)(sr / 4) - 1;
+    const auto load_s = [&](int at, uint32_t (&o)[NT]) {
+        const int word = at + lane % 4 < last ? at + lane % 4 : last;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t] = *reinterpret_cast<const uint32_t*>(sb + (s[t] + word * 4));
+    };
+    const auto multiply = [&](const u32x4 (&q)[NT], const uint32_t (&sc)[NT], int u, int groups_in) {
+        const auto moved = [&](uint32_t v) { return __int_as_float(__builtin_amdgcn_ds_bpermute(place, (int)v)); };
+        float c[NT][4];
+        uint32_t scales[NT];
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+            c[a][0] = moved(q[a].x);
+            c[a][1] = moved(q[a].y);
+            c[a][2] = moved(q[a].z);
+            c[a][3] = moved(q[a].w);
+            swap32(c[a][0], c[a][2]);
+            swap32(c[a][1], c[a][3]);
+            swap16(c[a][0], c[a][1]);
+            swap16(c[a][2], c[a][3]);
+            scales[a] = (uint32_t)__builtin_amdgcn_ds_bpermute((4 * r + u) * 4, (int)sc[a]);
+            if (groups_in < 4) {  // groups that are not there have no weights and a scale of one
+                const uint32_t kept = 0xffffffffu >> (8 * (4 - groups_in));
+                scales[a] = (scales[a] & kept) | (0x7f7f7f7fu & ~kept);
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            bf16x8 xb[MT];
+            bf16x8 xv[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xb[t] = load_x(t, k, i, whole);
+            for (int b = 0; b < MT; ++b) xv[b] = *reinterpret_cast<const bf16x8*>(xread[b] + 64 * i);
 #pragma unroll
             for (int a = 0; a < NT; ++a) {
-                const uint32_t c = i == 0 ? q[a].x : i == 1 ? q[a].y : i == 2 ? q[a].z : q[a].w;
-                const bf16x8 wv = expand8(c, scale[a]);
+                const uint32_t scale = scales[a] >> (8 * i) & 255;
+                top[a] = scale > top[a] ? scale : top[a];
+                const bf16x8 wv = expand8(__float_as_uint(c[a][i]), __uint_as_float(scale << 23));
 #pragma unroll
-                for (int b = 0; b < MT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xb[b], acc[a][b], 0, 0, 0);
+                for (int b = 0; b < MT; ++b)
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[b], acc[a][b], 0, 0, 0);
             }
         }
     };
@@ -114,29 +168,67 @@ __global__ __launch_bounds__(1024) void linear_w4_kernel(const W4Args p) {
     int at = wave * p.per;
     const int end = at + p.per < p.windows ? at + p.per : p.windows;
     const int whole = (int)(p.K / kWindow) < end ? (int)(p.K / kWindow) : end;
-    for (; at + kAhead <= whole; at += kAhead) {
-        uint4 q[kAhead][NT];
-        uint32_t sb[kAhead][NT];
+    if (at + kAhead <= whole) {
+        // a ring of kAhead windows of weights: the one that was multiplied makes room for the one kAhead later. X comes
+        // one window ahead, asked for before the weights that follow it: loads return in order.
+        u32x4 q[kAhead][NT], xs[XR];
+        uint32_t sc[NT];
+        load_s(at, sc);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
+        for (int u = 0; u < kAhead; ++u) load_w(at + u, true, q[u]);
+        if (XVEC) load_x(at, xs);
+        for (; at + 2 * kAhead <= whole; at += kAhead) {
+            uint32_t after[NT];
+            load_s(at + kAhead, after);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                q[u][t] = *reinterpret_cast<const uint4*>(w[t] + (int64_t)(at + u) * (kWindow / 2));
-                sb[u][t] = s[t][(at + u) * 4];
+            for (int u = 0; u < kAhead; ++u) {
+                if (XVEC) {
+                    stage(xs);
+                    load_x(at + u + 1, xs);
+                } else {
+                    stage_any(at + u);
+                }
+                u32x4 now[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) now[t] = q[u][t];
+                load_w(at + u + kAhead, true, q[u]);
+                multiply(now, sc, u, 4);
             }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) window((int64_t)(at + u) * kWindow, q[u], sb[u], true);
-    }
-    for (; at < end; ++at) {
-        uint4 q[NT];
-        uint32_t sb[NT];
-        const bool in = at < whole || at * 4 + j < G;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            q[t] = in ? *reinterpret_cast<const uint4*>(w[t] + (int64_t)at * (kWindow / 2)) : make_uint4(0, 0, 0, 0);
-            sb[t] = in ? s[t][at * 4] : 127;
+            for (int t = 0; t < NT; ++t) sc[t] = after[t];
         }
-        window((int64_t)at * kWindow, q, sb, at < whole);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (XVEC) {
+                stage(xs);
+                if (u + 1 < kAhead) load_x(at + u + 1, xs);
+            } else {
+                stage_any(at + u);
+            }
+            multiply(q[u], sc, u, 4);
+        }
+        at += kAhead;
+    }
+    if (at < end) {  // at most kAhead windows, the last of K perhaps not whole
+        u32x4 q[kAhead][NT];
+        uint32_t sc[NT];
+        load_s(at, sc);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (at + u < end) load_w(at + u, (at + u) * 4 + lane % 4 < G, q[u]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (at + u >= end) break;
+            const int left = (int)(G - (int64_t)(at + u) * 4);
+            if (XVEC && at + u < whole) {
+                u32x4 xs[XR];
+                load_x(at + u, xs);
+                stage(xs);
+            } else {
+                stage_any(at + u);
+            }
+            multiply(q[u], sc, u, left < 4 ? left : 4);
+        }
     }
     // a scale that is not a number makes its whole row one: NaN * 0 added to it
 #pragma unroll
@@ -149,21 +241,22 @@ __global__ __launch_bounds__(1024) void linear_w4_kernel(const W4Args p) {
             for (int b = 0; b < MT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, zero, acc[a][b], 0, 0, 0);
         }
 
+    __syncthreads();
     // The waves' sums in the order of K, then the epilogue; lane (m = r, 4j..4j+3) holds four outputs of a row of X.
 #pragma unroll
     for (int a = 0; a < NT; ++a)
 #pragma unroll
         for (int b = 0; b < MT; ++b)
-            *reinterpret_cast<f32x4*>(sums + ((wave * NT + a) * MT + b) * 256 + r * 16 + 4 * j) = acc[a][b];
+            *reinterpret_cast<f32x4*>(lds + ((wave * NT + a) * MT + b) * 256 + r * 16 + 4 * j) = acc[a][b];
     __syncthreads();
     TO* y = (TO*)p.Y;
     for (int o = threadIdx.x; o < NT * MT * 256; o += blockDim.x) {
         const int a = o / 16 % NT, row = o / (16 * NT);  // consecutive threads take consecutive outputs
         const int64_t n = n0 + 16 * a + o % 16, m = m0 + row;
         if (n >= p.N || m >= p.M) continue;
-        const float* at_o = sums + (a * MT + row / 16) * 256 + row % 16 * 16 + o % 16;
+        const float* at_o = lds + (a * MT + row / 16) * 256 + row % 16 * 16 + o % 16;
         float v = 0.0f;
-        for (int k = 0; k < waves; ++k) v += at_o[k * NT * MT * 256];
+        for (int k = 0; k < p.waves; ++k) v += at_o[k * NT * MT * 256];
         if (p.bias) v += p.bias[n];
         if (p.act & 1) v = silu(v);
         TO* to = y + m * p.ldy + n;
@@ -172,12 +265,16 @@ __global__ __launch_bounds__(1024) void linear_w4_kernel(const W4Args p) {
     }
 }
 
-template <int NT, int MT>
-int launch_w4(const W4Args& p, int waves, bool xvec, bool f32, hipStream_t s) {
-    const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
-    const auto k = f32 ? (xvec ? linear_w4_kernel<NT, MT, true, float> : linear_w4_kernel<NT, MT, false, float>)
-                       : (xvec ? linear_w4_kernel<NT, MT, true, uint16_t> : linear_w4_kernel<NT, MT, false, uint16_t>);
-    hipLaunchKernelGGL(k, grid, dim3(64 * waves), (size_t)waves * NT * MT * 256 * sizeof(float), s, p);
+template <int NT, int XR>
+int launch_w4(const W4Args& p, bool xvec, bool f32, hipStream_t s) {
+    const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)), (unsigned)((p.M + 4 * XR - 1) / (4 * XR)));
+    const auto k = f32 ? (xvec ? linear_w4_kernel<NT, XR, true, float> : linear_w4_kernel<NT, XR, false, float>)
+                       : (xvec ? linear_w4_kernel<NT, XR, true, uint16_t> : linear_w4_kernel<NT, XR, false, uint16_t>);
+    constexpr size_t staged = 4 * XR * kXRow, summed = NT * (XR < 4 ? 1 : XR / 4) * 256 * sizeof(float);
+    const size_t bytes = p.waves * (staged > summed ? staged : summed);
+    HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 0), HX_ERR_UNSUPPORTED,
+               "linear_w4: %zu bytes of LDS are not granted", bytes);
+    hipLaunchKernelGGL(k, grid, dim3((unsigned)(64 * p.waves)), bytes, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
@@ -235,16 +332,25 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
                "linear_w4: X, packed, scales and Y required, ldx >= K, ldy >= N");
     HX_REQUIRE(aligned(packed, 16) && aligned(scales, 16), HX_ERR_INVALID_INPUT,
                "linear_w4: packed and scales must be 16-byte aligned");
-    HX_REQUIRE(N < ((int64_t)1 << 34) && M <= 16 * (int64_t)65535 && K < ((int64_t)1 << 31), HX_ERR_UNSUPPORTED,
-               "linear_w4: at most %d rows of X, 2^34 outputs and K below 2^31", 16 * 65535);
-    // How K is cut decides the order of the sums, so it goes by N and K alone: enough waves for every CU's 16 (256 CUs),
-    // none with less than one window.
+    HX_REQUIRE(N < ((int64_t)1 << 34) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26), HX_ERR_UNSUPPORTED,
+               "linear_w4: at most %d rows of X, 2^34 outputs and K below 2^26", kRowsAtOnce * 65535);
+    // How K is cut decides the order of the sums, so it goes by N and K alone: two waves a tile of 16 outputs, more, up to 8,
+    // while there are fewer than 8 for each of 256 CUs; none without a window. 1 x 2048 x 4096: 8 waves 4.4 us, 4 waves
+    // 4.7, 2 waves 6.1; 1 x 16384 x 2048: 2 waves 6.3, 4 waves 7.0; 5 x 32768 x 8192: 2 waves 34.5, 4 waves 38.7.
     const int windows = (int)((K + kWindow - 1) / kWindow);
     const int64_t tiles = (N + 15) / 16;
-    int waves = 1;
-    while (waves < 16 && waves * 2 <= windows && tiles * waves < 4096) waves *= 2;
+    int waves = windows > 1 ? 2 : 1;
+    while (waves < 8 && waves * 2 <= windows && tiles * waves < 2048) waves *= 2;
     const W4Args p{M, N, K, ldx, ldy, (const uint16_t*)X, (const uint8_t*)packed, (const uint8_t*)scales, bias, Y, act, windows,
-                   (windows + waves - 1) / waves};
-    const bool xvec = aligned(X, 16) && ldx % 8 == 0, f32 = out_dtype == HX_F32;
-    return launch_w4<1, 1>(p, waves, xvec, f32, as_stream(stream));
+                   (windows + waves - 1) / waves, waves};
+    const bool xvec = aligned(X, 16) && ldx % 8 == 0 && ldx < (1 << 26), f32 = out_dtype == HX_F32;
+    hipStream_t s = as_stream(stream);
+    // Two tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs, with few rows nothing.
+    // 5 x 32768 x 8192: 1 tile 37.5 us, 2 tiles 34.5; 16 x 8192 x 4096: 8.3 and 7.7; 64 x 16384 x 8192: 86 and 46;
+    // 1 x 16384 x 2048: 6.3 and 7.6; 8 x 8192 x 4096: 7.3 and 7.4; 24 x 4096 x 4096: 7.6 and 8.6.
+    const bool two = M > 8 ? tiles >= 512 : M > 4 && tiles >= 1024;
+    if (M <= 4) return launch_w4<1, 1>(p, xvec, f32, s);
+    if (M <= 8) return two ? launch_w4<2, 2>(p, xvec, f32, s) : launch_w4<1, 2>(p, xvec, f32, s);
+    if (M <= 16) return two ? launch_w4<2, 4>(p, xvec, f32, s) : launch_w4<1, 4>(p, xvec, f32, s);
+    return two ? launch_w4<2, 8>(p, xvec, f32, s) : launch_w4<1, 8>(p, xvec, f32, s);
 }

@@ -92,7 +92,8 @@ def test_linear_refusals():
 
 # ------------------------------------------------------------------ products (device)
 SIZES = [(1, 1, 1), (1, 16, 32), (1, 17, 33), (2, 5, 64), (3, 100, 31), (1, 256, 512), (5, 160, 4096), (16, 64, 128), (17, 48, 96),
-         (33, 70, 1000), (64, 130, 544), (65, 33, 256), (130, 40, 160), (1, 1000, 2080), (7, 4100, 512), (4, 300, 777)]
+         (33, 70, 1000), (64, 130, 544), (65, 33, 256), (130, 40, 160), (1, 1000, 2080), (7, 4100, 512), (4, 300, 777),
+         (2, 16400, 160), (6, 16390, 288), (16, 16400, 1100), (40, 16500, 640), (33, 16384, 96)]
 
 
 def random_weights(N, K, seed, lo=120, hi=130):
@@ -184,7 +185,7 @@ def test_not_a_number(dev):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N,K", [(160, 4096), (1000, 512), (4100, 2048), (33, 77)])
+@pytest.mark.parametrize("N,K", [(160, 4096), (1000, 512), (4100, 2048), (33, 77), (16400, 544)])
 def test_a_row_does_not_depend_on_the_batch(dev, N, K):
     packed, scales = (t.to(dev) for t in random_weights(N, K, 9))
     X = torch.randn(80, K).to(dev, torch.bfloat16)
