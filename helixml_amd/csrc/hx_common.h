@@ -118,6 +118,19 @@ template <> struct Storage<uint16_t> {
     __device__ static inline void store(uint16_t* p, float v) { *p = round(v); }
 };
 
+// N elements from any address that an element may have: rows of an odd vocabulary start anywhere, and global memory takes
+// wide accesses there.
+template <int N, typename T>
+struct Run {
+    T v[N];
+    __device__ static inline Run load(const T* p) {
+        Run r;
+        __builtin_memcpy(&r, p, sizeof(r));
+        return r;
+    }
+    __device__ inline void store(T* p) const { __builtin_memcpy(p, this, sizeof(*this)); }
+};
+
 __device__ inline float bf16_bits_to_f32(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 
 // Workgroup barrier that orders LDS only. __syncthreads() is a workgroup-scope fence over all

@@ -21,7 +21,7 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _ffi
-from .ssm import _STORAGE, _need, _on_stream_device, _ptr, _stream, keep_for_stream, on_launch_stream
+from .ssm import _STORAGE, _on_stream_device, _operands, _ptr, _stream, keep_for_stream, on_launch_stream
 
 _F32, _BF16 = _ffi.HX_F32, _ffi.HX_BF16
 
@@ -107,27 +107,25 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
             raise _ffi.ShapeMismatch(f"history: expected [batch, n], got {list(history.shape)}")
         n = history.shape[1]
         ldh = _rows(history, "history", (bt, n), torch.int32)
-    for name, t, dtype in (("lengths", lengths, torch.int32), ("prompt_lengths", prompt_lengths, torch.int32),
-                           ("repetition", repetition, torch.float32), ("frequency", frequency, torch.float32),
-                           ("presence", presence, torch.float32)):
-        _need(t, name, (bt,), dtype)
+    one, i32, f32 = (bt,), torch.int32, torch.float32
+    _operands(stream, ("lengths", lengths, one, i32), ("prompt_lengths", prompt_lengths, one, i32),
+              ("repetition", repetition, one, f32), ("frequency", frequency, one, f32), ("presence", presence, one, f32))
     words = -(-V // 32)
     ldb = lda = 0
     if bias is not None:
         if bias.dim() == 1:
-            _need(bias, "bias", (V,), torch.float32)
+            _operands(stream, ("bias", bias, (V,), f32))
         else:
-            ldb = _rows(bias, "bias", shape, torch.float32)
+            ldb = _rows(bias, "bias", shape, f32)
     if allowed is not None:
         if allowed.dim() == 1:
-            _need(allowed, "allowed", (words,), torch.int32)
+            _operands(stream, ("allowed", allowed, (words,), i32))
         else:
-            lda = _rows(allowed, "allowed", (bt, words), torch.int32)
+            lda = _rows(allowed, "allowed", (bt, words), i32)
     if out is None:
         out = torch.empty((bt, V), device=logits.device, dtype=logits.dtype)
     ldo = _rows(out, "out", shape, logits.dtype)
-    _on_stream_device(stream, logits=logits, history=history, lengths=lengths, prompt_lengths=prompt_lengths,
-                      repetition=repetition, frequency=frequency, presence=presence, bias=bias, allowed=allowed, out=out)
+    _on_stream_device(stream, logits=logits, history=history, bias=bias, allowed=allowed, out=out)
     _ffi.call("hx_logits_adjust", bt, V, _STORAGE[logits.dtype], _ptr(logits), ldl, _ptr(history), ldh, n,
               _ptr(lengths), _ptr(prompt_lengths), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias), ldb,
               _ptr(allowed), lda, _ptr(out), ldo, _stream(stream))

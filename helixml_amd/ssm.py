@@ -86,6 +86,16 @@ def _on_stream_device(launch, **tensors) -> None:
             raise DeviceMismatch(f"{name} is on {t.device}, the launch stream on {launch.device}")
 
 
+def _operands(launch, *specs) -> None:
+    """_need and _on_stream_device for (name, tensor, shape, dtype) in turn, at the cost of a few attribute reads where
+    nothing is wrong: a decode step's call is a few microseconds in all."""
+    device = launch.device
+    for name, t, shape, dtype in specs:
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous()):
+            _need(t, name, shape, dtype)
+            _on_stream_device(launch, **{name: t})
+
+
 def selective_scan_workspace_size(batch, seqlen, dim, dstate, dtype=torch.float32):
     """Bytes of scratch hx_selective_scan_fwd_ws needs (0 when the sequence is not segmented)."""
     return int(_ffi.lib().hx_selective_scan_workspace_size(batch, seqlen, dim, dstate, _STORAGE[dtype]))
@@ -212,15 +222,13 @@ def gated_scan_fwd(x, f, z=None, init_state=None, return_last_state=False, retur
     st = x.dtype
     if st not in _STORAGE:
         raise DTypeMismatch(f"x: storage dtype {st} is neither float32 nor bfloat16")
-    _need(x, "x", shape, st)
-    _need(f, "f", shape, st)
-    _need(z, "z", shape, st)
-    _need(init_state, "init_state", (bt, dim), torch.float32)
-    _need(out, "out", shape, st)
-    _on_stream_device(stream, x=x, f=f, z=z, init_state=init_state, out=out, workspace=workspace)
+    f32 = torch.float32
+    _operands(stream, ("x", x, shape, st), ("f", f, shape, st), ("z", z, shape, st), ("init_state", init_state, (bt, dim), f32),
+              ("out", out, shape, st))
+    if workspace is not None:
+        _on_stream_device(stream, workspace=workspace)
     if out is None:
         out = torch.empty_like(x)
-    f32 = torch.float32
     last = torch.empty((bt, dim), device=x.device, dtype=f32) if return_last_state else None
     states = torch.empty((bt, -(-L // GATED_CHUNK), dim), device=x.device, dtype=f32) if return_states else None
     workspace, nbytes = _gated_workspace("hx_gated_scan_workspace_size", workspace, bt, L, dim, st, x.device)
@@ -242,16 +250,14 @@ def gated_scan_bwd(x, f, dout, states, z=None, dlast=None, workspace=None, strea
     st = x.dtype
     if st not in _STORAGE:
         raise DTypeMismatch(f"x: storage dtype {st} is neither float32 nor bfloat16")
-    _need(x, "x", shape, st)
-    _need(f, "f", shape, st)
-    _need(z, "z", shape, st)
-    _need(dout, "dout", shape, st)
-    _need(states, "states", (bt, -(-L // GATED_CHUNK), dim), torch.float32)
-    _need(dlast, "dlast", (bt, dim), torch.float32)
-    _on_stream_device(stream, x=x, f=f, z=z, dout=dout, states=states, dlast=dlast, workspace=workspace)
+    f32 = torch.float32
+    _operands(stream, ("x", x, shape, st), ("f", f, shape, st), ("z", z, shape, st), ("dout", dout, shape, st),
+              ("states", states, (bt, -(-L // GATED_CHUNK), dim), f32), ("dlast", dlast, (bt, dim), f32))
+    if workspace is not None:
+        _on_stream_device(stream, workspace=workspace)
     dx, df = torch.empty_like(x), torch.empty_like(x)
     dz = None if z is None else torch.empty_like(x)
-    dinit = torch.empty((bt, dim), device=x.device, dtype=torch.float32)
+    dinit = torch.empty((bt, dim), device=x.device, dtype=f32)
     workspace, nbytes = _gated_workspace("hx_gated_scan_bwd_workspace_size", workspace, bt, L, dim, st, x.device)
     _ffi.call("hx_gated_scan_bwd", bt, L, dim, _STORAGE[st], _ptr(x), _ptr(f), _ptr(z), _ptr(states), _ptr(dout),
               _ptr(dlast), _ptr(dx), _ptr(df), _ptr(dz), _ptr(dinit), _ptr(workspace), nbytes, _stream(stream))
@@ -273,12 +279,8 @@ def gated_state_update(state, x, f, z=None, out=None, stream=None):
     shape, st = x.shape, x.dtype
     if st not in _STORAGE:
         raise DTypeMismatch(f"x: storage dtype {st} is neither float32 nor bfloat16")
-    _need(state, "state", shape, torch.float32)
-    _need(x, "x", shape, st)
-    _need(f, "f", shape, st)
-    _need(z, "z", shape, st)
-    _need(out, "out", shape, st)
-    _on_stream_device(stream, state=state, x=x, f=f, z=z, out=out)
+    _operands(stream, ("state", state, shape, torch.float32), ("x", x, shape, st), ("f", f, shape, st), ("z", z, shape, st),
+              ("out", out, shape, st))
     if out is None:
         out = torch.empty_like(x)
     _ffi.call("hx_gated_state_update", shape[0], shape[1], _STORAGE[st], _ptr(state), _ptr(x), _ptr(f), _ptr(z),
@@ -457,9 +459,8 @@ def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out
     if K > 1 and X.stride(1) != 1:
         raise InvalidInput("linear_w4: X needs unit column stride")
     pr, sr = _w4_rows(K)
-    _need(packed, "packed", (N, pr), torch.uint8)
-    _need(scales, "scales", (N, sr), torch.uint8)
-    _need(bias, "bias", (N,), torch.float32)
+    _operands(stream, ("packed", packed, (N, pr), torch.uint8), ("scales", scales, (N, sr), torch.uint8),
+              ("bias", bias, (N,), torch.float32))
     if out is None:
         if act & 2:
             raise InvalidInput("linear_w4: act bit 1 adds to out, which is not given")
@@ -472,7 +473,7 @@ def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out
         raise DTypeMismatch(f"out: {out.dtype} is neither float32 nor bfloat16")
     elif N > 1 and out.stride(1) != 1:
         raise InvalidInput("linear_w4: out needs unit column stride")
-    _on_stream_device(stream, X=X, packed=packed, scales=scales, bias=bias, out=out)
+    _on_stream_device(stream, X=X, out=out)
     # a single row has no stride: torch may report any
     _ffi.call("hx_linear_w4", M, N, K, _ptr(X), X.stride(0) if M > 1 else K, _ptr(packed), _ptr(scales), _ptr(bias),
               int(act), _STORAGE[out.dtype], _ptr(out), out.stride(0) if M > 1 else N, _stream(stream))
