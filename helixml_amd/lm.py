@@ -21,7 +21,8 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _ffi
-from .ssm import _STORAGE, _on_stream_device, _operands, _ptr, _stream, keep_for_stream, on_launch_stream
+from .ssm import (_STORAGE, _on_stream_device, _operands, _ptr, _stream, keep_for_stream,
+                  on_current_or_launch_stream, on_launch_stream)
 
 _F32, _BF16 = _ffi.HX_F32, _ffi.HX_BF16
 
@@ -80,7 +81,7 @@ def _rows(t, name, shape, dtype):
     return t.stride(0) if shape[0] > 1 else shape[1]
 
 
-@on_launch_stream
+@on_current_or_launch_stream
 def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repetition=None, frequency=None,
                   presence=None, bias=None, allowed=None, out=None, stream=None):
     """What a decode step does to its logits [batch, vocab] (fp32 or bf16) before a token is chosen

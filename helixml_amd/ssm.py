@@ -51,10 +51,36 @@ def on_launch_stream(fn):
     @functools.wraps(fn)
     def run(*args, stream=None, **kwargs):
         ts = _torch_stream(stream)
-        if stream is None:  # the current stream: nothing to switch
-            return fn(*args, stream=ts, **kwargs)
         with torch.cuda.stream(ts):
             return fn(*args, stream=ts, **kwargs)
+    run.on_launch_stream = True
+    return run
+
+
+class _CurrentStream:
+    """The current stream of a device as the wrappers below need it: its handle and its device. torch's own object for it
+    costs three microseconds to make, as much as a launch."""
+    __slots__ = ("cuda_stream", "device")
+
+    def __init__(self, handle, device):
+        self.cuda_stream, self.device = handle, device
+
+
+_DEVICES: dict = {}
+
+
+def on_current_or_launch_stream(fn):
+    """on_launch_stream for wrappers of a few microseconds that need no more of their stream than its handle and device:
+    with no stream given they run on the current one, where there is nothing to switch."""
+    switched = on_launch_stream(fn)
+
+    @functools.wraps(fn)
+    def run(*args, stream=None, **kwargs):
+        if stream is not None or not torch.cuda.is_initialized():
+            return switched(*args, stream=stream, **kwargs)
+        i = torch._C._cuda_getDevice()
+        device = _DEVICES.get(i) or _DEVICES.setdefault(i, torch.device("cuda", i))
+        return fn(*args, stream=_CurrentStream(torch._C._cuda_getCurrentRawStream(i), device), **kwargs)
     run.on_launch_stream = True
     return run
 
@@ -208,7 +234,7 @@ def _gated_workspace(name, given, batch, seqlen, dim, dtype, device):
     return (None, 0) if given is None else (given, given.numel() * given.element_size())
 
 
-@on_launch_stream
+@on_current_or_launch_stream
 def gated_scan_fwd(x, f, z=None, init_state=None, return_last_state=False, return_states=False, out=None,
                    workspace=None, stream=None):
     """Gated linear recurrence (hx_gated_scan_fwd): a = sigmoid(f), h_t = a_t h_{t-1} + (1 - a_t) x_t,
@@ -239,7 +265,7 @@ def gated_scan_fwd(x, f, z=None, init_state=None, return_last_state=False, retur
     return (out,) + ((last,) if return_last_state else ()) + ((states,) if return_states else ())
 
 
-@on_launch_stream
+@on_current_or_launch_stream
 def gated_scan_bwd(x, f, dout, states, z=None, dlast=None, workspace=None, stream=None):
     """Gradients of gated_scan_fwd (hx_gated_scan_bwd): (dx, df, dz, dinit) from dout [batch, L, dim] and
     dlast [batch, dim] fp32 (the last state's gradient; None: zero). x, f, z: the forward's inputs, states: what
@@ -270,7 +296,7 @@ def gated_scan_workspace_size(batch, seqlen, dim, dtype=torch.float32, backward=
     return int(getattr(_ffi.lib(), name)(batch, seqlen, dim, _STORAGE[dtype]))
 
 
-@on_launch_stream
+@on_current_or_launch_stream
 def gated_state_update(state, x, f, z=None, out=None, stream=None):
     """One token of the gated recurrence (hx_gated_state_update); advances ``state`` [batch, dim] fp32 in
     place. x, f, z, out: [batch, dim] fp32 or bf16."""
@@ -445,7 +471,7 @@ def w4_quantize(W, device=None):
     return torch.from_numpy(packed).to(device), torch.from_numpy(scales).to(device)
 
 
-@on_launch_stream
+@on_current_or_launch_stream
 def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=None):
     """Y = X . W^T (+ bias)(, SiLU) with 4-bit weights (hx_linear_w4). X [M, K] bf16 (rows may be strided);
     packed, scales: what w4_quantize gives for W [N, K]; bias [N] fp32. act: bit 0 SiLU, bit 1 adds to
