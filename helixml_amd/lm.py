@@ -7,7 +7,9 @@ that model, pre-norm with a residual stream:
 
     x = embed[tokens]                                    (fp32 residual stream)
     for each layer: x += MambaBlock(RMSNorm(x))          (hx_mamba_layer_fwd / _decode)
-    logits = RMSNorm_f(x) . W_head^T                     (hx_rmsnorm_fwd + hx_gemm_bf16)
+    logits = RMSNorm_f(x) . W_head^T                     (hx_rmsnorm_fwd + hx_gemm_bf16, or
+                                                          hx_linear_w4 after quantize_head)
+    what a decode step does to them before a token is chosen       (hx_logits_adjust)
 
 ``prefill`` runs whole sequences and returns the per-layer decode state (the scan's last state
 and the conv window); ``decode_step`` advances every sequence by one token from that state.
@@ -22,7 +24,7 @@ import torch
 
 from . import _ffi
 from .ssm import (_STORAGE, _on_stream_device, _operands, _ptr, _stream, keep_for_stream,
-                  on_current_or_launch_stream, on_launch_stream)
+                  linear_w4, on_current_or_launch_stream, on_launch_stream, w4_quantize)
 
 _F32, _BF16 = _ffi.HX_F32, _ffi.HX_BF16
 
@@ -174,9 +176,15 @@ class ByteLM:
             ))
         self.norm_f = torch.ones(dm, dtype=f32, device=self.device)
         self.w_head = lin(vocab, dm)
+        self.w_head4 = None
         self._ws: Optional[torch.Tensor] = None
 
     # ------------------------------------------------------------------ helpers
+    def quantize_head(self):
+        """Rounds the head's weights to 4 bits with group scales (ssm.w4_quantize): from then on prefill and decode
+        alike read them through hx_linear_w4, whose rows do not depend on how many there are."""
+        self.w_head4 = w4_quantize(self.w_head)
+
     def _workspace(self, batch, seqlen):
         need = int(_ffi.lib().hx_mamba_layer_workspace_size(batch, seqlen, self.d_model, self.d_inner,
                                                             self.dt_rank, self.d_state))
@@ -194,6 +202,9 @@ class ByteLM:
         rows = x.numel() // self.d_model
         xn = rmsnorm(x, self.norm_f, self.eps, out_dtype=torch.bfloat16, stream=stream)
         logits = torch.empty((*x.shape[:-1], self.vocab), device=self.device, dtype=torch.float32)
+        if self.w_head4 is not None:
+            linear_w4(xn.view(rows, self.d_model), *self.w_head4, out=logits.view(rows, self.vocab), stream=stream)
+            return logits
         _ffi.call("hx_gemm_bf16", rows, self.vocab, self.d_model, _ptr(xn), self.d_model,
                   _ptr(self.w_head), self.d_model, None, 0, _F32, _ptr(logits), self.vocab,
                   self.vocab, None, 0, self.vocab, None, 0, _stream(stream))
@@ -219,10 +230,11 @@ class ByteLM:
         return self._head(x, stream), state
 
     @on_launch_stream
-    def decode_step(self, tokens, state, stream=None, workspace=None):
+    def decode_step(self, tokens, state, stream=None, workspace=None, adjust=None):
         """tokens int32 [batch] -> logits fp32 [batch, vocab]; advances ``state`` in place.
         ``workspace`` (uint8 device tensor of at least hx_mamba_layer_workspace_size(batch, 1,
-        ...) bytes) replaces the model's shared workspace."""
+        ...) bytes) replaces the model's shared workspace. ``adjust``: keyword arguments of
+        adjust_logits (history, lengths, penalties, bias, allowed), applied to the logits in place."""
         bt = tokens.shape[0]
         x = embedding(tokens, self.embed, stream=stream)
         ws = self._workspace(bt, 1) if workspace is None else workspace
@@ -234,14 +246,17 @@ class ByteLM:
                       self.dt_rank, self.d_conv, _ptr(x), _ptr(p["norm_w"]), float(self.eps),
                       *[_ptr(p[k]) for k in LAYER_KEYS], _ptr(ssm_st), _ptr(conv_st), _ptr(ws),
                       ws.numel(), s)
-        return self._head(x, stream)
+        logits = self._head(x, stream)
+        return logits if adjust is None else adjust_logits(logits, **adjust, out=logits, stream=stream)
 
-    def decode_graph(self, state, stream=None):
+    def decode_graph(self, state, stream=None, adjust=None):
         """Captures one decode step for ``state``'s batch into a HIP graph (torch.cuda.CUDAGraph
         over the C ABI's launches: no host round trips, no allocations, no memsets in the step).
         Returns ``step(tokens) -> logits``: it copies the tokens into the graph's input buffer
         and replays; ``state`` is advanced in place exactly as by decode_step. The logits tensor
-        is the graph's output buffer, overwritten by the next replay."""
+        is the graph's output buffer, overwritten by the next replay. ``adjust`` as in decode_step:
+        the graph reads its tensors at every replay, so the caller updates them (the history, its
+        lengths, the allowed tokens) in place between replays."""
         bt = state[0][0].shape[0]
         tok = torch.zeros((bt,), dtype=torch.int32, device=self.device)
         # the graph's own workspace: the captured launches hold its raw address, so it must live
@@ -255,11 +270,11 @@ class ByteLM:
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            self.decode_step(tok, scratch, workspace=ws)
+            self.decode_step(tok, scratch, workspace=ws, adjust=adjust)
         torch.cuda.current_stream().wait_stream(side)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            logits = self.decode_step(tok, state, workspace=ws)
+            logits = self.decode_step(tok, state, workspace=ws, adjust=adjust)
 
         def step(tokens):
             tok.copy_(tokens)
@@ -270,6 +285,8 @@ class ByteLM:
         step.workspace = ws
         step.tokens = tok
         step.state = state
+        step.adjust = adjust
+        step.head = self.w_head4  # the captured launches hold these tensors' addresses
         return step
 
     def host_params(self):

@@ -11,8 +11,8 @@ Six kinds, each through a public entry point of ``helixml_amd``:
            bit-exact to the reference, or time-parallel for long sequences
   s4d      the diagonal complex S4D recurrence (``ssm.s4d_complex_fwd``)
 
-Value distributions are those of the repository's benchmark and tests. There is no backward in this
-framework: every case is a forward.
+Value distributions are those of the repository's benchmark and tests. Every case is a forward; the
+gated recurrence's backward pass is among the operators of ``perf/operators.py``.
 """
 import math
 
