@@ -1,7 +1,6 @@
 // hx_gated.hip — the gated linear recurrence with one state per channel: forward, backward, one token.
 //   a = sigmoid(f), i = sigmoid(-f);  h_t = a_t h_{t-1} + i_t x_t;  out = h [silu(z)]
 #include "hx_common.h"
-#include <initializer_list>
 
 namespace hx {
 namespace {
@@ -31,38 +30,34 @@ __device__ inline void silu_grad(float z, float& v, float& d) {
 // 2c and 2c+1 of the kSteps consecutive steps of part p = 2w + half, so a row of the tile is one 128-byte (bf16)
 // or 256-byte (fp32) run and every element is read once and stays in registers. A part is the affine map
 // h -> A h + H (A the product of its gates); the tile's parts are joined in LDS and the tiles of a sequence
-// through the workspace: a tile publishes its map as soon as it has it, then its exit state once it knows its
-// entry state, which it forms from the nearest exit state that is there and the maps after it.
+// through the workspace (see Chain): a tile publishes its map as soon as it has it.
 constexpr int kSteps = 8, kWaves = 8, kParts = 2 * kWaves, kTile = kParts * kSteps, kWidth = 64;
 static_assert(kTile == HX_GATED_CHUNK, "a tile's entry state is one of `states`");
 
-// Two neighbouring channels as they are stored.
+// Two neighbouring channels as they are stored, at any address that an element may have: rows of odd width start anywhere.
 template <typename T> struct Pair;
 template <> struct Pair<float> {
     using raw = float2;
-    __device__ static inline raw wide(const float* p) { return *reinterpret_cast<const float2*>(p); }
     __device__ static inline raw make(float a, float b) { return make_float2(a, b); }
     __device__ static inline float lo(raw r) { return r.x; }
     __device__ static inline float hi(raw r) { return r.y; }
-    __device__ static inline void store(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+    __device__ static inline raw pack(float a, float b) { return make_float2(a, b); }
+    // Keeps the stored form in registers: what was computed from it before is not carried along to be used again.
     __device__ static inline void hold(raw& r) { asm("" : "+v"(r.x), "+v"(r.y)); }
 };
 template <> struct Pair<uint16_t> {
     using raw = uint32_t;
-    __device__ static inline raw wide(const uint16_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
     __device__ static inline raw make(uint16_t a, uint16_t b) { return (uint32_t)b << 16 | a; }
     __device__ static inline float lo(raw r) { return __uint_as_float(r << 16); }
     __device__ static inline float hi(raw r) { return __uint_as_float(r & 0xffff0000u); }
-    __device__ static inline void store(uint16_t* p, float a, float b) {
-        *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(a, b);
-    }
-    // Keeps the stored form in registers: what was computed from it before is not carried along to be used again.
+    __device__ static inline raw pack(float a, float b) { return pack_bf16x2(a, b); }
     __device__ static inline void hold(raw& r) { asm("" : "+v"(r)); }
 };
 
-// Where a lane's elements lie. VEC: even dim and pairs aligned to a wide load.
-template <typename T, bool VEC>
+// Where a lane's elements lie. EVEN: an even number of channels, so that every pair is whole.
+template <typename T, bool EVEN>
 struct Place {
+    using raw = typename Pair<T>::raw;
     int64_t row;   // of the wave's first step, its first channel (uniform)
     int64_t D;
     uint32_t off;  // the lane's part and channel from there
@@ -75,95 +70,160 @@ struct Place {
         off = (uint32_t)(half * kSteps * D + c);
         const int64_t left = L - t0 - (wave * 2 + half) * kSteps;
         steps = c0 + c < D ? (int)(left < 0 ? 0 : left < kSteps ? left : kSteps) : 0;
-        second = c0 + c + 1 < D;
+        second = EVEN || c0 + c + 1 < D;
     }
-    __device__ inline typename Pair<T>::raw load(const T* base, int j) const {
+    __device__ inline raw load(const T* base, int j) const {
         const T* p = base + (row + j * D);
-        if (VEC) return Pair<T>::wide(p + off);
-        return Pair<T>::make(p[off], second ? p[off + 1] : p[off]);
+        raw r;
+        if (second)
+            __builtin_memcpy(&r, p + off, sizeof(r));
+        else
+            r = Pair<T>::make(p[off], 0);
+        return r;
     }
     __device__ inline void store(T* base, int j, float a, float b) const {
         T* p = base + (row + j * D);
-        if (VEC) {
-            Pair<T>::store(p + off, a, b);
+        if (second) {
+            const raw r = Pair<T>::pack(a, b);
+            __builtin_memcpy(p + off, &r, sizeof(r));
         } else {
             Storage<T>::store(p + off, a);
-            if (second) Storage<T>::store(p + off + 1, b);
         }
     }
     // All of the tile's loads of one operand, for the steps that exist.
-    __device__ inline void load_all(const T* base, typename Pair<T>::raw (&r)[kSteps]) const {
+    __device__ inline void load_all(const T* base, raw (&r)[kSteps]) const {
         if (__all(steps == kSteps)) {
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) r[j] = load(base, j);
         } else {
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) r[j] = j < steps ? load(base, j) : typename Pair<T>::raw{};
+            for (int j = 0; j < kSteps; ++j) r[j] = j < steps ? load(base, j) : raw{};
         }
     }
 };
 
-// The workspace: a ticket, then one 64-bit word for each tile and channel: all ones while there is nothing, then the
-// tile's map (A, H), then its exit state (kExit, h). Each word is written whole and says itself what it is, so no fence
-// is needed, only that readers and writers meet beyond the L2 of their XCD (agent scope).
+// The workspace: a ticket, then 64-bit words, all ones while there is nothing: one for each tile and channel, the tile's
+// map (A, H); one for each group of kGroup tiles, the group's map, then its exit state (kExit, h). Each word is written
+// whole and says itself what it is, so no fence is needed, only that readers and writers meet beyond the L2 of their XCD
+// (agent scope).
+//   entry of a tile  = the maps of the tiles before it in its group, applied in turn to the group's entry;
+//   exit of a group  = the group's map (its tiles' maps joined in turn) applied to the group's entry;
+//   entry of a group = the nearest exit that is there, and the maps of the groups after it applied in turn.
+// What is applied to what does not depend on which words were there first, so neither do the bits.
 struct Chain {
     uint32_t* ticket;
-    unsigned long long* words;
+    unsigned long long *tiles_at, *groups_at;
     int tiles;       // of one sequence
     uint32_t lanes;  // sequences x column tiles
 };
 constexpr unsigned long long kAbsent = ~0ull;
 constexpr uint32_t kExit = 0xfffffffeu, kNaN = 0x7fc00000u;
+constexpr int kGroup = 16, kMine = kGroup / kWaves;
 // A wait ends by itself where the workspace is misused (two calls at once): some 10^5 looks of about a microsecond.
 constexpr int kLooks = 1 << 17;
 
-// The first word of tile k in a column: uniform, so that a lane's part of an address is its number.
-__device__ inline unsigned long long* words_of(const Chain& c, int k, uint32_t col) {
-    return c.words + ((size_t)k * c.lanes + col) * kWidth;
+// The first word of row k (of tiles or groups) in a column: uniform, so that a lane's part of an address is its number.
+__device__ inline unsigned long long* words_of(unsigned long long* words, const Chain& c, int k, uint32_t col) {
+    return words + ((size_t)k * c.lanes + col) * kWidth;
 }
 __device__ inline void publish(unsigned long long* word, uint32_t lo, float hi) {
     __hip_atomic_store(word, (unsigned long long)__float_as_uint(hi) << 32 | lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ inline void publish_map(const Chain& c, int k, uint32_t col, int lane, float A, float H) {
+__device__ inline void publish_map(unsigned long long* word, float A, float H) {
     const uint32_t u = __float_as_uint(A);
-    publish(words_of(c, k, col) + lane, u >= kExit ? kNaN : u, H);  // no NaN passes for a tag
+    publish(word, u >= kExit ? kNaN : u, H);  // no NaN passes for a tag
 }
-__device__ inline void publish_exit(const Chain& c, int k, uint32_t col, int lane, float v) {
-    publish(words_of(c, k, col) + lane, kExit, v);
+__device__ inline unsigned long long look_at(const unsigned long long* word) {
+    return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ inline float map_a(unsigned long long m) { return __uint_as_float((uint32_t)m); }
+__device__ inline float map_h(unsigned long long m) { return __uint_as_float((uint32_t)(m >> 32)); }
 
-// The state that tile k of a chain starts from; `first` is the chain's own. An exit state is its tile's map applied
-// to its entry state, whoever applies it, so the bits do not depend on which words were there. One look covers
-// kWindow tiles, all of its words in flight at once.
-template <int kWindow>
-__device__ inline float entry_of(const Chain& c, int k, uint32_t col, int lane, float first) {
-    float e = first;
-    bool have = k == 0;
-    for (int look = 0; look < kLooks && !__all(have); ++look) {
-        if (look) __builtin_amdgcn_s_sleep(1);
-        unsigned long long m[kWindow];
+// What the block's waves have seen: the maps of the tiles before theirs in the group, the words of the kWaves groups
+// before it.
+struct Looked {
+    unsigned long long tiles[kGroup][kWidth], groups[kWaves][kWidth];
+    int found[kWaves];
+};
+constexpr int kNoMap = 1, kGroupExit = 2, kGroupAbsent = 4;
+
+// The state that tile k of a chain starts from, in wave 0's lanes; `first` is the chain's own, (A, H) the tile's map. The
+// waves look together, two tiles and one group each: the maps of a group are all there about when the tile's own is, and a
+// chain of many tiles moves on by kWaves groups, 16384 steps, a look. 1 x 42983 x 70 bf16 takes 28 us; with a window of 8
+// tiles and an exit state for every tile it took 73.
+__device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, int lane, float first, float A, float H,
+                                 Looked& seen) {
+    const int group = k / kGroup, place = k % kGroup;
+    const bool closes = place == kGroup - 1 && k + 1 < c.tiles;
+    if (wave == 0 && k + 1 < c.tiles) publish_map(words_of(c.tiles_at, c, k, col) + lane, A, H);
+    float GA = 1.0f, GH = 0.0f;
+    bool mapped = false, ok = false, held = false;
+    int start = -1;
+    for (int look = 0; look < kLooks; ++look) {
+        int found = 0;
+        unsigned long long m[kMine], w = 0;
+        const int from = group - kWaves + wave;
 #pragma unroll
-        for (int i = 0; i < kWindow; ++i) {
-            const int j = k - kWindow + i;
-            m[i] = __hip_atomic_load(words_of(c, j < 0 ? 0 : j, col) + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        float v = first;
-        bool ok = k <= kWindow;  // the window reaches the chain's start
+        for (int i = 0; i < kMine; ++i)
+            if (!held && wave * kMine + i < place) m[i] = look_at(words_of(c.tiles_at, c, k - place + wave * kMine + i, col) + lane);
+        if (from >= 0) w = look_at(words_of(c.groups_at, c, from, col) + lane);
 #pragma unroll
-        for (int i = 0; i < kWindow; ++i) {
-            if (k - kWindow + i < 0) continue;
-            const uint32_t lo = (uint32_t)m[i];
-            const float H = __uint_as_float((uint32_t)(m[i] >> 32));
-            const bool exit = lo == kExit;
-            ok = exit || (ok && m[i] != kAbsent);
-            v = exit ? H : fmaf(__uint_as_float(lo), v, H);
+        for (int i = 0; i < kMine; ++i)
+            if (!held && wave * kMine + i < place) {
+                if (__any(m[i] == kAbsent)) found = kNoMap;
+                seen.tiles[wave * kMine + i][lane] = m[i];
+            }
+        held = found == 0;
+        if (from >= 0) {
+            if (__all((uint32_t)w == kExit)) found |= kGroupExit;
+            if (__any(w == kAbsent)) found |= kGroupAbsent;
+            seen.groups[wave][lane] = w;
         }
-        if (ok) {
-            e = v;
-            have = true;
+        if (lane == 0) seen.found[wave] = found;
+        __syncthreads();
+        int absent = -1;
+        bool maps = true;
+        start = -1;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const int f = seen.found[i];
+            maps = maps && !(f & kNoMap);
+            if (f & kGroupExit) start = i;
+            if (f & kGroupAbsent) absent = i;
         }
+        if (maps && closes && !mapped) {
+            mapped = true;
+            if (wave == 0) {
+#pragma unroll 4
+                for (int i = 0; i < kGroup - 1; ++i) {
+                    const unsigned long long t = seen.tiles[i][lane];
+                    GH = fmaf(map_a(t), GH, map_h(t));
+                    GA *= map_a(t);
+                }
+                GH = fmaf(A, GH, H);
+                GA *= A;
+                publish_map(words_of(c.groups_at, c, group, col) + lane, GA, GH);
+            }
+        }
+        ok = maps && (start > absent || (absent < 0 && group <= kWaves));  // or the look reaches the chain's start
+        if (ok) break;
+        __syncthreads();
+        __builtin_amdgcn_s_sleep(1);
     }
-    return have ? e : __uint_as_float(kNaN);
+    if (wave != 0) return 0.0f;
+    float e = ok ? first : __uint_as_float(kNaN);
+    if (ok)
+        for (int i = start >= 0 ? start : kWaves - (group < kWaves ? group : kWaves); i < kWaves; ++i) {
+            const unsigned long long g = seen.groups[i][lane];
+            e = (uint32_t)g == kExit ? map_h(g) : fmaf(map_a(g), e, map_h(g));
+        }
+    if (closes) publish(words_of(c.groups_at, c, group, col) + lane, kExit, fmaf(GA, e, GH));
+#pragma unroll 4
+    for (int i = 0; i < place; ++i) {
+        const unsigned long long t = seen.tiles[i][lane];
+        e = fmaf(map_a(t), e, map_h(t));
+    }
+    return e;
 }
 
 // Which tile this block takes: tickets are handed out in the order in which blocks start, tile 0 of every column
@@ -190,17 +250,18 @@ struct FwdArgs {
     Chain chain;
 };
 
-template <typename T, bool VEC, bool GATE>
+template <typename T, bool EVEN, bool GATE>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void gated_fwd_kernel(const FwdArgs p) {
     __shared__ float2 maps[kParts][kWidth];
     __shared__ float entries[kParts][kWidth];
+    __shared__ Looked seen;
     __shared__ uint32_t shared_unit;
     int k;
     uint32_t col;
     if (!take_unit(p.chain, shared_unit, k, col)) return;
     const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const Place<T, VEC> at(b, (int64_t)k * kTile, c0, wave, lane, p.L, p.D);
+    const Place<T, EVEN> at(b, (int64_t)k * kTile, c0, wave, lane, p.L, p.D);
     typename Pair<T>::raw rf[kSteps], rx[kSteps], rz[kSteps];
     at.load_all((const T*)p.f, rf);
     at.load_all((const T*)p.x, rx);
@@ -227,25 +288,23 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void g
     const int part = wave * 2 + (lane >> 5), c = (lane & 31) * 2;
     *reinterpret_cast<float4*>(&maps[part][c]) = make_float4(A0, H0, A1, H1);
     __syncthreads();
+    const bool in = c0 + lane < p.D;
+    const int64_t r = b * p.D + c0 + lane;
+    float A = 1.0f, H = 0.0f, e = 0.0f;
     if (wave == 0) {
-        const bool in = c0 + lane < p.D;
-        const int64_t r = b * p.D + c0 + lane;
-        float A = 1.0f, H = 0.0f;
-#pragma unroll 8
+#pragma unroll 4
         for (int s = 0; s < kParts; ++s) {
             const float2 m = maps[s][lane];
             H = fmaf(m.x, H, m.y);
             A *= m.x;
         }
-        float e = in && p.init ? p.init[r] : 0.0f;
-        if (p.chain.tiles > 1) {
-            if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, H);
-            e = entry_of<GATE && sizeof(T) == 2 ? 6 : 8>(p.chain, k, col, lane, e);
-            if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, H));
-        }
+        if (in && p.init) e = p.init[r];
+    }
+    if (p.chain.tiles > 1) e = entry_of(p.chain, k, col, wave, lane, e, A, H, seen);
+    if (wave == 0) {
         if (in && p.states) p.states[(b * p.chain.tiles + k) * p.D + c0 + lane] = e;
         if (in && p.last && k + 1 == p.chain.tiles) p.last[r] = fmaf(A, e, H);
-#pragma unroll 8
+#pragma unroll 4
         for (int s = 0; s < kParts; ++s) {
             const float2 m = maps[s][lane];
             entries[s][lane] = e;
@@ -253,8 +312,12 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void g
         }
     }
     __syncthreads();
-    const float2 e = *reinterpret_cast<const float2*>(&entries[part][c]);
-    float h0 = e.x, h1 = e.y;
+    const float2 start = *reinterpret_cast<const float2*>(&entries[part][c]);
+    float h0 = start.x, h1 = start.y;
+    if (GATE) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) Pair<T>::hold(rz[j]);
+    }
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
         h0 = fmaf(a0[j], h0, b0[j]);
@@ -276,9 +339,10 @@ struct BwdArgs {
 
 // The tiles from the last one back. The carry c_t = a_t g_t obeys c_t = a_t c_{t+1} + a_t dh_t, so parts and tiles
 // are affine maps again, with the same A. h is formed from `states` for the tile alone, without waiting.
-template <typename T, bool VEC, bool GATE>
+template <typename T, bool EVEN, bool GATE>
 __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs p) {
     __shared__ float maps_a[kParts][kWidth], maps_h[kParts][kWidth], maps_g[kParts][kWidth];
+    __shared__ Looked seen;
     __shared__ uint32_t shared_unit;
     int k;
     uint32_t col;
@@ -286,7 +350,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
     const int tile = p.chain.tiles - 1 - k;
     const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const Place<T, VEC> at(b, (int64_t)tile * kTile, c0, wave, lane, p.L, p.D);
+    const Place<T, EVEN> at(b, (int64_t)tile * kTile, c0, wave, lane, p.L, p.D);
     typename Pair<T>::raw rf[kSteps], rx[kSteps], rz[kSteps], rd[kSteps];
     at.load_all((const T*)p.f, rf);
     at.load_all((const T*)p.x, rx);
@@ -323,38 +387,36 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
     *reinterpret_cast<float2*>(&maps_h[part][c]) = make_float2(H0, H1);
     *reinterpret_cast<float2*>(&maps_g[part][c]) = make_float2(G0, G1);
     __syncthreads();
-    // Wave 0 joins the carries and waits for the tiles after this one, wave 1 the states; each leaves its parts' entry
-    // values where the maps were that only it reads.
+    // Wave 0 joins the carries, wave 1 meanwhile the states; each leaves its parts' entry values where the maps were that
+    // only it reads.
+    const bool in = c0 + lane < p.D;
+    const int64_t r = b * p.D + c0 + lane;
+    float A = 1.0f, G = 0.0f, e = 0.0f;
     if (wave == 0) {
-        const bool in = c0 + lane < p.D;
-        const int64_t r = b * p.D + c0 + lane;
-        float A = 1.0f, G = 0.0f;
-#pragma unroll 8
+#pragma unroll 4
         for (int s = kParts - 1; s >= 0; --s) {
             const float m = maps_a[s][lane];
             G = fmaf(m, G, maps_g[s][lane]);
             A *= m;
         }
-        float e = in && p.dlast ? p.dlast[r] : 0.0f;
-        if (p.chain.tiles > 1) {
-            if (k + 1 < p.chain.tiles) publish_map(p.chain, k, col, lane, A, G);
-            e = entry_of<8>(p.chain, k, col, lane, e);
-            if (k + 1 < p.chain.tiles) publish_exit(p.chain, k, col, lane, fmaf(A, e, G));
-        }
-        if (in && p.dinit && tile == 0) p.dinit[r] = fmaf(A, e, G);
-#pragma unroll 8
-        for (int s = kParts - 1; s >= 0; --s) {
-            const float g = maps_g[s][lane];
-            maps_g[s][lane] = e;
-            e = fmaf(maps_a[s][lane], e, g);
-        }
+        if (in && p.dlast) e = p.dlast[r];
     } else if (wave == 1) {
-        float h = c0 + lane < p.D ? p.states[(b * p.chain.tiles + tile) * p.D + c0 + lane] : 0.0f;
-#pragma unroll 8
+        float h = in ? p.states[(b * p.chain.tiles + tile) * p.D + c0 + lane] : 0.0f;
+#pragma unroll 4
         for (int s = 0; s < kParts; ++s) {
             const float m = maps_h[s][lane];
             maps_h[s][lane] = h;
             h = fmaf(maps_a[s][lane], h, m);
+        }
+    }
+    if (p.chain.tiles > 1) e = entry_of(p.chain, k, col, wave, lane, e, A, G, seen);
+    if (wave == 0) {
+        if (in && p.dinit && tile == 0) p.dinit[r] = fmaf(A, e, G);
+#pragma unroll 4
+        for (int s = kParts - 1; s >= 0; --s) {
+            const float g = maps_g[s][lane];
+            maps_g[s][lane] = e;
+            e = fmaf(maps_a[s][lane], e, g);
         }
     }
     __syncthreads();
@@ -410,7 +472,7 @@ __global__ __launch_bounds__(256) void gated_chain_clear_kernel(uint4* ws, int64
 }
 
 // One token: four channels a thread (16 bytes of state), bound by the state's read and write; the last n % 4 channels
-// one a thread. 256 x 4096 fp32: XXX us, one channel a thread 5.5.
+// one a thread. 256 x 4096 fp32: 5.2 us, one channel a thread 5.5.
 template <typename T, int N>
 __device__ inline void step_run(int64_t o, float* state, const T* x, const T* f, const T* z, T* out) {
     const Run<N, T> xv = Run<N, T>::load(x + o), fv = Run<N, T>::load(f + o);
@@ -457,10 +519,12 @@ struct Shape {
         return batch < kMaxBlocks && D < (1 << 26) && L < ((int64_t)1 << 37) &&
                (__int128)batch * cols * (tiles > 0 ? tiles : 1) < kMaxBlocks && (__int128)batch * L * D < ((__int128)1 << 60);
     }
-    // 16 bytes for the ticket, a word per tile and channel; one tile waits for nobody
-    size_t workspace() const { return tiles > 1 ? 16 + (size_t)units * kWidth * 8 : 0; }
+    // 16 bytes for the ticket, a word per channel of each tile and group; one tile waits for nobody
+    int64_t groups() const { return (tiles + kGroup - 1) / kGroup; }
+    size_t workspace() const { return tiles > 1 ? 16 + ((size_t)units + groups() * batch * cols) * kWidth * 8 : 0; }
     Chain chain(void* ws) const {
-        return Chain{(uint32_t*)ws, (unsigned long long*)((char*)ws + 16), (int)tiles, (uint32_t)(batch * cols)};
+        unsigned long long* const words = (unsigned long long*)((char*)ws + 16);
+        return Chain{(uint32_t*)ws, words, words + (size_t)units * kWidth, (int)tiles, (uint32_t)(batch * cols)};
     }
 };
 
@@ -479,20 +543,10 @@ int copy_state(int64_t rows, const float* src, float* dst, hipStream_t s) {
     return HX_OK;
 }
 
-// Pairs can be loaded whole: even rows, every operand aligned to a pair.
-template <typename T>
-bool pairs(int64_t D, std::initializer_list<const void*> ops) {
-    if (D % 2) return false;
-    for (const void* p : ops)
-        if (!aligned(p, 2 * sizeof(T))) return false;
-    return true;
-}
-
 template <typename T>
 int fwd(const Shape& g, const FwdArgs& p, hipStream_t s) {
-    const bool vec = pairs<T>(g.D, {p.x, p.f, p.z, p.out});
-    const auto k = vec ? (p.z ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
-                       : (p.z ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
+    const auto k = g.D % 2 == 0 ? (p.z ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
+                             : (p.z ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
     hipLaunchKernelGGL(k, dim3((unsigned)g.units), dim3(64 * kWaves), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
@@ -500,9 +554,8 @@ int fwd(const Shape& g, const FwdArgs& p, hipStream_t s) {
 
 template <typename T>
 int bwd(const Shape& g, const BwdArgs& p, hipStream_t s) {
-    const bool vec = pairs<T>(g.D, {p.x, p.f, p.z, p.dout, p.dx, p.df, p.dz});
-    const auto k = vec ? (p.z ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
-                       : (p.z ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
+    const auto k = g.D % 2 == 0 ? (p.z ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
+                             : (p.z ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
     hipLaunchKernelGGL(k, dim3((unsigned)g.units), dim3(64 * kWaves), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;

@@ -55,8 +55,8 @@ __device__ inline bf16x8 expand8(uint32_t q, float scale) {
 //            groups need no sums of their own);
 //   X        16 lanes read a row's 256 bytes of the window and leave them in the wave's own LDS rows, 16 bytes apart
 //            from a power of two, so that 16 rows read at one place of theirs meet all banks.
-// XVEC: 16-byte aligned rows of X.
-template <int NT, int XR, bool XVEC, typename TO>
+// Rows of X start anywhere: global memory takes 16-byte accesses at any element.
+template <int NT, int XR, typename TO>
 __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
     constexpr int MT = XR < 4 ? 1 : XR / 4, kRows = 4 * XR;  // column tiles of 16, rows of X that are staged
     extern __shared__ float lds[];  // first the waves' rows of X, then [waves][NT][MT][16 m][16 n] sums
@@ -95,25 +95,31 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
     const auto load_x = [&](int at, u32x4 (&o)[XR]) {
         const uint16_t* from = xb + (int64_t)at * kWindow;
 #pragma unroll
-        for (int t = 0; t < XR; ++t) o[t] = *reinterpret_cast<const u32x4*>(from + x[t]);
+        for (int t = 0; t < XR; ++t) __builtin_memcpy(&o[t], from + x[t], 16);
     };
     // A wave's own rows, and its LDS accesses keep their order: no barrier, and the registers are free for the next window.
     const auto stage = [&](const u32x4 (&xs)[XR]) {
 #pragma unroll
         for (int t = 0; t < XR; ++t) *reinterpret_cast<u32x4*>(xrow + (4 * t + j) * kXRow + 16 * r) = xs[t];
     };
-    // Element by element: rows of any alignment, and the window that K ends in, elements from K on as zero.
-    const auto stage_any = [&](int at) {
-        const int64_t left = p.K - (int64_t)at * kWindow - 8 * r;
-        for (int row = j; row < rows_in; row += 4) {
-            const uint16_t* from = xb + row * p.ldx + (int64_t)at * kWindow + 8 * r;
-            union {
-                u32x4 v;
-                uint16_t e[8];
-            } u;
+    // The window that K ends in: elements from K on are zero. The eight that hold K are loaded ending at K and moved up, so
+    // that nothing behind a row is touched; rows of fewer than eight go one by one.
+    const auto load_x_end = [&](int at, u32x4 (&o)[XR]) {
+        const int left = (int)(p.K - (int64_t)at * kWindow) - 8 * r;
+        const int back = left >= 8 ? 0 : 8 - left;
+        const uint16_t* from = xb + (int64_t)at * kWindow;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u.e[e] = e < left ? from[e] : 0;
-            *reinterpret_cast<u32x4*>(xrow + row * kXRow + 16 * r) = u.v;
+        for (int t = 0; t < XR; ++t) {
+            unsigned __int128 v = 0;
+            if (left > 0) {
+                if (p.K >= 8) {
+                    __builtin_memcpy(&v, from + x[t] - back, 16);
+                    v >>= 16 * back;
+                } else {
+                    for (int e = 0; e < left; ++e) v |= (unsigned __int128)from[x[t] + e] << (16 * e);
+                }
+            }
+            __builtin_memcpy(&o[t], &v, 16);
         }
     };
     const auto load_w = [&](int at, bool in, u32x4 (&o)[NT]) {
@@ -176,18 +182,14 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
         load_s(at, sc);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) load_w(at + u, true, q[u]);
-        if (XVEC) load_x(at, xs);
+        load_x(at, xs);
         for (; at + 2 * kAhead <= whole; at += kAhead) {
             uint32_t after[NT];
             load_s(at + kAhead, after);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                if (XVEC) {
-                    stage(xs);
-                    load_x(at + u + 1, xs);
-                } else {
-                    stage_any(at + u);
-                }
+                stage(xs);
+                load_x(at + u + 1, xs);
                 u32x4 now[NT];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) now[t] = q[u][t];
@@ -199,12 +201,8 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (XVEC) {
-                stage(xs);
-                if (u + 1 < kAhead) load_x(at + u + 1, xs);
-            } else {
-                stage_any(at + u);
-            }
+            stage(xs);
+            if (u + 1 < kAhead) load_x(at + u + 1, xs);
             multiply(q[u], sc, u, 4);
         }
         at += kAhead;
@@ -220,13 +218,12 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
         for (int u = 0; u < kAhead; ++u) {
             if (at + u >= end) break;
             const int left = (int)(G - (int64_t)(at + u) * 4);
-            if (XVEC && at + u < whole) {
-                u32x4 xs[XR];
+            u32x4 xs[XR];
+            if (at + u < whole)
                 load_x(at + u, xs);
-                stage(xs);
-            } else {
-                stage_any(at + u);
-            }
+            else
+                load_x_end(at + u, xs);
+            stage(xs);
             multiply(q[u], sc, u, left < 4 ? left : 4);
         }
     }
@@ -266,10 +263,9 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
 }
 
 template <int NT, int XR>
-int launch_w4(const W4Args& p, bool xvec, bool f32, hipStream_t s) {
+int launch_w4(const W4Args& p, bool f32, hipStream_t s) {
     const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)), (unsigned)((p.M + 4 * XR - 1) / (4 * XR)));
-    const auto k = f32 ? (xvec ? linear_w4_kernel<NT, XR, true, float> : linear_w4_kernel<NT, XR, false, float>)
-                       : (xvec ? linear_w4_kernel<NT, XR, true, uint16_t> : linear_w4_kernel<NT, XR, false, uint16_t>);
+    const auto k = f32 ? linear_w4_kernel<NT, XR, float> : linear_w4_kernel<NT, XR, uint16_t>;
     constexpr size_t staged = 4 * XR * kXRow, summed = NT * (XR < 4 ? 1 : XR / 4) * 256 * sizeof(float);
     const size_t bytes = p.waves * (staged > summed ? staged : summed);
     HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 0), HX_ERR_UNSUPPORTED,
@@ -332,8 +328,8 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
                "linear_w4: X, packed, scales and Y required, ldx >= K, ldy >= N");
     HX_REQUIRE(aligned(packed, 16) && aligned(scales, 16), HX_ERR_INVALID_INPUT,
                "linear_w4: packed and scales must be 16-byte aligned");
-    HX_REQUIRE(N < ((int64_t)1 << 34) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26), HX_ERR_UNSUPPORTED,
-               "linear_w4: at most %d rows of X, 2^34 outputs and K below 2^26", kRowsAtOnce * 65535);
+    HX_REQUIRE(N < ((int64_t)1 << 34) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26) && ldx < (1 << 26),
+               HX_ERR_UNSUPPORTED, "linear_w4: at most %d rows of X, 2^34 outputs, K and ldx below 2^26", kRowsAtOnce * 65535);
     // How K is cut decides the order of the sums, so it goes by N and K alone: two waves a tile of 16 outputs, more, up to 8,
     // while there are fewer than 8 for each of 256 CUs; none without a window. 1 x 2048 x 4096: 8 waves 4.4 us, 4 waves
     // 4.7, 2 waves 6.1; 1 x 16384 x 2048: 2 waves 6.3, 4 waves 7.0; 5 x 32768 x 8192: 2 waves 34.5, 4 waves 38.7.
@@ -343,14 +339,14 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
     while (waves < 8 && waves * 2 <= windows && tiles * waves < 2048) waves *= 2;
     const W4Args p{M, N, K, ldx, ldy, (const uint16_t*)X, (const uint8_t*)packed, (const uint8_t*)scales, bias, Y, act, windows,
                    (windows + waves - 1) / waves, waves};
-    const bool xvec = aligned(X, 16) && ldx % 8 == 0 && ldx < (1 << 26), f32 = out_dtype == HX_F32;
+    const bool f32 = out_dtype == HX_F32;
     hipStream_t s = as_stream(stream);
     // Two tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs, with few rows nothing.
     // 5 x 32768 x 8192: 1 tile 37.5 us, 2 tiles 34.5; 16 x 8192 x 4096: 8.3 and 7.7; 64 x 16384 x 8192: 86 and 46;
     // 1 x 16384 x 2048: 6.3 and 7.6; 8 x 8192 x 4096: 7.3 and 7.4; 24 x 4096 x 4096: 7.6 and 8.6.
     const bool two = M > 8 ? tiles >= 512 : M > 4 && tiles >= 1024;
-    if (M <= 4) return launch_w4<1, 1>(p, xvec, f32, s);
-    if (M <= 8) return two ? launch_w4<2, 2>(p, xvec, f32, s) : launch_w4<1, 2>(p, xvec, f32, s);
-    if (M <= 16) return two ? launch_w4<2, 4>(p, xvec, f32, s) : launch_w4<1, 4>(p, xvec, f32, s);
-    return two ? launch_w4<2, 8>(p, xvec, f32, s) : launch_w4<1, 8>(p, xvec, f32, s);
+    if (M <= 4) return launch_w4<1, 1>(p, f32, s);
+    if (M <= 8) return two ? launch_w4<2, 2>(p, f32, s) : launch_w4<1, 2>(p, f32, s);
+    if (M <= 16) return two ? launch_w4<2, 4>(p, f32, s) : launch_w4<1, 4>(p, f32, s);
+    return two ? launch_w4<2, 8>(p, f32, s) : launch_w4<1, 8>(p, f32, s);
 }
