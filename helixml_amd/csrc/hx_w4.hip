@@ -330,22 +330,23 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
                "linear_w4: packed and scales must be 16-byte aligned");
     HX_REQUIRE(N < ((int64_t)1 << 34) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26) && ldx < (1 << 26),
                HX_ERR_UNSUPPORTED, "linear_w4: at most %d rows of X, 2^34 outputs, K and ldx below 2^26", kRowsAtOnce * 65535);
-    // How K is cut decides the order of the sums, so it goes by N and K alone: two waves a tile of 16 outputs, more, up to 8,
-    // while there are fewer than 8 for each of 256 CUs; none without a window. 1 x 2048 x 4096: 8 waves 4.4 us, 4 waves
-    // 4.7, 2 waves 6.1; 1 x 16384 x 2048: 2 waves 6.3, 4 waves 7.0; 5 x 32768 x 8192: 2 waves 34.5, 4 waves 38.7.
+    // How K is cut decides the order of the sums, so it goes by N and K alone: up to 8 waves a tile of 16 outputs while there
+    // are fewer than 8 for each of 256 CUs, or 16 where a wave would walk more than 8 windows, none with fewer than two.
+    // 1 x 2048 x 4096: 8 waves 4.4 us, 4 waves 4.7, 2 waves 6.1; 2 x 16384 x 4096: 4 waves 11.1, 8 waves 12.2; 1 x 16384 x
+    // 2048: 2 waves 6.3, 4 waves 7.0; 5 x 32768 x 8192: 2 waves 34.6, 4 waves 39; 45 x 14152 x 736: 2 waves 10.4, 4 waves 12.9.
     const int windows = (int)((K + kWindow - 1) / kWindow);
     const int64_t tiles = (N + 15) / 16;
-    int waves = windows > 1 ? 2 : 1;
-    while (waves < 8 && waves * 2 <= windows && tiles * waves < 2048) waves *= 2;
+    int waves = 1;
+    while (waves < 8 && windows >= 4 * waves && (tiles * waves < 2048 || (windows > 8 * waves && tiles * waves < 4096))) waves *= 2;
     const W4Args p{M, N, K, ldx, ldy, (const uint16_t*)X, (const uint8_t*)packed, (const uint8_t*)scales, bias, Y, act, windows,
                    (windows + waves - 1) / waves, waves};
     const bool f32 = out_dtype == HX_F32;
     hipStream_t s = as_stream(stream);
-    // Two tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs, with few rows nothing.
-    // 5 x 32768 x 8192: 1 tile 37.5 us, 2 tiles 34.5; 16 x 8192 x 4096: 8.3 and 7.7; 64 x 16384 x 8192: 86 and 46;
-    // 1 x 16384 x 2048: 6.3 and 7.6; 8 x 8192 x 4096: 7.3 and 7.4; 24 x 4096 x 4096: 7.6 and 8.6.
-    const bool two = M > 8 ? tiles >= 512 : M > 4 && tiles >= 1024;
-    if (M <= 4) return launch_w4<1, 1>(p, f32, s);
+    // Two tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs. 1 tile and 2 tiles:
+    // 1 x 32768 x 8192 36.3 and 32.8 us, 1 x 16384 x 2048 6.3 and 7.6; 5 x 32768 x 8192 38.4 and 34.6, 8 x 8192 x 4096 7.3
+    // and 7.4; 9 x 5314 x 6080 10.9 and 9.9, 24 x 4096 x 4096 7.6 and 8.6; 64 x 16384 x 8192 70 and 47.
+    const bool two = M > 8 ? tiles > 256 : tiles >= (M > 4 ? 1024 : 2048);
+    if (M <= 4) return two ? launch_w4<2, 1>(p, f32, s) : launch_w4<1, 1>(p, f32, s);
     if (M <= 8) return two ? launch_w4<2, 2>(p, f32, s) : launch_w4<1, 2>(p, f32, s);
     if (M <= 16) return two ? launch_w4<2, 4>(p, f32, s) : launch_w4<1, 4>(p, f32, s);
     return two ? launch_w4<2, 8>(p, f32, s) : launch_w4<1, 8>(p, f32, s);

@@ -93,7 +93,7 @@ def test_linear_refusals():
 # ------------------------------------------------------------------ products (device)
 SIZES = [(1, 1, 1), (1, 16, 32), (1, 17, 33), (2, 5, 64), (3, 100, 31), (1, 256, 512), (5, 160, 4096), (16, 64, 128), (17, 48, 96),
          (33, 70, 1000), (64, 130, 544), (65, 33, 256), (130, 40, 160), (1, 1000, 2080), (7, 4100, 512), (4, 300, 777),
-         (2, 16400, 160), (6, 16390, 288), (16, 16400, 1100), (40, 16500, 640), (33, 16384, 96)]
+         (2, 16400, 160), (6, 16390, 288), (16, 16400, 1100), (40, 16500, 640), (33, 16384, 96), (3, 32770, 264), (9, 4113, 1056)]
 
 
 def random_weights(N, K, seed, lo=120, hi=130):
