@@ -70,15 +70,16 @@ def conv1d_step(x, weight, bias, state, out=None, stream=None):
     return out
 
 
-def _rows(t, name, shape, dtype):
-    """Checks a [batch, n] device tensor with unit column stride; its row stride (n for a single row)."""
-    if not t.is_cuda:
-        raise _ffi.InvalidInput(f"{name} must be a device tensor")
-    if tuple(t.shape) != tuple(shape):
-        raise _ffi.ShapeMismatch(f"{name}: expected {list(shape)}, got {list(t.shape)}")
-    if t.dtype != dtype:
-        raise _ffi.DTypeMismatch(f"{name}: expected {dtype}, got {t.dtype}")
-    if shape[1] > 1 and t.stride(1) != 1:
+def _rows(launch, t, name, shape, dtype):
+    """Checks a [batch, n] tensor of the launch's device with unit column stride; its row stride (n for a single row)."""
+    if t.shape != shape or t.dtype != dtype or t.device != launch.device or (shape[1] > 1 and t.stride(1) != 1):
+        if not t.is_cuda:
+            raise _ffi.InvalidInput(f"{name} must be a device tensor")
+        if t.shape != shape:
+            raise _ffi.ShapeMismatch(f"{name}: expected {list(shape)}, got {list(t.shape)}")
+        if t.dtype != dtype:
+            raise _ffi.DTypeMismatch(f"{name}: expected {dtype}, got {t.dtype}")
+        _on_stream_device(launch, **{name: t})
         raise _ffi.InvalidInput(f"{name} needs unit column stride")
     return t.stride(0) if shape[0] > 1 else shape[1]
 
@@ -103,13 +104,13 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
     if logits.dtype not in _STORAGE:
         raise _ffi.DTypeMismatch(f"logits: {logits.dtype} is neither float32 nor bfloat16")
     bt, V = shape = logits.shape
-    ldl = _rows(logits, "logits", shape, logits.dtype)
+    ldl = _rows(stream, logits, "logits", shape, logits.dtype)
     ldh = n = 0
     if history is not None:
         if history.dim() != 2:
             raise _ffi.ShapeMismatch(f"history: expected [batch, n], got {list(history.shape)}")
         n = history.shape[1]
-        ldh = _rows(history, "history", (bt, n), torch.int32)
+        ldh = _rows(stream, history, "history", (bt, n), torch.int32)
     one, i32, f32 = (bt,), torch.int32, torch.float32
     _operands(stream, ("lengths", lengths, one, i32), ("prompt_lengths", prompt_lengths, one, i32),
               ("repetition", repetition, one, f32), ("frequency", frequency, one, f32), ("presence", presence, one, f32))
@@ -119,16 +120,16 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
         if bias.dim() == 1:
             _operands(stream, ("bias", bias, (V,), f32))
         else:
-            ldb = _rows(bias, "bias", shape, f32)
+            ldb = _rows(stream, bias, "bias", shape, f32)
     if allowed is not None:
         if allowed.dim() == 1:
             _operands(stream, ("allowed", allowed, (words,), i32))
         else:
-            lda = _rows(allowed, "allowed", (bt, words), i32)
+            lda = _rows(stream, allowed, "allowed", (bt, words), i32)
     if out is None:
-        out = torch.empty((bt, V), device=logits.device, dtype=logits.dtype)
-    ldo = _rows(out, "out", shape, logits.dtype)
-    _on_stream_device(stream, logits=logits, history=history, bias=bias, allowed=allowed, out=out)
+        out, ldo = torch.empty(shape, device=logits.device, dtype=logits.dtype), V
+    else:
+        ldo = ldl if out is logits else _rows(stream, out, "out", shape, logits.dtype)
     _ffi.call("hx_logits_adjust", bt, V, _STORAGE[logits.dtype], _ptr(logits), ldl, _ptr(history), ldh, n,
               _ptr(lengths), _ptr(prompt_lengths), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias), ldb,
               _ptr(allowed), lda, _ptr(out), ldo, _stream(stream))
