@@ -268,8 +268,9 @@ int launch_w4(const W4Args& p, bool f32, hipStream_t s) {
     const auto k = f32 ? linear_w4_kernel<NT, XR, float> : linear_w4_kernel<NT, XR, uint16_t>;
     constexpr size_t staged = 4 * XR * kXRow, summed = NT * (XR < 4 ? 1 : XR / 4) * 256 * sizeof(float);
     const size_t bytes = p.waves * (staged > summed ? staged : summed);
-    HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 0), HX_ERR_UNSUPPORTED,
-               "linear_w4: %zu bytes of LDS are not granted", bytes);
+    if (bytes > 65536 && !grant_dynamic_lds((const void*)k, bytes, 0)) {
+        if constexpr (XR > 4) return launch_w4<NT, XR / 2>(p, f32, s);  // the same sums, X's rows in two blocks
+    }
     hipLaunchKernelGGL(k, grid, dim3((unsigned)(64 * p.waves)), bytes, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;

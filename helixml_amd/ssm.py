@@ -71,16 +71,21 @@ _DEVICES: dict = {}
 
 def on_current_or_launch_stream(fn):
     """on_launch_stream for wrappers of a few microseconds that need no more of their stream than its handle and device:
-    with no stream given they run on the current one, where there is nothing to switch."""
-    switched = on_launch_stream(fn)
-
+    with no stream given they run on the current one, where there is nothing to switch. On a stream that is given, the
+    operands are marked as used there (keep_for_stream): the caller may drop them while the work is still queued."""
     @functools.wraps(fn)
     def run(*args, stream=None, **kwargs):
-        if stream is not None or not torch.cuda.is_initialized():
-            return switched(*args, stream=stream, **kwargs)
-        i = torch._C._cuda_getDevice()
-        device = _DEVICES.get(i) or _DEVICES.setdefault(i, torch.device("cuda", i))
-        return fn(*args, stream=_CurrentStream(torch._C._cuda_getCurrentRawStream(i), device), **kwargs)
+        if stream is None and torch.cuda.is_initialized():
+            i = torch._C._cuda_getDevice()
+            device = _DEVICES.get(i) or _DEVICES.setdefault(i, torch.device("cuda", i))
+            return fn(*args, stream=_CurrentStream(torch._C._cuda_getCurrentRawStream(i), device), **kwargs)
+        ts = _torch_stream(stream)
+        with torch.cuda.stream(ts):
+            result = fn(*args, stream=ts, **kwargs)
+            for t in (*args, *kwargs.values()):
+                if isinstance(t, torch.Tensor):
+                    keep_for_stream(t, ts)
+            return result
     run.on_launch_stream = True
     return run
 

@@ -139,6 +139,68 @@ def test_forward_and_gradients(dev, bt, L, dim, gate, chunk, dtype):
     check("dinit", got["dinit"], b["dinit"], b["dinit_E"], 2.0 ** -24)
 
 
+@pytest.mark.parametrize("bt,L,dim,dtype", [(1, 70001, 2, torch.float32), (2, 40000, 5, torch.bfloat16), (12, 2300, 700, torch.bfloat16),
+                                            (1, 16384, 3, torch.float32), (1, 16385, 3, torch.float32)])
+def test_long_chains(dev, bt, L, dim, dtype):
+    """Sequences of many groups of tiles, and more tiles than fit the GPU at once."""
+    x = inputs(bt, L, dim, seed=L, dtype=dtype)
+    got = run(dev, x)
+    ref = {k: f64(v) for k, v in x.items()}
+    o = oracle_fwd(**ref)
+    check("out", got["out"], o["out"], o["out_E"], HALF[dtype])
+    check("last", got["last"], o["last"], o["last_E"], 2.0 ** -24)
+    check("states", got["states"], o["before"][:, ::CHUNK], o["bE"][:, ::CHUNK] + U * np.abs(o["before"][:, ::CHUNK]), 2.0 ** -24)
+    b = oracle_bwd(**ref)
+    for k in ("dx", "df", "dz"):
+        check(k, got[k], b[k], b[k + "_E"], HALF[dtype])
+    check("dinit", got["dinit"], b["dinit"], b["dinit_E"], 2.0 ** -24)
+
+
+@pytest.mark.parametrize("fill", [0, 255, None], ids=["zeros", "ones", "numbers"])
+def test_a_workspace_may_hold_anything(dev, fill):
+    """What an earlier call left, zeros, or numbers: a workspace is cleared by the call that uses it."""
+    x = inputs(2, 3000, 70, seed=11, dtype=torch.float32)
+    d = to(dev, x)
+    want = run(dev, x)
+    n = max(ssm.gated_scan_workspace_size(2, 3000, 70, backward=b) for b in (False, True))
+    ws = torch.randn(n // 4 + 4, device=dev).view(torch.uint8)[:n].contiguous()
+    if fill is not None:
+        ws.fill_(fill)
+    out, last, states = ssm.gated_scan_fwd(d["x"], d["f"], d["z"], d["init"], return_last_state=True, return_states=True, workspace=ws)
+    if fill is not None:
+        ws.fill_(fill)
+    got = ssm.gated_scan_bwd(d["x"], d["f"], d["dout"], states, z=d["z"], dlast=d["dlast"], workspace=ws)
+    for k, v in zip(("out", "last", "states", "dx", "df", "dz", "dinit"), (out, last, states) + got):
+        assert torch.equal(v, want[k]), k
+
+
+def test_operands_may_be_dropped_while_their_work_is_queued(dev):
+    """A call on a side stream that is still busy: the inputs are released and their memory is written again by the main
+    stream before the kernels run."""
+    x = inputs(1, 2000, 64, seed=12, dtype=torch.float32)
+    want = run(dev, x)["out"]
+    side = torch.cuda.Stream()
+    d = to(dev, x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+    out = ssm.gated_scan_fwd(d["x"], d["f"], d["z"], d["init"], stream=side)
+    shapes = {k: v.shape for k, v in d.items()}
+    d.clear()
+    again = [torch.full(s, float("nan"), device=dev) for s in shapes.values() for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and len(again) > 0
+
+
+def test_in_place(dev):
+    """out may be x, f or z: every element is read before its place is written, by the same lane."""
+    x = inputs(2, 700, 66, seed=13, dtype=torch.bfloat16)
+    want = run(dev, x)["out"]
+    for k in ("x", "f", "z"):
+        d = to(dev, x)
+        assert torch.equal(ssm.gated_scan_fwd(d["x"], d["f"], d["z"], d["init"], out=d[k]), want), k
+
+
 def test_gradients_against_differences():
     """The oracle's gradients against central differences of the float64 forward (step 1e-5: the difference's own
     error is about 1e-10 of the loss's third derivative, and 1e-16 / 1e-5 of its value)."""

@@ -1,0 +1,80 @@
+"""Operands past 2^31 elements and 2^32 bytes: every offset has to be 64 bits wide. The end of each is held to its
+definition, with the bounds of the operators' own tests."""
+import numpy as np
+import pytest
+import torch
+
+from helixml_amd import lm, ssm
+from tests.test_gated_gpu import CHUNK, HALF, check, f64, oracle_bwd, oracle_fwd
+from tests.test_logits_gpu import compare, oracle as logits_oracle
+from tests.test_w4_gpu import expand, rows
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def test_recurrence(dev):
+    """1 x 1050000 x 2050: 2.15e9 elements a tensor. The last steps follow from the state that was kept before them; the
+    gradients there follow from dlast."""
+    L, D, tail = 1050000, 2050, 300
+    g = torch.Generator(device=dev).manual_seed(0)
+    n = lambda *s: torch.randn(s, device=dev, generator=g, dtype=BF)  # noqa: E731
+    x, f = n(1, L, D), n(1, L, D)
+    out, last, states = ssm.gated_scan_fwd(x, f, return_last_state=True, return_states=True)
+    first = (L - tail) // CHUNK
+    t0 = first * CHUNK
+    pick = torch.tensor([0, 1, 63, 64, 1000, 2048, 2049], device=dev)
+    cut = lambda t: f64(t[:, t0:].index_select(2, pick).cpu())  # noqa: E731
+    at = lambda t: f64(t.index_select(1, pick).cpu())  # noqa: E731
+    init = f64(states[:, first].index_select(1, pick).cpu())
+    o = oracle_fwd(cut(x), cut(f), None, init)
+    check("out", out[:, t0:].index_select(2, pick), o["out"], o["out_E"], HALF[BF])
+    check("last", last.index_select(1, pick), o["last"], o["last_E"], 2.0 ** -24)
+    del out
+    dlast = torch.randn(1, D, device=dev, generator=g)
+    dout = n(1, L, D)
+    dx, df, _, dinit = ssm.gated_scan_bwd(x, f, dout, states, dlast=dlast)
+    b = oracle_bwd(cut(x), cut(f), cut(dout), None, init, at(dlast))
+    check("dx", dx[:, t0:].index_select(2, pick), b["dx"], b["dx_E"], HALF[BF])
+    check("df", df[:, t0:].index_select(2, pick), b["df"], b["df_E"], HALF[BF])
+    assert torch.isfinite(dinit).all()
+
+
+def test_step(dev):
+    """40000 x 55000: 2.2e9 channels in one step, the state past 8e9 bytes."""
+    bt, D = 40000, 55000
+    x = torch.randn(D, device=dev).to(BF).expand(bt, D).contiguous()
+    f = torch.randn(D, device=dev).to(BF).expand(bt, D).contiguous()
+    state = torch.full((bt, D), 0.5, device=dev)
+    out = ssm.gated_state_update(state, x, f)
+    r = lambda t: f64(t[:1].cpu())[:, None]  # noqa: E731
+    o = oracle_fwd(r(x), r(f), None, np.full((1, D), 0.5))
+    check("out", out[:1], o["out"][:, 0], o["out_E"][:, 0], HALF[BF])
+    for t in (1, bt // 2 + 1, bt - 1):
+        assert torch.equal(out[t], out[0]) and torch.equal(state[t], state[0])
+
+
+def test_weights(dev):
+    """3 x 270000 x 32768: 4.4e9 bytes of codes; outputs at the front, past 2^32 bytes and at the end."""
+    M, N, K = 3, 270000, 32768
+    pr, sr = rows(K)
+    packed = torch.randint(0, 256, (N, pr), device=dev, dtype=torch.uint8)
+    scales = torch.full((N, sr), 127, device=dev, dtype=torch.uint8)
+    X = torch.randint(-4, 5, (M, K)).to(BF)
+    got = ssm.linear_w4(X.to(dev), packed, scales, out_dtype=torch.float32)
+    for n in (0, 131072, 262143, 262144, N - 1):
+        want = X.double().numpy() @ expand(packed[n: n + 1].cpu(), scales[n: n + 1].cpu(), K).T
+        assert np.array_equal(got[:, n: n + 1].double().cpu().numpy(), want), n
+
+
+def test_logits(dev):
+    """16500 x 131072 bf16: 2.2e9 logits with bias and mask rows of their own stride."""
+    bt, V, H = 16500, 131072, 64
+    logits = torch.randn(bt, V, device=dev, dtype=BF)
+    history = torch.randint(0, V, (bt, H), device=dev, dtype=torch.int32)
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (bt, V // 32), device=dev, dtype=torch.int64).to(torch.int32)
+    rep = torch.full((bt,), 1.5, device=dev)
+    got = lm.adjust_logits(logits, history, repetition=rep, presence=rep, allowed=allowed)
+    for rows_at in (slice(0, 2), slice(16384, 16386), slice(bt - 2, bt)):
+        compare(got[rows_at], *logits_oracle(logits[rows_at].cpu(), history[rows_at].cpu(), repetition=rep[rows_at].cpu(),
+                                             presence=rep[rows_at].cpu(), allowed=allowed[rows_at].cpu()), BF)

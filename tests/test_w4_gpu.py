@@ -93,7 +93,7 @@ def test_linear_refusals():
 # ------------------------------------------------------------------ products (device)
 SIZES = [(1, 1, 1), (1, 16, 32), (1, 17, 33), (2, 5, 64), (3, 100, 31), (1, 256, 512), (5, 160, 4096), (16, 64, 128), (17, 48, 96),
          (33, 70, 1000), (64, 130, 544), (65, 33, 256), (130, 40, 160), (1, 1000, 2080), (7, 4100, 512), (4, 300, 777),
-         (2, 16400, 160), (6, 16390, 288), (16, 16400, 1100), (40, 16500, 640), (33, 16384, 96), (3, 32770, 264), (9, 4113, 1056)]
+         (2, 16400, 160), (6, 16390, 288), (16, 16400, 1100), (40, 16500, 640), (33, 16384, 96), (3, 32770, 264), (9, 4113, 1056), (20, 48, 4100), (31, 4120, 2500)]
 
 
 def random_weights(N, K, seed, lo=120, hi=130):
@@ -165,6 +165,31 @@ def test_every_scale_byte(dev, M, N, K):
     want = expand(packed, scales, K).T[at.numpy()]
     got = ssm.linear_w4(X.to(dev), packed.to(dev), scales.to(dev), out_dtype=torch.float32)
     assert np.array_equal(got.double().cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_no_inner_elements(dev):
+    """K = 0: the bias alone, or nothing."""
+    packed, scales = torch.empty(5, 0, device=dev, dtype=torch.uint8), torch.empty(5, 0, device=dev, dtype=torch.uint8)
+    X = torch.empty(3, 0, device=dev, dtype=torch.bfloat16)
+    b = torch.randn(5, device=dev)
+    assert torch.equal(ssm.linear_w4(X, packed, scales, bias=b, out_dtype=torch.float32), b.expand(3, 5))
+    assert (ssm.linear_w4(X, packed, scales, out_dtype=torch.float32) == 0).all()
+
+
+@pytest.mark.gpu
+def test_unaligned_rows_of_x(dev):
+    """Rows of X that start at any element, in a buffer whose other elements are NaN."""
+    M, N, K = 7, 60, 300
+    packed, scales = random_weights(N, K, 4)
+    scales[:, : -(-K // 32)] = 127
+    X = torch.randint(-8, 9, (M, K)).to(torch.bfloat16)
+    want = X.double().numpy() @ expand(packed, scales, K).T
+    for left, right in ((1, 0), (3, 2), (5, 8)):
+        buf = torch.full((M, K + left + right), float("nan"), device=dev, dtype=torch.bfloat16)
+        buf[:, left: left + K] = X.to(dev)
+        got = ssm.linear_w4(buf[:, left: left + K], packed.to(dev), scales.to(dev), out_dtype=torch.float32)
+        assert np.array_equal(got.double().cpu().numpy(), want)
 
 
 @pytest.mark.gpu
