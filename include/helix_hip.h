@@ -158,13 +158,17 @@ int hx_selective_state_update(int64_t batch, int64_t dim, int64_t dstate,
  * (1 - a is formed as sigmoid(-f), so closed and open gates keep their relative accuracy.)
  * The reference's recurrences (crates/nn/src/ssm.rs:138-186, :474-483) carry dstate states and no
  * gate per token; this is the elementwise member of the family and the only one with a gradient.
- * x, f, z, out: [batch, seqlen, dim] of `dtype`; init_state, last_state: [batch, dim] fp32.
+ * x, f, z, out: [batch, seqlen, dim] of `dtype` (out may be one of the others); init_state,
+ * last_state: [batch, dim] fp32. dim < 2^26, and batch * ceil(dim / 64) * ceil(seqlen / 128) < 2^31.
  * init_state (nullable) seeds h; last_state (nullable) receives h after the last step (init_state,
  * or zero, where seqlen is 0).
  * states (nullable): [batch, ceil(seqlen / HX_GATED_CHUNK), dim] fp32, receives h BEFORE steps 0,
  * HX_GATED_CHUNK, 2 * HX_GATED_CHUNK, ...: what hx_gated_scan_bwd forms h from again.
- * workspace: hx_gated_scan_workspace_size(...) bytes of device memory (0: none needed), 16-byte
- * aligned; it holds nothing between calls, and one call uses it at a time. */
+ * Steps are grouped (in tiles of 128), so results agree with the step-by-step recurrence to fp32
+ * rounding, the same bits on every call; a state that is infinite stays so or becomes NaN.
+ * workspace: hx_gated_scan_workspace_size(...) bytes of device memory (0 up to 128 steps: none
+ * needed), 16-byte aligned; it holds nothing between calls, and one call uses it at a time (calls
+ * that overlap on one workspace end, with undefined outputs). */
 #define HX_GATED_CHUNK 128
 size_t hx_gated_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype);
 int hx_gated_scan_fwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, const void* x,
@@ -288,8 +292,8 @@ int hx_gemm_bf16_splitk(int64_t M, int64_t N, int64_t K, const void* X, int64_t 
  * per HX_W4_GROUP = 32 elements along k. Row n of `packed` starts at n * 16 * G bytes, G = ceil(K / 32):
  * element 2j in the low and 2j + 1 in the high nibble of byte j, elements from K on unused. Row n of
  * `scales` starts at n * 16 * ceil(G / 16) bytes, group g's byte at g, bytes from G on unused. Scale
- * bytes 2..252 (2^-125 .. 2^125, what hx_w4_quantize writes) are exact; 255 is NaN; with 0, 1, 253 and
- * 254 a weight can leave the normal range of bf16 and then is flushed or overflows there. */
+ * bytes 0..252 are exact (hx_w4_quantize writes 2..252); with 253 and 254 a weight past bf16's largest
+ * number becomes an infinity; 255 is NaN and makes its row's outputs NaN. */
 #define HX_W4_GROUP 32
 /* Rounds weights w [N, K] (the Linear layout, row stride K) to that format, all three on the HOST: a
  * group's scale is the power of two that puts its largest magnitude into [4, 8) (clamped to the exact
@@ -302,7 +306,8 @@ int hx_w4_quantize(int64_t N, int64_t K, const float* w, void* packed, void* sca
  * packed and scales as above (device, 16-byte aligned), bias [N] fp32 (nullable), Y [M, N] of
  * out_dtype HX_F32 or HX_BF16 (row stride ldy); act as in hx_gemm_bf16 (bit 0 SiLU, bit 1 Y = Y + result).
  * Weights are expanded to bf16 exactly and multiplied on the matrix core with fp32 accumulation. Any
- * M, N, K; every X row gets the same arithmetic whatever M is. */
+ * M, N, K and any alignment of X and Y (K and ldx below 2^26, N below 2^34, M up to 32 * 65535, else
+ * HX_ERR_UNSUPPORTED); every X row gets the same arithmetic, bit for bit, whatever M is. */
 int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const void* packed,
                  const void* scales, const float* bias, int act, int out_dtype, void* Y,
                  int64_t ldy, void* stream);

@@ -157,14 +157,41 @@ def test_product_and_epilogue(dev, M, N, K, bias, act, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,N,K", [(3, 40, 100), (20, 64, 512), (1, 33, 2048)])
 def test_every_scale_byte(dev, M, N, K):
-    """Scale bytes 2..252 are exact powers of two (one nonzero activation a row: each output is one product)."""
-    packed, scales = random_weights(N, K, 5, 2, 253)
+    """Scale bytes 0..252 are exact powers of two (one nonzero activation a row: each output is one product)."""
+    packed, scales = random_weights(N, K, 5, 0, 253)
     X = torch.zeros(M, K, dtype=torch.bfloat16)
     at = torch.arange(M) * 31 % K
     X[torch.arange(M), at] = 1.0
     want = expand(packed, scales, K).T[at.numpy()]
     got = ssm.linear_w4(X.to(dev), packed.to(dev), scales.to(dev), out_dtype=torch.float32)
     assert np.array_equal(got.double().cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("byte", [253, 254])
+def test_scales_past_the_range_of_bf16(dev, byte):
+    """What bf16 cannot hold becomes an infinity of its sign."""
+    packed = torch.zeros(16, 16, dtype=torch.uint8)
+    packed[:, 0] = torch.arange(16, dtype=torch.uint8)
+    scales = torch.full((16, 16), 127, dtype=torch.uint8)
+    scales[:, 0] = byte
+    X = torch.zeros(1, 32, dtype=torch.bfloat16)
+    X[0, 0] = 2.0 ** -10
+    want = VALUES * 2.0 ** (byte - 127)
+    want = np.where(np.abs(want) < 2.0 ** 128, want, np.sign(want) * np.inf) * 2.0 ** -10
+    got = ssm.linear_w4(X.to(dev), packed.to(dev), scales.to(dev), out_dtype=torch.float32)[0]
+    assert np.array_equal(got.double().cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_subnormal_activations(dev):
+    """A product of a subnormal activation is that number's, not nought's."""
+    packed = torch.full((1, 16), 0x22, dtype=torch.uint8)  # ones
+    scales = torch.full((1, 16), 227, dtype=torch.uint8)  # 2^100
+    for e in (-126, -127, -130, -133):
+        X = torch.zeros(1, 32, dtype=torch.bfloat16)
+        X[0, 3] = 2.0 ** e
+        assert ssm.linear_w4(X.to(dev), packed.to(dev), scales.to(dev), out_dtype=torch.float32).item() == 2.0 ** (e + 100)
 
 
 @pytest.mark.gpu
