@@ -1,5 +1,7 @@
 // hx_gated.hip — the gated linear recurrence with one state per channel: forward, backward, one token.
 //   a = sigmoid(f), i = sigmoid(-f);  h_t = a_t h_{t-1} + i_t x_t;  out = h [silu(z)]
+#include <type_traits>
+
 #include "hx_common.h"
 
 namespace hx {
@@ -90,9 +92,10 @@ struct Place {
             Storage<T>::store(p + off, a);
         }
     }
+    __device__ inline bool whole() const { return __all(steps == kSteps); }  // the wave's rows are all there
     // All of the tile's loads of one operand, for the steps that exist.
     __device__ inline void load_all(const T* base, raw (&r)[kSteps]) const {
-        if (__all(steps == kSteps)) {
+        if (whole()) {
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) r[j] = load(base, j);
         } else {
@@ -269,22 +272,28 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void g
 
     float a0[kSteps], a1[kSteps], b0[kSteps], b1[kSteps];
     float A0 = 1.0f, A1 = 1.0f, H0 = 0.0f, H1 = 0.0f;
+    const auto open = [&](auto whole) {
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        float i0, i1;
-        gates(Pair<T>::lo(rf[j]), a0[j], i0);
-        gates(Pair<T>::hi(rf[j]), a1[j], i1);
-        b0[j] = i0 * Pair<T>::lo(rx[j]);
-        b1[j] = i1 * Pair<T>::hi(rx[j]);
-        if (j >= at.steps) {  // a step that is not there changes nothing
-            a0[j] = a1[j] = 1.0f;
-            b0[j] = b1[j] = 0.0f;
+        for (int j = 0; j < kSteps; ++j) {
+            float i0, i1;
+            gates(Pair<T>::lo(rf[j]), a0[j], i0);
+            gates(Pair<T>::hi(rf[j]), a1[j], i1);
+            b0[j] = i0 * Pair<T>::lo(rx[j]);
+            b1[j] = i1 * Pair<T>::hi(rx[j]);
+            if (!decltype(whole)::value && j >= at.steps) {  // a step that is not there changes nothing
+                a0[j] = a1[j] = 1.0f;
+                b0[j] = b1[j] = 0.0f;
+            }
+            H0 = fmaf(a0[j], H0, b0[j]);
+            H1 = fmaf(a1[j], H1, b1[j]);
+            A0 *= a0[j];
+            A1 *= a1[j];
         }
-        H0 = fmaf(a0[j], H0, b0[j]);
-        H1 = fmaf(a1[j], H1, b1[j]);
-        A0 *= a0[j];
-        A1 *= a1[j];
-    }
+    };
+    if (at.whole())
+        open(std::true_type{});
+    else
+        open(std::false_type{});
     const int part = wave * 2 + (lane >> 5), c = (lane & 31) * 2;
     *reinterpret_cast<float4*>(&maps[part][c]) = make_float4(A0, H0, A1, H1);
     __syncthreads();
@@ -359,19 +368,25 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
 
     float a0[kSteps], a1[kSteps], i0[kSteps], i1[kSteps];
     float A0 = 1.0f, A1 = 1.0f, H0 = 0.0f, H1 = 0.0f, G0 = 0.0f, G1 = 0.0f;
+    const auto open = [&](auto whole) {
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        gates(Pair<T>::lo(rf[j]), a0[j], i0[j]);
-        gates(Pair<T>::hi(rf[j]), a1[j], i1[j]);
-        if (j >= at.steps) {
-            a0[j] = a1[j] = 1.0f;
-            i0[j] = i1[j] = 0.0f;
+        for (int j = 0; j < kSteps; ++j) {
+            gates(Pair<T>::lo(rf[j]), a0[j], i0[j]);
+            gates(Pair<T>::hi(rf[j]), a1[j], i1[j]);
+            if (!decltype(whole)::value && j >= at.steps) {
+                a0[j] = a1[j] = 1.0f;
+                i0[j] = i1[j] = 0.0f;
+            }
+            H0 = fmaf(a0[j], H0, i0[j] * Pair<T>::lo(rx[j]));
+            H1 = fmaf(a1[j], H1, i1[j] * Pair<T>::hi(rx[j]));
+            A0 *= a0[j];
+            A1 *= a1[j];
         }
-        H0 = fmaf(a0[j], H0, i0[j] * Pair<T>::lo(rx[j]));
-        H1 = fmaf(a1[j], H1, i1[j] * Pair<T>::hi(rx[j]));
-        A0 *= a0[j];
-        A1 *= a1[j];
-    }
+    };
+    if (at.whole())
+        open(std::true_type{});
+    else
+        open(std::false_type{});
 #pragma unroll
     for (int j = kSteps - 1; j >= 0; --j) {
         float d0 = Pair<T>::lo(rd[j]), d1 = Pair<T>::hi(rd[j]);

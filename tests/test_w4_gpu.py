@@ -178,7 +178,7 @@ def test_scales_past_the_range_of_bf16(dev, byte):
     X = torch.zeros(1, 32, dtype=torch.bfloat16)
     X[0, 0] = 2.0 ** -10
     want = VALUES * 2.0 ** (byte - 127)
-    want = np.where(np.abs(want) < 2.0 ** 128, want, np.sign(want) * np.inf) * 2.0 ** -10
+    want = np.where(np.abs(want) < 2.0 ** 128, want, np.copysign(np.inf, want)) * 2.0 ** -10
     got = ssm.linear_w4(X.to(dev), packed.to(dev), scales.to(dev), out_dtype=torch.float32)[0]
     assert np.array_equal(got.double().cpu().numpy(), want)
 
