@@ -232,7 +232,7 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
 // Which tile this block takes: tickets are handed out in the order in which blocks start, tile 0 of every column
 // first, so what a block waits for is always held by a block that has started.
 __device__ inline bool take_unit(const Chain& c, uint32_t& shared_unit, int& k, uint32_t& col) {
-    uint32_t unit = blockIdx.x;
+    uint32_t unit = blockIdx.y * gridDim.x + blockIdx.x;
     if (c.tiles > 1) {
         if (threadIdx.x == 0) shared_unit = atomicAdd(c.ticket, 1u);
         __syncthreads();
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void g
     __syncthreads();
     const float2 start = *reinterpret_cast<const float2*>(&entries[part][c]);
     float h0 = start.x, h1 = start.y;
-    if (GATE) {
+    if (GATE) {  // silu(z) is formed here, not carried through the wait
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) Pair<T>::hold(rz[j]);
     }
@@ -480,10 +480,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
 
 // Every word of the workspace absent, the ticket at its start.
 __global__ __launch_bounds__(256) void gated_chain_clear_kernel(uint4* ws, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const uint32_t v = i == 0 ? 0 : 0xffffffffu;
-    ws[i] = make_uint4(v, v, v, v);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const uint32_t v = i == 0 ? 0 : 0xffffffffu;
+        ws[i] = make_uint4(v, v, v, v);
+    }
 }
 
 // One token: four channels a thread (16 bytes of state), bound by the state's read and write; the last n % 4 channels
@@ -505,9 +505,8 @@ __device__ inline void step_run(int64_t o, float* state, const T* x, const T* f,
     y.store(out + o);
 }
 template <typename T>
-__global__ __launch_bounds__(256) void gated_step_kernel(int64_t n, float* __restrict__ state, const T* __restrict__ x,
-                                                         const T* __restrict__ f, const T* __restrict__ z,
-                                                         T* __restrict__ out) {
+__global__ __launch_bounds__(256) void gated_step_kernel(int64_t n, float* state, const T* x, const T* f, const T* z,
+                                                         T* out) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, runs = n / 4;
     if (t < runs)
         step_run<T, 4>(4 * t, state, x, f, z, out);
@@ -518,21 +517,29 @@ __global__ __launch_bounds__(256) void gated_step_kernel(int64_t n, float* __res
 // dst = src, or zero: what is left of a sequence without steps.
 __global__ __launch_bounds__(256) void gated_state_copy_kernel(int64_t n, const float* __restrict__ src,
                                                                float* __restrict__ dst) {
-    const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (o < n) dst[o] = src ? src[o] : 0.0f;
+    for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < n; o += (int64_t)gridDim.x * 256) dst[o] = src ? src[o] : 0.0f;
 }
 
-constexpr int64_t kMaxBlocks = 0x7fffffff;  // of one grid axis
+// A grid axis counts its threads in 32 bits: kernels over many elements loop, kernels over many tiles take two axes.
+constexpr int64_t kMaxBlocks = 0x7fffffff, kAxis = 1 << 20;
+inline dim3 looped(int64_t n) {
+    const int64_t blocks = (n + 255) / 256;
+    return dim3((unsigned)(blocks < kAxis ? blocks : kAxis));
+}
 
 struct Shape {
     int64_t batch, L, D, cols, tiles, units;
     Shape(int64_t batch_, int64_t L_, int64_t D_)
-        : batch(batch_), L(L_), D(D_), cols((D_ + kWidth - 1) / kWidth), tiles((L_ + kTile - 1) / kTile),
+        : batch(batch_), L(L_), D(D_), cols(D_ / kWidth + (D_ % kWidth != 0)), tiles(L_ / kTile + (L_ % kTile != 0)),
           units(fits() ? batch_ * cols * tiles : 0) {}
     // Byte offsets of 63 bits, a lane's offset inside its wave's rows of 32, one block a tile.
     bool fits() const {
         return batch < kMaxBlocks && D < (1 << 26) && L < ((int64_t)1 << 37) &&
                (__int128)batch * cols * (tiles > 0 ? tiles : 1) < kMaxBlocks && (__int128)batch * L * D < ((__int128)1 << 60);
+    }
+    dim3 grid() const {
+        const int64_t x = units < kAxis ? units : kAxis;
+        return dim3((unsigned)x, (unsigned)((units + x - 1) / x));
     }
     // 16 bytes for the ticket, a word per channel of each tile and group; one tile waits for nobody
     int64_t groups() const { return (tiles + kGroup - 1) / kGroup; }
@@ -546,14 +553,14 @@ struct Shape {
 int clear_chain(const Shape& g, void* ws, hipStream_t s) {
     if (g.tiles <= 1) return HX_OK;
     const int64_t n = (int64_t)(g.workspace() / 16);
-    hipLaunchKernelGGL(gated_chain_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (uint4*)ws, n);
+    hipLaunchKernelGGL(gated_chain_clear_kernel, looped(n), dim3(256), 0, s, (uint4*)ws, n);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
 
 int copy_state(int64_t rows, const float* src, float* dst, hipStream_t s) {
     if (!dst) return HX_OK;
-    hipLaunchKernelGGL(gated_state_copy_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, rows, src, dst);
+    hipLaunchKernelGGL(gated_state_copy_kernel, looped(rows), dim3(256), 0, s, rows, src, dst);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
@@ -562,7 +569,7 @@ template <typename T>
 int fwd(const Shape& g, const FwdArgs& p, hipStream_t s) {
     const auto k = g.D % 2 == 0 ? (p.z ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
                              : (p.z ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
-    hipLaunchKernelGGL(k, dim3((unsigned)g.units), dim3(64 * kWaves), 0, s, p);
+    hipLaunchKernelGGL(k, g.grid(), dim3(64 * kWaves), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
@@ -571,7 +578,7 @@ template <typename T>
 int bwd(const Shape& g, const BwdArgs& p, hipStream_t s) {
     const auto k = g.D % 2 == 0 ? (p.z ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
                              : (p.z ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
-    hipLaunchKernelGGL(k, dim3((unsigned)g.units), dim3(64 * kWaves), 0, s, p);
+    hipLaunchKernelGGL(k, g.grid(), dim3(64 * kWaves), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
@@ -640,7 +647,7 @@ extern "C" int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, floa
     HX_REQUIRE(batch >= 0 && dim >= 0, HX_ERR_INVALID_DIMENSION, "gated_state_update: negative size");
     HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, HX_ERR_DTYPE_MISMATCH, "gated_state_update: dtype %d", dtype);
     if (batch == 0 || dim == 0) return HX_OK;
-    HX_REQUIRE((__int128)batch * dim < (__int128)256 * kMaxBlocks, HX_ERR_UNSUPPORTED, "gated_state_update: too many elements");
+    HX_REQUIRE((__int128)batch * dim < ((__int128)1 << 33), HX_ERR_UNSUPPORTED, "gated_state_update: too many elements");
     HX_REQUIRE(state && x && f && out, HX_ERR_INVALID_INPUT, "gated_state_update: state, x, f and out are required");
     const int64_t n = batch * dim, threads = n / 4 + n % 4;
     dim3 grid((unsigned)((threads + 255) / 256));

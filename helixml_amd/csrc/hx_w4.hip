@@ -329,8 +329,8 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
                "linear_w4: X, packed, scales and Y required, ldx >= K, ldy >= N");
     HX_REQUIRE(aligned(packed, 16) && aligned(scales, 16), HX_ERR_INVALID_INPUT,
                "linear_w4: packed and scales must be 16-byte aligned");
-    HX_REQUIRE(N < ((int64_t)1 << 34) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26) && ldx < (1 << 26),
-               HX_ERR_UNSUPPORTED, "linear_w4: at most %d rows of X, 2^34 outputs, K and ldx below 2^26", kRowsAtOnce * 65535);
+    HX_REQUIRE(N < (1 << 30) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26) && ldx < (1 << 26),
+               HX_ERR_UNSUPPORTED, "linear_w4: at most %d rows of X, N below 2^30, K and ldx below 2^26", kRowsAtOnce * 65535);
     // How K is cut decides the order of the sums, so it goes by N and K alone: up to 8 waves a tile of 16 outputs while there
     // are fewer than 8 for each of 256 CUs, or 16 where a wave would walk more than 8 windows, none with fewer than two.
     // 1 x 2048 x 4096: 8 waves 4.4 us, 4 waves 4.7, 2 waves 6.1; 2 x 16384 x 4096: 4 waves 11.1, 8 waves 12.2; 1 x 16384 x

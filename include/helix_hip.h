@@ -190,7 +190,7 @@ int hx_gated_scan_bwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, con
                       const float* dlast, void* dx, void* df, void* dz, float* dinit,
                       void* workspace, size_t workspace_bytes, void* stream);
 /* One token of that recurrence for every sequence: state [batch, dim] fp32 is advanced in place;
- * x, f, z (nullable), out: [batch, dim] of `dtype`. */
+ * x, f, z (nullable), out: [batch, dim] of `dtype` (out may be one of the others), batch * dim < 2^33. */
 int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, const void* x,
                           const void* f, const void* z, void* out, void* stream);
 
@@ -306,7 +306,7 @@ int hx_w4_quantize(int64_t N, int64_t K, const float* w, void* packed, void* sca
  * packed and scales as above (device, 16-byte aligned), bias [N] fp32 (nullable), Y [M, N] of
  * out_dtype HX_F32 or HX_BF16 (row stride ldy); act as in hx_gemm_bf16 (bit 0 SiLU, bit 1 Y = Y + result).
  * Weights are expanded to bf16 exactly and multiplied on the matrix core with fp32 accumulation. Any
- * M, N, K and any alignment of X and Y (K and ldx below 2^26, N below 2^34, M up to 32 * 65535, else
+ * M, N, K and any alignment of X and Y (K and ldx below 2^26, N below 2^30, M up to 32 * 65535, else
  * HX_ERR_UNSUPPORTED); every X row gets the same arithmetic, bit for bit, whatever M is. */
 int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const void* packed,
                  const void* scales, const float* bias, int act, int out_dtype, void* Y,

@@ -31,6 +31,9 @@ def test_sizes_and_types():
         assert call(bt=0) == 0 and call(dim=0) == 0
     for call in (fwd, bwd):
         assert call(L=-1) == _ffi.InvalidDimension.status
+        assert call(L=2 ** 63 - 1) == _ffi.UnsupportedOperation.status
+        assert call(dim=2 ** 63 - 1) == _ffi.UnsupportedOperation.status
+        assert call(bt=2 ** 63 - 1) == _ffi.UnsupportedOperation.status
         assert call(L=2 ** 62) == _ffi.UnsupportedOperation.status
         assert call(L=0, x=None, f=None) == 0  # no steps, no state wanted: nothing to do
 

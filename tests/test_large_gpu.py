@@ -40,6 +40,25 @@ def test_recurrence(dev):
     assert torch.isfinite(dinit).all()
 
 
+@pytest.mark.parametrize("bt,L,D", [(9000000, 2, 3), (4300000, 130, 1)])
+def test_more_tiles_than_one_grid_axis_takes(dev, bt, L, D):
+    """More than 2^23 tiles of 512 threads: rows of the first, middle and last sequences."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    n = lambda *s: torch.randn(s, device=dev, generator=g, dtype=BF)  # noqa: E731
+    x, f, dout = n(bt, L, D), n(bt, L, D), n(bt, L, D)
+    init = torch.randn(bt, D, device=dev, generator=g)
+    out, last, states = ssm.gated_scan_fwd(x, f, None, init, return_last_state=True, return_states=True)
+    dx, df, _, dinit = ssm.gated_scan_bwd(x, f, dout, states)
+    pick = torch.tensor([0, 1, bt // 2, bt - 2, bt - 1], device=dev)
+    r = lambda t: f64(t[pick].cpu())  # noqa: E731
+    o, b = oracle_fwd(r(x), r(f), None, r(init)), oracle_bwd(r(x), r(f), r(dout), None, r(init))
+    check("out", out[pick], o["out"], o["out_E"], HALF[BF])
+    check("last", last[pick], o["last"], o["last_E"], 2.0 ** -24)
+    check("dx", dx[pick], b["dx"], b["dx_E"], HALF[BF])
+    check("df", df[pick], b["df"], b["df_E"], HALF[BF])
+    check("dinit", dinit[pick], b["dinit"], b["dinit_E"], 2.0 ** -24)
+
+
 def test_step(dev):
     """40000 x 55000: 2.2e9 channels in one step, the state past 8e9 bytes."""
     bt, D = 40000, 55000

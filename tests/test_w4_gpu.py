@@ -88,6 +88,8 @@ def test_linear_refusals():
     assert call(W=ctypes.c_void_p(4104)) == _ffi.InvalidInput.status
     assert call(S=ctypes.c_void_p(4097)) == _ffi.InvalidInput.status
     assert call(M=0) == 0 and call(N=0) == 0
+    for big in (dict(N=2 ** 30, ldy=2 ** 30), dict(M=32 * 65535 + 1), dict(K=2 ** 26, ldx=2 ** 26), dict(ldx=2 ** 26)):
+        assert call(**big) == _ffi.UnsupportedOperation.status
 
 
 # ------------------------------------------------------------------ products (device)
