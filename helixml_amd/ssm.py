@@ -236,6 +236,8 @@ def _gated_workspace(name, given, batch, seqlen, dim, dtype, device):
     need = int(getattr(_ffi.lib(), name)(batch, seqlen, dim, _STORAGE[dtype]))
     if need and given is None:
         given = torch.empty(need, device=device, dtype=torch.uint8)
+    elif given is not None and not given.is_contiguous():
+        raise InvalidInput("workspace must be contiguous")
     return (None, 0) if given is None else (given, given.numel() * given.element_size())
 
 

@@ -378,6 +378,31 @@ def test_captured_and_replayed(dev):
             assert torch.equal(a, b), (seed, n)
 
 
+def test_two_graphs_share_a_workspace(dev):
+    """A forward and a backward captured apart on one workspace, of different sizes, replayed in turn on one stream."""
+    xa, xb = (to(dev, inputs(1, L, d, seed=s, dtype=torch.float32)) for L, d, s in ((2500, 70, 41), (900, 200, 42)))
+    n = max(ssm.gated_scan_workspace_size(1, 2500, 70), ssm.gated_scan_workspace_size(1, 900, 200, backward=True))
+    ws = torch.empty(n, device=dev, dtype=torch.uint8)
+    st = ssm.gated_scan_fwd(xb["x"], xb["f"], xb["z"], xb["init"], return_states=True)[1]
+    calls = (lambda: (ssm.gated_scan_fwd(xa["x"], xa["f"], xa["z"], xa["init"], workspace=ws),),
+             lambda: ssm.gated_scan_bwd(xb["x"], xb["f"], xb["dout"], st, z=xb["z"], dlast=xb["dlast"], workspace=ws))
+    want = [[t.clone() for t in c()] for c in calls]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(c())
+        graphs.append(g)
+    for _ in range(3):
+        for n in (0, 1, 1, 0):
+            for t in held[n]:
+                t.zero_()
+            graphs[n].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held[n], want[n])), n
+
+
 def test_two_streams_at_once(dev):
     """Calls on two streams, each with its own inputs, give what they give alone."""
     xs = [to(dev, inputs(1, 4000, 96, seed=s, dtype=torch.float32)) for s in (31, 32)]
@@ -391,6 +416,10 @@ def test_two_streams_at_once(dev):
     for pair in got:
         for (o, l), (ro, rl) in zip(pair, alone):
             assert torch.equal(o, ro) and torch.equal(l, rl)
+    # a raw handle works the same way
+    raw = ssm.gated_scan_fwd(xs[0]["x"], xs[0]["f"], xs[0]["z"], xs[0]["init"], stream=streams[0].cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(raw, alone[0][0])
 
 
 def test_refusals(dev):
@@ -410,7 +439,12 @@ def test_refusals(dev):
     with pytest.raises(_ffi.ShapeMismatch):
         ssm.gated_state_update(torch.zeros(2, 5, device=dev), x[:, 0].contiguous(), x[:, 0].contiguous())
     need = ssm.gated_scan_workspace_size(1, 100000, 4)
-    if need:
-        big = torch.zeros(1, 100000, 4, device=dev)
+    assert need > 0
+    big = torch.zeros(1, 100000, 4, device=dev)
+    for ws in (torch.empty(need - 1, device=dev, dtype=torch.uint8), torch.empty(1, device=dev, dtype=torch.uint8).expand(need)):
         with pytest.raises(_ffi.InvalidInput):
-            ssm.gated_scan_fwd(big, big, workspace=torch.empty(need - 1, device=dev, dtype=torch.uint8))
+            ssm.gated_scan_fwd(big, big, workspace=ws)
+        with pytest.raises(_ffi.InvalidInput):
+            ssm.gated_scan_bwd(big, big, big, torch.zeros(1, 782, 4, device=dev), workspace=ws)
+    with pytest.raises(_ffi.DeviceMismatch):
+        ssm.gated_scan_fwd(big, big, workspace=torch.empty(need, dtype=torch.uint8))
