@@ -105,7 +105,7 @@ struct Place {
     }
 };
 
-// The workspace: a ticket, then 64-bit words, all ones while there is nothing: one for each tile and channel, the tile's
+// The workspace: tickets, then 64-bit words, all ones while there is nothing: one for each tile and channel, the tile's
 // map (A, H); one for each group of kGroup tiles, the group's map, then its exit state (kExit, h). Each word is written
 // whole and says itself what it is, so no fence is needed, only that readers and writers meet beyond the L2 of their XCD
 // (agent scope).
@@ -114,10 +114,11 @@ struct Place {
 //   entry of a group = the nearest exit that is there, and the maps of the groups after it applied in turn.
 // What is applied to what does not depend on which words were there first, so neither do the bits.
 struct Chain {
-    uint32_t* ticket;
+    uint32_t* tickets;
     unsigned long long *tiles_at, *groups_at;
     int tiles;       // of one sequence
     uint32_t lanes;  // sequences x column tiles
+    uint32_t together;  // neighbouring columns that share a counter
 };
 constexpr unsigned long long kAbsent = ~0ull;
 constexpr uint32_t kExit = 0xfffffffeu, kNaN = 0x7fc00000u;
@@ -229,17 +230,27 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
     return e;
 }
 
-// Which tile this block takes: tickets are handed out in the order in which blocks start, tile 0 of every column
-// first, so what a block waits for is always held by a block that has started.
-__device__ inline bool take_unit(const Chain& c, uint32_t& shared_unit, int& k, uint32_t& col) {
-    uint32_t unit = blockIdx.y * gridDim.x + blockIdx.x;
-    if (c.tiles > 1) {
-        if (threadIdx.x == 0) shared_unit = atomicAdd(c.ticket, 1u);
-        __syncthreads();
-        unit = __builtin_amdgcn_readfirstlane(shared_unit);
-    }
+// Which tile this block takes: tickets are handed out in the order in which blocks start, tile 0 of every column first, so
+// what a block waits for is always held by a block that has started. Adding to one word takes the chip about 13.5 ns a
+// block, all blocks in turn (1 x 65536 x 2048 bf16 took 227 us for it alone), so the columns are dealt in runs to up to
+// kCounters words of lines of their own; a column's tiles all come from one of them. Runs of kTogether neighbours, since
+// columns that drift apart share no DRAM page: 1 x 65536 x 2048 fp32 335 us with runs of one, 310 from four on; bf16 230,
+// 208 with four, 204 with eight, 226 with all 32 columns on one word; 1 x 1999 x 768 11.5, 11.8, 12.2 and 12.9.
+constexpr uint32_t kCounters = 64, kCounterStride = 32, kTogether = 8;
+__device__ inline bool take_unit(const Chain& c, uint32_t& shared_ticket, int& k, uint32_t& col) {
+    const uint32_t unit = blockIdx.y * gridDim.x + blockIdx.x;
     k = (int)(unit / c.lanes);
     col = unit - (uint32_t)k * c.lanes;
+    if (k >= c.tiles) return false;
+    if (c.tiles > 1) {
+        const uint32_t mine = col / c.together, first = mine * c.together;
+        if (threadIdx.x == 0) shared_ticket = atomicAdd(c.tickets + mine * kCounterStride, 1u);
+        __syncthreads();
+        const uint32_t ticket = __builtin_amdgcn_readfirstlane(shared_ticket);
+        const uint32_t columns = c.lanes - first < c.together ? c.lanes - first : c.together;
+        k = (int)(ticket / columns);
+        col = first + ticket - (uint32_t)k * columns;
+    }
     return k < c.tiles;
 }
 
@@ -258,10 +269,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void g
     __shared__ float2 maps[kParts][kWidth];
     __shared__ float entries[kParts][kWidth];
     __shared__ Looked seen;
-    __shared__ uint32_t shared_unit;
+    __shared__ uint32_t shared_ticket;
     int k;
     uint32_t col;
-    if (!take_unit(p.chain, shared_unit, k, col)) return;
+    if (!take_unit(p.chain, shared_ticket, k, col)) return;
     const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const Place<T, EVEN> at(b, (int64_t)k * kTile, c0, wave, lane, p.L, p.D);
@@ -352,10 +363,10 @@ template <typename T, bool EVEN, bool GATE>
 __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs p) {
     __shared__ float maps_a[kParts][kWidth], maps_h[kParts][kWidth], maps_g[kParts][kWidth];
     __shared__ Looked seen;
-    __shared__ uint32_t shared_unit;
+    __shared__ uint32_t shared_ticket;
     int k;
     uint32_t col;
-    if (!take_unit(p.chain, shared_unit, k, col)) return;
+    if (!take_unit(p.chain, shared_ticket, k, col)) return;
     const int tile = p.chain.tiles - 1 - k;
     const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -478,10 +489,11 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
     }
 }
 
-// Every word of the workspace absent, the ticket at its start.
+// Every word of the workspace absent, the tickets at their start.
+constexpr size_t kTicketBytes = kCounters * kCounterStride * sizeof(uint32_t);
 __global__ __launch_bounds__(256) void gated_chain_clear_kernel(uint4* ws, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const uint32_t v = i == 0 ? 0 : 0xffffffffu;
+        const uint32_t v = i < (int64_t)(kTicketBytes / sizeof(uint4)) ? 0 : 0xffffffffu;
         ws[i] = make_uint4(v, v, v, v);
     }
 }
@@ -541,12 +553,17 @@ struct Shape {
         const int64_t x = units < kAxis ? units : kAxis;
         return dim3((unsigned)x, (unsigned)((units + x - 1) / x));
     }
-    // 16 bytes for the ticket, a word per channel of each tile and group; one tile waits for nobody
+    int64_t together() const {
+        const int64_t share = (batch * cols + kCounters - 1) / kCounters;
+        return share > kTogether ? share : kTogether;
+    }
+    // The tickets, a word per channel of each tile and group; one tile waits for nobody
     int64_t groups() const { return (tiles + kGroup - 1) / kGroup; }
-    size_t workspace() const { return tiles > 1 ? 16 + ((size_t)units + groups() * batch * cols) * kWidth * 8 : 0; }
+    size_t workspace() const { return tiles > 1 ? kTicketBytes + ((size_t)units + groups() * batch * cols) * kWidth * 8 : 0; }
     Chain chain(void* ws) const {
-        unsigned long long* const words = (unsigned long long*)((char*)ws + 16);
-        return Chain{(uint32_t*)ws, words, words + (size_t)units * kWidth, (int)tiles, (uint32_t)(batch * cols)};
+        unsigned long long* const words = (unsigned long long*)((char*)ws + kTicketBytes);
+        return Chain{(uint32_t*)ws, words, words + (size_t)units * kWidth, (int)tiles, (uint32_t)(batch * cols),
+                     (uint32_t)together()};
     }
 };
 
