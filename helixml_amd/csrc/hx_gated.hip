@@ -29,12 +29,18 @@ __device__ inline void silu_grad(float z, float& v, float& d) {
 
 // ------------------------------------------------------------------ tiles
 // A block owns a tile of kTile steps x 64 channels of one sequence. Lane (half, c) of wave w holds channels
-// 2c and 2c+1 of the kSteps consecutive steps of part p = 2w + half, so a row of the tile is one 128-byte (bf16)
+// 2c and 2c+1 of the S consecutive steps of part p = 2w + half, so a row of the tile is one 128-byte (bf16)
 // or 256-byte (fp32) run and every element is read once and stays in registers. A part is the affine map
 // h -> A h + H (A the product of its gates); the tile's parts are joined in LDS and the tiles of a sequence
 // through the workspace (see Chain): a tile publishes its map as soon as it has it.
-constexpr int kSteps = 8, kWaves = 8, kParts = 2 * kWaves, kTile = kParts * kSteps, kWidth = 64;
-static_assert(kTile == HX_GATED_CHUNK, "a tile's entry state is one of `states`");
+constexpr int kTile = HX_GATED_CHUNK, kWidth = 64;  // a tile's entry state is one of `states`
+// Steps of a lane: as many as fit the registers of four waves a SIMD, since a tile of fewer waves has fewer parts to join
+// and a CU holds more such tiles. bf16 forward 16 (tiles of 4 waves) against 8 (of 8): 1 x 65536 x 2048 184 us against 204
+// ungated, 242 against 256 gated; 8 x 2048 x 1536 42 against 44, 51 against 53; one tile to a sequence, 3 x 124 x 899, 6.9
+// against 5.9. With 16, fp32 spills: 348 us against 300 ungated at 1 x 65536 x 2048. The backward pass holds twice as much.
+template <typename T> constexpr int kForwardSteps = sizeof(T) == 2 ? 16 : 8;
+constexpr int kBackwardSteps = 8;
+template <int S> constexpr int kWaves = kTile / (2 * S);
 
 // Two neighbouring channels as they are stored, at any address that an element may have: rows of odd width start anywhere.
 template <typename T> struct Pair;
@@ -57,7 +63,7 @@ template <> struct Pair<uint16_t> {
 };
 
 // Where a lane's elements lie. EVEN: an even number of channels, so that every pair is whole.
-template <typename T, bool EVEN>
+template <typename T, bool EVEN, int S>
 struct Place {
     using raw = typename Pair<T>::raw;
     int64_t row;   // of the wave's first step, its first channel (uniform)
@@ -68,10 +74,10 @@ struct Place {
 
     __device__ Place(int64_t b, int64_t t0, int64_t c0, int wave, int lane, int64_t L, int64_t dim) : D(dim) {
         const int half = lane >> 5, c = (lane & 31) * 2;
-        row = (b * L + t0 + wave * 2 * kSteps) * D + c0;
-        off = (uint32_t)(half * kSteps * D + c);
-        const int64_t left = L - t0 - (wave * 2 + half) * kSteps;
-        steps = c0 + c < D ? (int)(left < 0 ? 0 : left < kSteps ? left : kSteps) : 0;
+        row = (b * L + t0 + wave * 2 * S) * D + c0;
+        off = (uint32_t)(half * S * D + c);
+        const int64_t left = L - t0 - (wave * 2 + half) * S;
+        steps = c0 + c < D ? (int)(left < 0 ? 0 : left < S ? left : S) : 0;
         second = EVEN || c0 + c + 1 < D;
     }
     __device__ inline raw load(const T* base, int j) const {
@@ -92,15 +98,15 @@ struct Place {
             Storage<T>::store(p + off, a);
         }
     }
-    __device__ inline bool whole() const { return __all(steps == kSteps); }  // the wave's rows are all there
+    __device__ inline bool whole() const { return __all(steps == S); }  // the wave's rows are all there
     // All of the tile's loads of one operand, for the steps that exist.
-    __device__ inline void load_all(const T* base, raw (&r)[kSteps]) const {
+    __device__ inline void load_all(const T* base, raw (&r)[S]) const {
         if (whole()) {
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) r[j] = load(base, j);
+            for (int j = 0; j < S; ++j) r[j] = load(base, j);
         } else {
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) r[j] = j < steps ? load(base, j) : raw{};
+            for (int j = 0; j < S; ++j) r[j] = j < steps ? load(base, j) : raw{};
         }
     }
 };
@@ -122,7 +128,7 @@ struct Chain {
 };
 constexpr unsigned long long kAbsent = ~0ull;
 constexpr uint32_t kExit = 0xfffffffeu, kNaN = 0x7fc00000u;
-constexpr int kGroup = 16, kMine = kGroup / kWaves;
+constexpr int kGroup = 16;
 // A wait ends by itself where the workspace is misused (two calls at once): some 10^5 looks of about a microsecond.
 constexpr int kLooks = 1 << 17;
 
@@ -143,20 +149,23 @@ __device__ inline unsigned long long look_at(const unsigned long long* word) {
 __device__ inline float map_a(unsigned long long m) { return __uint_as_float((uint32_t)m); }
 __device__ inline float map_h(unsigned long long m) { return __uint_as_float((uint32_t)(m >> 32)); }
 
-// What the block's waves have seen: the maps of the tiles before theirs in the group, the words of the kWaves groups
+// What the block's waves have seen: the maps of the tiles before theirs in the group, the words of the W groups
 // before it.
+template <int W>
 struct Looked {
-    unsigned long long tiles[kGroup][kWidth], groups[kWaves][kWidth];
-    int found[kWaves];
+    unsigned long long tiles[kGroup][kWidth], groups[W][kWidth];
+    int found[W];
 };
 constexpr int kNoMap = 1, kGroupExit = 2, kGroupAbsent = 4;
 
 // The state that tile k of a chain starts from, in wave 0's lanes; `first` is the chain's own, (A, H) the tile's map. The
-// waves look together, two tiles and one group each: the maps of a group are all there about when the tile's own is, and a
-// chain of many tiles moves on by kWaves groups, 16384 steps, a look. 1 x 42983 x 70 bf16 takes 28 us; with a window of 8
-// tiles and an exit state for every tile it took 73.
+// W waves look together, a share of the tiles and one group each: the maps of a group are all there about when the tile's own
+// is, and a chain of many tiles moves on by W groups, 8192 steps or 16384, a look. 1 x 42983 x 70 bf16 takes 26 us; with a
+// window of 8 tiles and an exit state for every tile it took 73.
+template <int W>
 __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, int lane, float first, float A, float H,
-                                 Looked& seen) {
+                                 Looked<W>& seen) {
+    constexpr int kMine = kGroup / W;
     const int group = k / kGroup, place = k % kGroup;
     const bool closes = place == kGroup - 1 && k + 1 < c.tiles;
     if (wave == 0 && k + 1 < c.tiles) publish_map(words_of(c.tiles_at, c, k, col) + lane, A, H);
@@ -166,7 +175,7 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
     for (int look = 0; look < kLooks; ++look) {
         int found = 0;
         unsigned long long m[kMine], w = 0;
-        const int from = group - kWaves + wave;
+        const int from = group - W + wave;
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
             if (!held && wave * kMine + i < place) m[i] = look_at(words_of(c.tiles_at, c, k - place + wave * kMine + i, col) + lane);
@@ -189,7 +198,7 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
         bool maps = true;
         start = -1;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
+        for (int i = 0; i < W; ++i) {
             const int f = seen.found[i];
             maps = maps && !(f & kNoMap);
             if (f & kGroupExit) start = i;
@@ -209,7 +218,7 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
                 publish_map(words_of(c.groups_at, c, group, col) + lane, GA, GH);
             }
         }
-        ok = maps && (start > absent || (absent < 0 && group <= kWaves));  // or the look reaches the chain's start
+        ok = maps && (start > absent || (absent < 0 && group <= W));  // or the look reaches the chain's start
         if (ok) break;
         __syncthreads();
         __builtin_amdgcn_s_sleep(1);
@@ -217,7 +226,7 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
     if (wave != 0) return 0.0f;
     float e = ok ? first : __uint_as_float(kNaN);
     if (ok)
-        for (int i = start >= 0 ? start : kWaves - (group < kWaves ? group : kWaves); i < kWaves; ++i) {
+        for (int i = start >= 0 ? start : W - (group < W ? group : W); i < W; ++i) {
             const unsigned long long g = seen.groups[i][lane];
             e = (uint32_t)g == kExit ? map_h(g) : fmaf(map_a(g), e, map_h(g));
         }
@@ -265,17 +274,18 @@ struct FwdArgs {
 };
 
 template <typename T, bool EVEN, bool GATE>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void gated_fwd_kernel(const FwdArgs p) {
+__global__ __launch_bounds__(64 * kWaves<kForwardSteps<T>>, sizeof(T) == 4 && !GATE ? 6 : 4) void gated_fwd_kernel(const FwdArgs p) {
+    constexpr int kSteps = kForwardSteps<T>, W = kWaves<kSteps>, kParts = 2 * W;
     __shared__ float2 maps[kParts][kWidth];
     __shared__ float entries[kParts][kWidth];
-    __shared__ Looked seen;
+    __shared__ Looked<W> seen;
     __shared__ uint32_t shared_ticket;
     int k;
     uint32_t col;
     if (!take_unit(p.chain, shared_ticket, k, col)) return;
     const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const Place<T, EVEN> at(b, (int64_t)k * kTile, c0, wave, lane, p.L, p.D);
+    const Place<T, EVEN, kSteps> at(b, (int64_t)k * kTile, c0, wave, lane, p.L, p.D);
     typename Pair<T>::raw rf[kSteps], rx[kSteps], rz[kSteps];
     at.load_all((const T*)p.f, rf);
     at.load_all((const T*)p.x, rx);
@@ -320,7 +330,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && GATE ? 4 : 6) void g
         }
         if (in && p.init) e = p.init[r];
     }
-    if (p.chain.tiles > 1) e = entry_of(p.chain, k, col, wave, lane, e, A, H, seen);
+    if (p.chain.tiles > 1) e = entry_of<W>(p.chain, k, col, wave, lane, e, A, H, seen);
     if (wave == 0) {
         if (in && p.states) p.states[(b * p.chain.tiles + k) * p.D + c0 + lane] = e;
         if (in && p.last && k + 1 == p.chain.tiles) p.last[r] = fmaf(A, e, H);
@@ -360,9 +370,10 @@ struct BwdArgs {
 // The tiles from the last one back. The carry c_t = a_t g_t obeys c_t = a_t c_{t+1} + a_t dh_t, so parts and tiles
 // are affine maps again, with the same A. h is formed from `states` for the tile alone, without waiting.
 template <typename T, bool EVEN, bool GATE>
-__global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs p) {
+__global__ __launch_bounds__(64 * kWaves<kBackwardSteps>, 4) void gated_bwd_kernel(const BwdArgs p) {
+    constexpr int kSteps = kBackwardSteps, W = kWaves<kSteps>, kParts = 2 * W;
     __shared__ float maps_a[kParts][kWidth], maps_h[kParts][kWidth], maps_g[kParts][kWidth];
-    __shared__ Looked seen;
+    __shared__ Looked<W> seen;
     __shared__ uint32_t shared_ticket;
     int k;
     uint32_t col;
@@ -370,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
     const int tile = p.chain.tiles - 1 - k;
     const int64_t b = col / p.cols, c0 = (int64_t)(col - (uint32_t)b * p.cols) * kWidth;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const Place<T, EVEN> at(b, (int64_t)tile * kTile, c0, wave, lane, p.L, p.D);
+    const Place<T, EVEN, kSteps> at(b, (int64_t)tile * kTile, c0, wave, lane, p.L, p.D);
     typename Pair<T>::raw rf[kSteps], rx[kSteps], rz[kSteps], rd[kSteps];
     at.load_all((const T*)p.f, rf);
     at.load_all((const T*)p.x, rx);
@@ -435,7 +446,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_bwd_kernel(const BwdArgs
             h = fmaf(maps_a[s][lane], h, m);
         }
     }
-    if (p.chain.tiles > 1) e = entry_of(p.chain, k, col, wave, lane, e, A, G, seen);
+    if (p.chain.tiles > 1) e = entry_of<W>(p.chain, k, col, wave, lane, e, A, G, seen);
     if (wave == 0) {
         if (in && p.dinit && tile == 0) p.dinit[r] = fmaf(A, e, G);
 #pragma unroll 4
@@ -586,7 +597,7 @@ template <typename T>
 int fwd(const Shape& g, const FwdArgs& p, hipStream_t s) {
     const auto k = g.D % 2 == 0 ? (p.z ? gated_fwd_kernel<T, true, true> : gated_fwd_kernel<T, true, false>)
                              : (p.z ? gated_fwd_kernel<T, false, true> : gated_fwd_kernel<T, false, false>);
-    hipLaunchKernelGGL(k, g.grid(), dim3(64 * kWaves), 0, s, p);
+    hipLaunchKernelGGL(k, g.grid(), dim3(64 * kWaves<kForwardSteps<T>>), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
@@ -595,7 +606,7 @@ template <typename T>
 int bwd(const Shape& g, const BwdArgs& p, hipStream_t s) {
     const auto k = g.D % 2 == 0 ? (p.z ? gated_bwd_kernel<T, true, true> : gated_bwd_kernel<T, true, false>)
                              : (p.z ? gated_bwd_kernel<T, false, true> : gated_bwd_kernel<T, false, false>);
-    hipLaunchKernelGGL(k, g.grid(), dim3(64 * kWaves), 0, s, p);
+    hipLaunchKernelGGL(k, g.grid(), dim3(64 * kWaves<kBackwardSteps>), 0, s, p);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
