@@ -156,6 +156,21 @@ def test_long_chains(dev, bt, L, dim, dtype):
     check("dinit", got["dinit"], b["dinit"], b["dinit_E"], 2.0 ** -24)
 
 
+@pytest.mark.parametrize("bt,L,dim,dtype", [(3, 260, 192, torch.float32), (67, 300, 513, torch.bfloat16), (601, 131, 65, torch.float32)])
+def test_many_columns(dev, bt, L, dim, dtype):
+    """9, 603 and 1202 columns of 64 channels: several ticket counters, the last of them with fewer columns."""
+    x = inputs(bt, L, dim, seed=bt, dtype=dtype)
+    got = run(dev, x)
+    ref = {k: f64(v) for k, v in x.items()}
+    o = oracle_fwd(**ref)
+    check("out", got["out"], o["out"], o["out_E"], HALF[dtype])
+    check("last", got["last"], o["last"], o["last_E"], 2.0 ** -24)
+    b = oracle_bwd(**ref)
+    for k in ("dx", "df", "dz"):
+        check(k, got[k], b[k], b[k + "_E"], HALF[dtype])
+    check("dinit", got["dinit"], b["dinit"], b["dinit_E"], 2.0 ** -24)
+
+
 @pytest.mark.parametrize("fill", [0, 255, None], ids=["zeros", "ones", "numbers"])
 def test_a_workspace_may_hold_anything(dev, fill):
     """What an earlier call left, zeros, or numbers: a workspace is cleared by the call that uses it."""
