@@ -38,6 +38,7 @@ constexpr int kTile = HX_GATED_CHUNK, kWidth = 64;  // a tile's entry state is o
 // and a CU holds more such tiles. bf16 forward 16 (tiles of 4 waves) against 8 (of 8): 1 x 65536 x 2048 184 us against 204
 // ungated, 242 against 256 gated; 8 x 2048 x 1536 42 against 44, 51 against 53; one tile to a sequence, 3 x 124 x 899, 6.9
 // against 5.9. With 16, fp32 spills: 348 us against 300 ungated at 1 x 65536 x 2048. The backward pass holds twice as much.
+// (Registers for six waves a SIMD: fp32 with z spills 100 bytes a lane, 8 x 2048 x 1536 136 us against 87.)
 template <typename T> constexpr int kForwardSteps = sizeof(T) == 2 ? 16 : 8;
 constexpr int kBackwardSteps = 8;
 template <int S> constexpr int kWaves = kTile / (2 * S);
@@ -274,7 +275,7 @@ struct FwdArgs {
 };
 
 template <typename T, bool EVEN, bool GATE>
-__global__ __launch_bounds__(64 * kWaves<kForwardSteps<T>>, sizeof(T) == 4 && !GATE ? 6 : 4) void gated_fwd_kernel(const FwdArgs p) {
+__global__ __launch_bounds__(64 * kWaves<kForwardSteps<T>>, 4) void gated_fwd_kernel(const FwdArgs p) {
     constexpr int kSteps = kForwardSteps<T>, W = kWaves<kSteps>, kParts = 2 * W;
     __shared__ float2 maps[kParts][kWidth];
     __shared__ float entries[kParts][kWidth];
