@@ -56,8 +56,11 @@ __device__ inline bf16x8 expand8(uint32_t q, float scale) {
 //   X        16 lanes read a row's 256 bytes of the window and leave them in the wave's own LDS rows, 16 bytes apart
 //            from a power of two, so that 16 rows read at one place of theirs meet all banks.
 // Rows of X start anywhere: global memory takes 16-byte accesses at any element.
+// The next weights are asked for once the registers that take them are read, and no address is kept, which leaves room for two
+// blocks of 8 waves to a CU (four waves a SIMD): 1 x 32768 x 8192 33.1 -> 29.7 us, 1 x 8950 x 7360 15.2 -> 12.3. With 32 rows
+// of X the registers of four waves do not hold two tiles (220 bytes spilled): two waves.
 template <int NT, int XR, typename TO>
-__global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
+__global__ __launch_bounds__(512, XR > 4 ? 2 : 4) void linear_w4_kernel(const W4Args p) {
     constexpr int MT = XR < 4 ? 1 : XR / 4, kRows = 4 * XR;  // column tiles of 16, rows of X that are staged
     extern __shared__ float lds[];  // first the waves' rows of X, then [waves][NT][MT][16 m][16 n] sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -78,10 +81,10 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
     char* const xrow = (char*)lds + wave * (kRows * kXRow);
     const int64_t rows = p.M - m0 < kRows ? p.M - m0 : kRows;
     const int rows_in = (int)rows;
-    const uint16_t* const xb = p.X + m0 * p.ldx;
+    const char* const xb = (const char*)(p.X + m0 * p.ldx);
     uint32_t x[XR];
 #pragma unroll
-    for (int t = 0; t < XR; ++t) x[t] = (uint32_t)((4 * t + j < rows_in ? 4 * t + j : rows_in - 1) * p.ldx) + 8 * r;
+    for (int t = 0; t < XR; ++t) x[t] = (uint32_t)((4 * t + j < rows_in ? 4 * t + j : rows_in - 1) * p.ldx * 2) + 16 * r;
     const char* xread[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) xread[t] = xrow + (16 * t + r < rows_in ? 16 * t + r : rows_in - 1) * kXRow + 16 * j;
@@ -92,10 +95,15 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
         for (int b = 0; b < MT; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
     uint32_t top[NT] = {};  // the largest scale byte of each row: 255 is not a number
 
+    // Kept 32 bits wide up to the load, which adds it to a scalar base by itself; 64-bit sums would stay in registers.
+    const auto offset = [](uint32_t v) {
+        asm("" : "+v"(v));
+        return v;
+    };
     const auto load_x = [&](int at, u32x4 (&o)[XR]) {
-        const uint16_t* from = xb + (int64_t)at * kWindow;
+        const char* from = xb + (int64_t)at * (2 * kWindow);
 #pragma unroll
-        for (int t = 0; t < XR; ++t) __builtin_memcpy(&o[t], from + x[t], 16);
+        for (int t = 0; t < XR; ++t) __builtin_memcpy(&o[t], from + offset(x[t]), 16);
     };
     // A wave's own rows, and its LDS accesses keep their order: no barrier, and the registers are free for the next window.
     const auto stage = [&](const u32x4 (&xs)[XR]) {
@@ -107,16 +115,16 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
     const auto load_x_end = [&](int at, u32x4 (&o)[XR]) {
         const int left = (int)(p.K - (int64_t)at * kWindow) - 8 * r;
         const int back = left >= 8 ? 0 : 8 - left;
-        const uint16_t* from = xb + (int64_t)at * kWindow;
+        const char* from = xb + (int64_t)at * (2 * kWindow);
 #pragma unroll
         for (int t = 0; t < XR; ++t) {
             unsigned __int128 v = 0;
             if (left > 0) {
                 if (p.K >= 8) {
-                    __builtin_memcpy(&v, from + x[t] - back, 16);
+                    __builtin_memcpy(&v, from + x[t] - 2 * back, 16);
                     v >>= 16 * back;
                 } else {
-                    for (int e = 0; e < left; ++e) v |= (unsigned __int128)from[x[t] + e] << (16 * e);
+                    for (int e = 0; e < left; ++e) v |= (unsigned __int128)*(const uint16_t*)(from + x[t] + 2 * e) << (16 * e);
                 }
             }
             __builtin_memcpy(&o[t], &v, 16);
@@ -125,7 +133,7 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
     const auto load_w = [&](int at, bool in, u32x4 (&o)[NT]) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-            o[t] = in ? *reinterpret_cast<const u32x4*>(wb + (int64_t)at * (kWindow / 2) + w[t]) : u32x4{0, 0, 0, 0};
+            o[t] = in ? *reinterpret_cast<const u32x4*>(wb + (int64_t)at * (kWindow / 2) + offset(w[t])) : u32x4{0, 0, 0, 0};
     };
     // lane 4n + u: the four scale bytes of row n's window at + u
     const int last = (int)(sr / 4) - 1;
@@ -134,7 +142,7 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[t] = *reinterpret_cast<const uint32_t*>(sb + (s[t] + word * 4));
     };
-    const auto multiply = [&](const u32x4 (&q)[NT], const uint32_t (&sc)[NT], int u, int groups_in) {
+    const auto multiply = [&](u32x4 (&q)[NT], const uint32_t (&sc)[NT], int u, int groups_in, const auto& refill) {
         const auto moved = [&](uint32_t v) { return __int_as_float(__builtin_amdgcn_ds_bpermute(place, (int)v)); };
         float c[NT][4];
         uint32_t scales[NT];
@@ -154,6 +162,7 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
                 scales[a] = (scales[a] & kept) | (0x7f7f7f7fu & ~kept);
             }
         }
+        refill(q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             bf16x8 xv[MT];
@@ -190,11 +199,7 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
             for (int u = 0; u < kAhead; ++u) {
                 stage(xs);
                 load_x(at + u + 1, xs);
-                u32x4 now[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) now[t] = q[u][t];
-                load_w(at + u + kAhead, true, q[u]);
-                multiply(now, sc, u, 4);
+                multiply(q[u], sc, u, 4, [&](u32x4 (&o)[NT]) { load_w(at + u + kAhead, true, o); });
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) sc[t] = after[t];
@@ -203,7 +208,7 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
         for (int u = 0; u < kAhead; ++u) {
             stage(xs);
             if (u + 1 < kAhead) load_x(at + u + 1, xs);
-            multiply(q[u], sc, u, 4);
+            multiply(q[u], sc, u, 4, [](auto&) {});
         }
         at += kAhead;
     }
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(512) void linear_w4_kernel(const W4Args p) {
             else
                 load_x_end(at + u, xs);
             stage(xs);
-            multiply(q[u], sc, u, left < 4 ? left : 4);
+            multiply(q[u], sc, u, left < 4 ? left : 4, [](auto&) {});
         }
     }
     // a scale that is not a number makes its whole row one: NaN * 0 added to it
@@ -332,20 +337,23 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
     HX_REQUIRE(N < (1 << 30) && M <= kRowsAtOnce * (int64_t)65535 && K < (1 << 26) && ldx < (1 << 26),
                HX_ERR_UNSUPPORTED, "linear_w4: at most %d rows of X, N below 2^30, K and ldx below 2^26", kRowsAtOnce * 65535);
     // How K is cut decides the order of the sums, so it goes by N and K alone: up to 8 waves a tile of 16 outputs while there
-    // are fewer than 8 for each of 256 CUs, or 16 where a wave would walk more than 8 windows, none with fewer than two.
-    // 1 x 2048 x 4096: 8 waves 4.4 us, 4 waves 4.7, 2 waves 6.1; 2 x 16384 x 4096: 4 waves 11.1, 8 waves 12.2; 1 x 16384 x
-    // 2048: 2 waves 6.3, 4 waves 7.0; 5 x 32768 x 8192: 2 waves 34.6, 4 waves 39; 45 x 14152 x 736: 2 waves 10.4, 4 waves 12.9.
+    // are fewer than 8 for each of 256 CUs, or 16 where a wave would walk more than 8 windows, none with fewer than two; and
+    // up to 4 where each still walks 8. 1 x 8192 x 8192: 8 waves 11.1 us, 4 waves 12.7; 2 x 16384 x 4096: 4 waves 10.7, 8 waves
+    // 11.5, 2 waves 12.6; 45 x 14152 x 736: 2 waves 10.4, 4 waves 12.9; 1 x 32768 x 4096: 4 waves 16.8, 2 waves 19.6; 5 x 32768 x
+    // 8192: 34.5 and 34.1; 64 x 32768 x 4096: 52.0 and 50.8; 1 x 65536 x 2048: 2 waves 17.3, 1 wave 20.7.
     const int windows = (int)((K + kWindow - 1) / kWindow);
     const int64_t tiles = (N + 15) / 16;
     int waves = 1;
-    while (waves < 8 && windows >= 4 * waves && (tiles * waves < 2048 || (windows > 8 * waves && tiles * waves < 4096))) waves *= 2;
+    while (waves < 8 && windows >= 4 * waves && (tiles * waves < 2048 || (windows > 8 * waves && tiles * waves < 4096) ||
+                                                   (windows >= 16 * waves && waves < 4)))
+        waves *= 2;
     const W4Args p{M, N, K, ldx, ldy, (const uint16_t*)X, (const uint8_t*)packed, (const uint8_t*)scales, bias, Y, act, windows,
                    (windows + waves - 1) / waves, waves};
     const bool f32 = out_dtype == HX_F32;
     hipStream_t s = as_stream(stream);
     // Two tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs. 1 tile and 2 tiles:
-    // 1 x 32768 x 8192 36.3 and 32.8 us, 1 x 16384 x 2048 6.3 and 7.6; 5 x 32768 x 8192 38.4 and 34.6, 8 x 8192 x 4096 7.3
-    // and 7.4; 9 x 5314 x 6080 10.9 and 9.9, 24 x 4096 x 4096 7.6 and 8.6; 64 x 16384 x 8192 70 and 47.
+    // 1 x 32768 x 8192 32.5 and 29.8 us, 2 x 16384 x 4096 10.7 and 11.8; 5 x 32768 x 8192 39.1 and 34.5, 8 x 8950 x 7360 15.6
+    // and 18.3; 16 x 8192 x 8192 15.2 and 13.7, 24 x 4096 x 4096 7.6 and 8.6; 64 x 16384 x 8192 66 and 46.
     const bool two = M > 8 ? tiles > 256 : tiles >= (M > 4 ? 1024 : 2048);
     if (M <= 4) return two ? launch_w4<2, 1>(p, f32, s) : launch_w4<1, 1>(p, f32, s);
     if (M <= 8) return two ? launch_w4<2, 2>(p, f32, s) : launch_w4<1, 2>(p, f32, s);
