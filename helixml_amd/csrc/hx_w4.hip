@@ -19,7 +19,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWindow = 128;  // elements of K that one 16-byte load per lane covers for 16 rows
-constexpr int kAhead = 4;     // windows whose weights are in flight at once, and whose scales one load covers
+constexpr int kAhead = 4;     // windows whose scales one load covers, and whose weights are in flight at once
 constexpr int kRowsAtOnce = 32;  // rows of X that one block takes at most
 constexpr int kXRow = 2 * kWindow + 16;  // bytes from one staged row of X to the next
 
@@ -58,9 +58,9 @@ __device__ inline bf16x8 expand8(uint32_t q, float scale) {
 // Rows of X start anywhere: global memory takes 16-byte accesses at any element.
 // The next weights are asked for once the registers that take them are read, and no address is kept, which leaves room for two
 // blocks of 8 waves to a CU (four waves a SIMD): 1 x 32768 x 8192 33.1 -> 29.7 us, 1 x 8950 x 7360 15.2 -> 12.3. With 32 rows
-// of X the registers of four waves do not hold two tiles (220 bytes spilled): two waves.
+// of X, or four tiles, they do not hold it (220 bytes spilled): two waves.
 template <int NT, int XR, typename TO>
-__global__ __launch_bounds__(512, XR > 4 ? 2 : 4) void linear_w4_kernel(const W4Args p) {
+__global__ __launch_bounds__(512, XR > 4 || NT > 2 ? 2 : 4) void linear_w4_kernel(const W4Args p) {
     constexpr int MT = XR < 4 ? 1 : XR / 4, kRows = 4 * XR;  // column tiles of 16, rows of X that are staged
     extern __shared__ float lds[];  // first the waves' rows of X, then [waves][NT][MT][16 m][16 n] sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -184,13 +184,14 @@ __global__ __launch_bounds__(512, XR > 4 ? 2 : 4) void linear_w4_kernel(const W4
     const int end = at + p.per < p.windows ? at + p.per : p.windows;
     const int whole = (int)(p.K / kWindow) < end ? (int)(p.K / kWindow) : end;
     if (at + kAhead <= whole) {
-        // a ring of kAhead windows of weights: the one that was multiplied makes room for the one kAhead later. X comes
-        // one window ahead, asked for before the weights that follow it: loads return in order.
-        u32x4 q[kAhead][NT], xs[XR];
+        // a ring of R windows of weights: the one that was multiplied makes room for the one R later. X comes one window
+        // ahead, asked for before the weights that follow it: loads return in order.
+        constexpr int R = NT > 2 ? kAhead / 2 : kAhead;  // four tiles' registers
+        u32x4 q[R][NT], xs[XR];
         uint32_t sc[NT];
         load_s(at, sc);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) load_w(at + u, true, q[u]);
+        for (int u = 0; u < R; ++u) load_w(at + u, true, q[u]);
         load_x(at, xs);
         for (; at + 2 * kAhead <= whole; at += kAhead) {
             uint32_t after[NT];
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(512, XR > 4 ? 2 : 4) void linear_w4_kernel(const W4
             for (int u = 0; u < kAhead; ++u) {
                 stage(xs);
                 load_x(at + u + 1, xs);
-                multiply(q[u], sc, u, 4, [&](u32x4 (&o)[NT]) { load_w(at + u + kAhead, true, o); });
+                multiply(q[u % R], sc, u, 4, [&](u32x4 (&o)[NT]) { load_w(at + u + R, true, o); });
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) sc[t] = after[t];
@@ -208,7 +209,9 @@ __global__ __launch_bounds__(512, XR > 4 ? 2 : 4) void linear_w4_kernel(const W4
         for (int u = 0; u < kAhead; ++u) {
             stage(xs);
             if (u + 1 < kAhead) load_x(at + u + 1, xs);
-            multiply(q[u], sc, u, 4, [](auto&) {});
+            multiply(q[u % R], sc, u, 4, [&](u32x4 (&o)[NT]) {
+                if (u + R < kAhead) load_w(at + u + R, true, o);
+            });
         }
         at += kAhead;
     }
@@ -355,8 +358,15 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
     // 1 x 32768 x 8192 32.5 and 29.8 us, 2 x 16384 x 4096 10.7 and 11.8; 5 x 32768 x 8192 39.1 and 34.5, 8 x 8950 x 7360 15.6
     // and 18.3; 16 x 8192 x 8192 15.2 and 13.7, 24 x 4096 x 4096 7.6 and 8.6; 64 x 16384 x 8192 66 and 46.
     const bool two = M > 8 ? tiles > 256 : tiles >= (M > 4 ? 1024 : 2048);
+    // Four share them where a wave's X is long: with up to 16 rows and more than 512 tiles of more than 32 windows (16 x 32768 x
+    // 8192 43 -> 36 us, 16 x 8950 x 7360 20.8 -> 18.5; 16 x 8192 x 8192 13.6 -> 17.1, 12 x 32768 x 2048 12.9 -> 14.2); with more
+    // rows, of which the registers leave a CU 8 waves either way, where that saves a third of the rounds of blocks, since a
+    // round then takes about 1.6 times as long (64 x 16384 x 8192 48 -> 39, 64 x 8192 x 8192 28 -> 22, 64 x 24576 x 8192 67 ->
+    // 58; with the rounds the same 64 x 4096 x 4096 8.7 -> 12.0, 24 x 8192 x 4096 10.8 -> 14.1).
+    const auto rounds = [&](int64_t t) { return ((tiles + t - 1) / t * ((M + kRowsAtOnce - 1) / kRowsAtOnce) * waves + 2047) / 2048; };
+    const bool four = M > 16 ? 3 * rounds(4) <= 2 * rounds(2) : M > 8 && tiles > 512 && windows > 32;
     if (M <= 4) return two ? launch_w4<2, 1>(p, f32, s) : launch_w4<1, 1>(p, f32, s);
     if (M <= 8) return two ? launch_w4<2, 2>(p, f32, s) : launch_w4<1, 2>(p, f32, s);
-    if (M <= 16) return two ? launch_w4<2, 4>(p, f32, s) : launch_w4<1, 4>(p, f32, s);
-    return two ? launch_w4<2, 8>(p, f32, s) : launch_w4<1, 8>(p, f32, s);
+    if (M <= 16) return four ? launch_w4<4, 4>(p, f32, s) : two ? launch_w4<2, 4>(p, f32, s) : launch_w4<1, 4>(p, f32, s);
+    return four ? launch_w4<4, 8>(p, f32, s) : two ? launch_w4<2, 8>(p, f32, s) : launch_w4<1, 8>(p, f32, s);
 }

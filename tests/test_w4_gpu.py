@@ -266,3 +266,45 @@ def test_wrapper_refusals(dev):
         ssm.linear_w4(X, packed, scales, out_dtype=torch.float16)
     with pytest.raises(_ffi.InvalidInput):
         ssm.linear_w4(X, packed.cpu(), scales)
+
+
+# ------------------------------------------------------------------ many outputs, many rows (device)
+LARGE = [(13, 8250, 4200), (40, 9000, 2100), (9000, 40, 1100), (64, 16390, 1030)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", LARGE)
+def test_large_products(dev, M, N, K):
+    g = torch.Generator().manual_seed(M + N)
+    packed, scales = random_weights(N, K, K)
+    W = packed.to(dev)
+    ones = scales.clone()
+    ones[:, : -(-K // 32)] = 127
+    X = torch.randint(-8, 9, (M, K), generator=g).to(torch.bfloat16)
+    got = ssm.linear_w4(X.to(dev), W, ones.to(dev), out_dtype=torch.float32)
+    assert np.array_equal(got.double().cpu().numpy(), X.double().numpy() @ expand(packed, ones, K).T)
+
+    X = torch.randn(M, K, generator=g).to(torch.bfloat16)
+    y0 = torch.randn(M, N, generator=g).to(torch.bfloat16)
+    Y = torch.full((M, N + 3), 7.0, device=dev, dtype=torch.bfloat16)
+    Y[:, :N] = y0.to(dev)
+    ssm.linear_w4(X.to(dev), W, scales.to(dev), act=2, out=Y[:, :N])
+    w = expand(packed, scales, K)
+    want = X.double().numpy() @ w.T
+    E = K * 2.0 ** -23 * (np.abs(X.double().numpy()) @ np.abs(w).T)
+    want = want + y0.double().numpy()
+    E = E + 2.0 ** -23 * np.abs(want)
+    tol = E + 2.0 ** -8 * (np.abs(want) + E)
+    bad = np.abs(Y[:, :N].double().cpu().numpy() - want) > tol
+    assert not bad.any(), np.argwhere(bad)[:4].tolist()
+    assert (Y[:, N:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(8250, 4200), (9000, 2100), (32780, 4096)])
+def test_a_row_of_a_large_product_does_not_depend_on_the_batch(dev, N, K):
+    packed, scales = (t.to(dev) for t in random_weights(N, K, 9))
+    X = torch.randn(100, K).to(dev, torch.bfloat16)
+    whole = ssm.linear_w4(X, packed, scales, out_dtype=torch.float32)
+    for m in (1, 4, 5, 8, 9, 16, 17, 32, 40, 64):
+        assert torch.equal(ssm.linear_w4(X[:m], packed, scales, out_dtype=torch.float32), whole[:m]), m
