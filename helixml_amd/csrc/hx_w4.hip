@@ -354,16 +354,16 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
                    (windows + waves - 1) / waves, waves};
     const bool f32 = out_dtype == HX_F32;
     hipStream_t s = as_stream(stream);
-    // Two tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs. 1 tile and 2 tiles:
-    // 1 x 32768 x 8192 32.5 and 29.8 us, 2 x 16384 x 4096 10.7 and 11.8; 5 x 32768 x 8192 39.1 and 34.5, 8 x 8950 x 7360 15.6
-    // and 18.3; 16 x 8192 x 8192 15.2 and 13.7, 24 x 4096 x 4096 7.6 and 8.6; 64 x 16384 x 8192 66 and 46.
-    const bool two = M > 8 ? tiles > 256 : tiles >= (M > 4 ? 1024 : 2048);
-    // Four share them where a wave's X is long: with up to 16 rows and more than 512 tiles of more than 32 windows (16 x 32768 x
-    // 8192 43 -> 36 us, 16 x 8950 x 7360 20.8 -> 18.5; 16 x 8192 x 8192 13.6 -> 17.1, 12 x 32768 x 2048 12.9 -> 14.2); with more
-    // rows, of which the registers leave a CU 8 waves either way, where that saves a third of the rounds of blocks, since a
-    // round then takes about 1.6 times as long (64 x 16384 x 8192 48 -> 39, 64 x 8192 x 8192 28 -> 22, 64 x 24576 x 8192 67 ->
-    // 58; with the rounds the same 64 x 4096 x 4096 8.7 -> 12.0, 24 x 8192 x 4096 10.8 -> 14.1).
+    // Two or four tiles share a wave's rows of X where it is X that costs: with few tiles it is the idle CUs.
+    //   up to 16 rows  1 tile and 2 tiles: 1 x 32768 x 8192 32.5 and 29.8 us, 2 x 16384 x 4096 10.7 and 11.8; 5 x 32768 x 8192
+    //       39.1 and 34.5, 8 x 8950 x 7360 15.6 and 18.3; 16 x 8192 x 8192 15.2 and 13.7. 2 and 4: 16 x 32768 x 8192 43 and 36,
+    //       16 x 8950 x 7360 20.8 and 18.5; 16 x 8192 x 8192 13.6 and 17.1, 12 x 32768 x 2048 12.9 and 14.2.
+    //   more  the registers leave a CU 8 waves in every form, and a round of blocks takes up to 1.6 times as long with twice
+    //       the tiles, so they are doubled where that saves a third of the rounds. 1 and 2 tiles: 60 x 4096 x 4096 12.3 and 9.7
+    //       (2 rounds and 1), 24 x 8192 x 544 5.8 and 6.4 (1 and 1). 2 and 4: 64 x 8192 x 8192 28 and 22, 64 x 24576 x 8192 67
+    //       and 58 (3 and 2), 64 x 4096 x 4096 8.7 and 12.0 (1 and 1), 57 x 8950 x 7360 36.5 and 38.4 (3 and 2).
     const auto rounds = [&](int64_t t) { return ((tiles + t - 1) / t * ((M + kRowsAtOnce - 1) / kRowsAtOnce) * waves + 2047) / 2048; };
+    const bool two = M > 16 ? 3 * rounds(2) <= 2 * rounds(1) : M > 8 ? tiles > 256 : tiles >= (M > 4 ? 1024 : 2048);
     const bool four = M > 16 ? 3 * rounds(4) <= 2 * rounds(2) : M > 8 && tiles > 512 && windows > 32;
     if (M <= 4) return two ? launch_w4<2, 1>(p, f32, s) : launch_w4<1, 1>(p, f32, s);
     if (M <= 8) return two ? launch_w4<2, 2>(p, f32, s) : launch_w4<1, 2>(p, f32, s);
