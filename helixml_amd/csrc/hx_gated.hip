@@ -245,7 +245,8 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
 // block, all blocks in turn (1 x 65536 x 2048 bf16 took 227 us for it alone), so the columns are dealt in runs to up to
 // kCounters words of lines of their own; a column's tiles all come from one of them. Runs of kTogether neighbours, since
 // columns that drift apart share no DRAM page: 1 x 65536 x 2048 fp32 335 us with runs of one, 310 from four on; bf16 230,
-// 208 with four, 204 with eight, 226 with all 32 columns on one word; 1 x 1999 x 768 11.5, 11.8, 12.2 and 12.9.
+// 208 with four, 204 with eight, 226 with all 32 columns on one word; 1 x 1999 x 768 11.5, 11.8, 12.2 and 12.9. Narrower
+// sequences have their own: 4 x 25945 x 98 bf16 31 us, 41 with four sequences to a word; 15 x 3568 x 68 18.5 and 17.6.
 constexpr uint32_t kCounters = 64, kCounterStride = 32, kTogether = 8;
 __device__ inline bool take_unit(const Chain& c, uint32_t& shared_ticket, int& k, uint32_t& col) {
     const uint32_t unit = blockIdx.y * gridDim.x + blockIdx.x;
@@ -567,7 +568,8 @@ struct Shape {
     }
     int64_t together() const {
         const int64_t share = (batch * cols + kCounters - 1) / kCounters;
-        return share > kTogether ? share : kTogether;
+        const int64_t near = cols < kTogether ? cols : kTogether;
+        return share > near ? share : near;
     }
     // The tickets, a word per channel of each tile and group; one tile waits for nobody
     int64_t groups() const { return (tiles + kGroup - 1) / kGroup; }

@@ -158,7 +158,7 @@ def test_long_chains(dev, bt, L, dim, dtype):
 
 @pytest.mark.parametrize("bt,L,dim,dtype", [(3, 260, 192, torch.float32), (67, 300, 513, torch.bfloat16), (601, 131, 65, torch.float32)])
 def test_many_columns(dev, bt, L, dim, dtype):
-    """9, 603 and 1202 columns of 64 channels: several ticket counters, the last of them with fewer columns."""
+    """9, 603 and 1202 columns of 64 channels: several ticket counters, in the larger two the last with fewer columns."""
     x = inputs(bt, L, dim, seed=bt, dtype=dtype)
     got = run(dev, x)
     ref = {k: f64(v) for k, v in x.items()}
