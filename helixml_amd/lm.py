@@ -257,8 +257,11 @@ class ByteLM:
         and replays; ``state`` is advanced in place exactly as by decode_step. The logits tensor
         is the graph's output buffer, overwritten by the next replay. ``adjust`` as in decode_step:
         the graph reads its tensors at every replay, so the caller updates them (the history, its
-        lengths, the allowed tokens) in place between replays."""
+        lengths, the allowed tokens) in place between replays. The step keeps the tensors that it was
+        captured with (``adjust``'s and the weights): another one put into the caller's dict or into the
+        model later does not reach it."""
         bt = state[0][0].shape[0]
+        adjust = None if adjust is None else dict(adjust)
         tok = torch.zeros((bt,), dtype=torch.int32, device=self.device)
         # the graph's own workspace: the captured launches hold its raw address, so it must live
         # as long as the graph and never be replaced (the model's shared workspace is, whenever
@@ -286,8 +289,11 @@ class ByteLM:
         step.workspace = ws
         step.tokens = tok
         step.state = state
+        # the captured launches hold these tensors' addresses: they live as long as the step, whatever becomes of
+        # the caller's dict and of the model
         step.adjust = adjust
-        step.head = self.w_head4  # the captured launches hold these tensors' addresses
+        step.head = self.w_head4
+        step.weights = (self.embed, self.norm_f, self.w_head, [dict(p) for p in self.layers])
         return step
 
     def host_params(self):
