@@ -24,7 +24,7 @@ import torch
 
 from . import _ffi
 from .ssm import (_STORAGE, _on_stream_device, _operands, _ptr, _stream, keep_for_stream,
-                  linear_w4, on_current_or_launch_stream, on_launch_stream, w4_quantize)
+                  linear_w4, on_current_or_launch_stream, on_launch_stream, w4_quantize, w4_values)
 
 _F32, _BF16 = _ffi.HX_F32, _ffi.HX_BF16
 
@@ -136,6 +136,11 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
     return out
 
 
+def _version(t):
+    """Counts the writes to a tensor; one made under inference mode has no count."""
+    return None if t.is_inference() else t._version
+
+
 LAYER_KEYS = ("w_in", "conv_w", "conv_b", "w_x", "w_dt", "dt_bias", "A", "D", "w_out")
 
 
@@ -177,14 +182,28 @@ class ByteLM:
             ))
         self.norm_f = torch.ones(dm, dtype=f32, device=self.device)
         self.w_head = lin(vocab, dm)
-        self.w_head4 = None
+        self._head4 = None
         self._ws: Optional[torch.Tensor] = None
 
     # ------------------------------------------------------------------ helpers
     def quantize_head(self):
         """Rounds the head's weights to 4 bits with group scales (ssm.w4_quantize): from then on prefill and decode
-        alike read them through hx_linear_w4, whose rows do not depend on how many there are."""
+        alike read them through hx_linear_w4, whose rows do not depend on how many there are. The model goes back to
+        w_head itself once that is assigned or written to (writes through ``.data`` are not seen): the 4-bit form is of
+        what it held before, and is made again by another call. ``w_head4 = None`` does the same by hand."""
         self.w_head4 = w4_quantize(self.w_head)
+
+    @property
+    def w_head4(self):
+        """The 4-bit head (packed, scales), None where there is none of what w_head holds now."""
+        if self._head4 is None:
+            return None
+        pair, of, version = self._head4
+        return pair if of is self.w_head and version == _version(of) else None
+
+    @w_head4.setter
+    def w_head4(self, pair):
+        self._head4 = None if pair is None else (pair, self.w_head, _version(self.w_head))
 
     def _workspace(self, batch, seqlen):
         need = int(_ffi.lib().hx_mamba_layer_workspace_size(batch, seqlen, self.d_model, self.d_inner,
@@ -203,8 +222,9 @@ class ByteLM:
         rows = x.numel() // self.d_model
         xn = rmsnorm(x, self.norm_f, self.eps, out_dtype=torch.bfloat16, stream=stream)
         logits = torch.empty((*x.shape[:-1], self.vocab), device=self.device, dtype=torch.float32)
-        if self.w_head4 is not None:
-            linear_w4(xn.view(rows, self.d_model), *self.w_head4, out=logits.view(rows, self.vocab), stream=stream)
+        head4 = self.w_head4
+        if head4 is not None:
+            linear_w4(xn.view(rows, self.d_model), *head4, out=logits.view(rows, self.vocab), stream=stream)
             return logits
         _ffi.call("hx_gemm_bf16", rows, self.vocab, self.d_model, _ptr(xn), self.d_model,
                   _ptr(self.w_head), self.d_model, None, 0, _F32, _ptr(logits), self.vocab,
@@ -297,7 +317,10 @@ class ByteLM:
         return step
 
     def host_params(self):
-        """Every parameter as float32 numpy arrays (for the CPU oracle in tests)."""
+        """Every parameter as float32 numpy arrays (for the CPU oracle in tests); w_head is the head that the
+        logits come from, so the 4-bit form's values where there is one."""
         f = lambda t: t.float().cpu().numpy()  # noqa: E731
-        return dict(embed=f(self.embed), norm_f=f(self.norm_f), w_head=f(self.w_head),
+        head4 = self.w_head4
+        head = f(self.w_head) if head4 is None else w4_values(*head4, self.d_model)
+        return dict(embed=f(self.embed), norm_f=f(self.norm_f), w_head=head,
                     layers=[{k: f(v) for k, v in p.items()} for p in self.layers])

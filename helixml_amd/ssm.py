@@ -478,6 +478,16 @@ def w4_quantize(W, device=None):
     return torch.from_numpy(packed).to(device), torch.from_numpy(scales).to(device)
 
 
+def w4_values(packed, scales, K):
+    """What a packed pair [N, ...] of rows of K weights stands for: a float32 numpy array [N, K] (scale byte 255: NaN)."""
+    q, s = packed.cpu().numpy(), scales.cpu().numpy()
+    code = np.stack((q & 15, q >> 4), -1).reshape(q.shape[0], -1)[:, :K]
+    table = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6], np.float32)
+    power = np.where(s == 255, np.float32(np.nan), np.exp2(s.astype(np.float64) - 127))
+    with np.errstate(over="ignore"):
+        return (np.concatenate((table, -table))[code] * np.repeat(power, W4_GROUP, 1)[:, :K]).astype(np.float32)
+
+
 @on_current_or_launch_stream
 def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=None):
     """Y = X . W^T (+ bias)(, SiLU) with 4-bit weights (hx_linear_w4). X [M, K] bf16 (rows may be strided);
