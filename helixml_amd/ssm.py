@@ -455,6 +455,7 @@ def gemm_bf16(X, W, bias=None, act=0, out_dtype=torch.bfloat16, splits=None, str
 
 
 W4_GROUP = 32
+W4_ROWS = 32 * 65535  # of X that one hx_linear_w4 takes
 
 
 def _w4_rows(K):
@@ -517,6 +518,10 @@ def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out
     elif N > 1 and out.stride(1) != 1:
         raise InvalidInput("linear_w4: out needs unit column stride")
     _on_stream_device(stream, X=X, out=out)
+    if M > W4_ROWS:  # a row's bits do not depend on the rows beside it, so they are cut anywhere
+        for i in range(0, M, W4_ROWS):
+            linear_w4.__wrapped__(X[i: i + W4_ROWS], packed, scales, bias, act, out=out[i: i + W4_ROWS], stream=stream)
+        return out
     # a single row has no stride: torch may report any
     _ffi.call("hx_linear_w4", M, N, K, _ptr(X), X.stride(0) if M > 1 else K, _ptr(packed), _ptr(scales), _ptr(bias),
               int(act), _STORAGE[out.dtype], _ptr(out), out.stride(0) if M > 1 else N, _stream(stream))
