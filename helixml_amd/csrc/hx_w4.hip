@@ -135,6 +135,19 @@ __global__ __launch_bounds__(512, XR > 4 || NT > 2 ? 2 : 4) void linear_w4_kerne
         for (int t = 0; t < NT; ++t)
             o[t] = in ? *reinterpret_cast<const u32x4*>(wb + (int64_t)at * (kWindow / 2) + offset(w[t])) : u32x4{0, 0, 0, 0};
     };
+    // The window that K ends in: codes from K on are zero too, whatever the rows hold there, since X's zeros do not cancel
+    // an infinity (scale bytes 253 and 254). Lane 4n + j holds 32 codes of row n from element 32j of the window on.
+    const auto cut_w = [&](int at, u32x4 (&o)[NT]) {
+        const int left = (int)(p.K - (int64_t)at * kWindow) - 32 * (lane % 4);
+        u32x4 kept;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int codes = left - 8 * i;
+            kept[i] = codes <= 0 ? 0u : codes >= 8 ? 0xffffffffu : (1u << (4 * codes)) - 1u;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t] &= kept;
+    };
     // lane 4n + u: the four scale bytes of row n's window at + u
     const int last = (int)(sr / 4) - 1;
     const auto load_s = [&](int at, uint32_t (&o)[NT]) {
@@ -227,10 +240,12 @@ __global__ __launch_bounds__(512, XR > 4 || NT > 2 ? 2 : 4) void linear_w4_kerne
             if (at + u >= end) break;
             const int left = (int)(G - (int64_t)(at + u) * 4);
             u32x4 xs[XR];
-            if (at + u < whole)
+            if (at + u < whole) {
                 load_x(at + u, xs);
-            else
+            } else {
                 load_x_end(at + u, xs);
+                cut_w(at + u, q[u]);
+            }
             stage(xs);
             multiply(q[u], sc, u, left < 4 ? left : 4, [](auto&) {});
         }

@@ -308,3 +308,23 @@ def test_a_row_of_a_large_product_does_not_depend_on_the_batch(dev, N, K):
     whole = ssm.linear_w4(X, packed, scales, out_dtype=torch.float32)
     for m in (1, 4, 5, 8, 9, 16, 17, 32, 40, 64):
         assert torch.equal(ssm.linear_w4(X[:m], packed, scales, out_dtype=torch.float32), whole[:m]), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("byte", [252, 253, 254])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 33), (5, 40, 70), (20, 33, 1), (9, 50, 127), (3, 20, 555), (17, 64, 4107)])
+def test_unused_codes_reach_nothing_at_any_scale(dev, M, N, K, byte):
+    """Codes from K on are unused: random ones change no output, also where the last group's scale makes an infinity of
+    them. Its own weights are zero, so what the row gives is the other groups' products, equal bit for bit."""
+    packed, scales = random_weights(N, K, K + byte)
+    groups = -(-K // 32)
+    scales[:, :groups] = 127
+    scales[:, groups - 1] = byte
+    code = torch.stack((packed & 15, packed >> 4), -1).view(N, -1)
+    code[:, 32 * (groups - 1): K] = 0
+    code[:, K:] |= 4  # 2 and more: past bf16's range at scale bytes 253 and 254 for most
+    packed = code[:, 0::2] | code[:, 1::2] << 4
+    X = torch.randint(-8, 9, (M, K)).to(torch.bfloat16)
+    want = X.double().numpy() @ expand(packed, scales, K).T
+    got = ssm.linear_w4(X.to(dev), packed.to(dev), scales.to(dev), out_dtype=torch.float32)
+    assert np.array_equal(got.double().cpu().numpy(), want)
