@@ -169,7 +169,11 @@ __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, 
     constexpr int kMine = kGroup / W;
     const int group = k / kGroup, place = k % kGroup;
     const bool closes = place == kGroup - 1 && k + 1 < c.tiles;
-    if (wave == 0 && k + 1 < c.tiles) publish_map(words_of(c.tiles_at, c, k, col) + lane, A, H);
+    if (wave == 0 && k + 1 < c.tiles) {
+        // `first` has arrived before anyone can go on from this tile: the chain's last tile may write its place
+        asm volatile("" : "+v"(first)::"memory");
+        publish_map(words_of(c.tiles_at, c, k, col) + lane, A, H);
+    }
     float GA = 1.0f, GH = 0.0f;
     bool mapped = false, ok = false, held = false;
     int start = -1;
@@ -324,13 +328,13 @@ __global__ __launch_bounds__(64 * kWaves<kForwardSteps<T>>, 4) void gated_fwd_ke
     const int64_t r = b * p.D + c0 + lane;
     float A = 1.0f, H = 0.0f, e = 0.0f;
     if (wave == 0) {
+        if (in && p.init) e = p.init[r];
 #pragma unroll 4
         for (int s = 0; s < kParts; ++s) {
             const float2 m = maps[s][lane];
             H = fmaf(m.x, H, m.y);
             A *= m.x;
         }
-        if (in && p.init) e = p.init[r];
     }
     if (p.chain.tiles > 1) e = entry_of<W>(p.chain, k, col, wave, lane, e, A, H, seen);
     if (wave == 0) {
@@ -432,13 +436,13 @@ __global__ __launch_bounds__(64 * kWaves<kBackwardSteps>, 4) void gated_bwd_kern
     const int64_t r = b * p.D + c0 + lane;
     float A = 1.0f, G = 0.0f, e = 0.0f;
     if (wave == 0) {
+        if (in && p.dlast) e = p.dlast[r];
 #pragma unroll 4
         for (int s = kParts - 1; s >= 0; --s) {
             const float m = maps_a[s][lane];
             G = fmaf(m, G, maps_g[s][lane]);
             A *= m;
         }
-        if (in && p.dlast) e = p.dlast[r];
     } else if (wave == 1) {
         float h = in ? p.states[(b * p.chain.tiles + tile) * p.D + c0 + lane] : 0.0f;
 #pragma unroll 4

@@ -161,7 +161,7 @@ int hx_selective_state_update(int64_t batch, int64_t dim, int64_t dstate,
  * x, f, z, out: [batch, seqlen, dim] of `dtype` (out may be one of the others); init_state,
  * last_state: [batch, dim] fp32. dim < 2^26, and batch * ceil(dim / 64) * ceil(seqlen / 128) < 2^31.
  * init_state (nullable) seeds h; last_state (nullable) receives h after the last step (init_state,
- * or zero, where seqlen is 0).
+ * or zero, where seqlen is 0); both may be one buffer, a state that is carried in place.
  * states (nullable): [batch, ceil(seqlen / HX_GATED_CHUNK), dim] fp32, receives h BEFORE steps 0,
  * HX_GATED_CHUNK, 2 * HX_GATED_CHUNK, ...: what hx_gated_scan_bwd forms h from again.
  * Steps are grouped (in tiles of 128), so results agree with the step-by-step recurrence to fp32
@@ -181,7 +181,7 @@ int hx_gated_scan_fwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, con
  *   dinit = a_0 * g_0  (the gradient of the entry state; dlast, or zero, where seqlen is 0)
  * x, f, z and states: what hx_gated_scan_fwd took and gave (its init_state is states' first entry).
  * dout, dx, df, dz: [batch, seqlen, dim] of `dtype`; dlast (nullable: zero), dinit (nullable: not
- * wanted): [batch, dim] fp32. dz is required exactly where z is given. h is formed again in fp32
+ * wanted): [batch, dim] fp32, which may be one buffer. dz is required exactly where z is given. h is formed again in fp32
  * from `states`, so nothing of `out`'s rounding enters a gradient. workspace as above, of
  * hx_gated_scan_bwd_workspace_size(...) bytes. */
 size_t hx_gated_scan_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int dtype);
