@@ -97,3 +97,20 @@ def test_logits(dev):
     for rows_at in (slice(0, 2), slice(16384, 16386), slice(bt - 2, bt)):
         compare(got[rows_at], *logits_oracle(logits[rows_at].cpu(), history[rows_at].cpu(), repetition=rep[rows_at].cpu(),
                                              presence=rep[rows_at].cpu(), allowed=allowed[rows_at].cpu()), BF)
+
+
+@pytest.mark.parametrize("bt,L,D,dtype", [(9000000, 2, 3, torch.float32), (17000000, 2, 3, BF), (4300000, 130, 1, torch.float32),
+                                          (8500000, 130, 1, BF)])
+def test_more_threads_than_one_grid_axis_takes_forward(dev, bt, L, D, dtype):
+    """More than 2^23 tiles of 512 threads (fp32) or 2^24 of 256 (bf16), in both past 2^32 threads."""
+    assert bt * -(-L // CHUNK) * (512 if dtype == torch.float32 else 256) > 2 ** 32
+    g = torch.Generator(device=dev).manual_seed(2)
+    n = lambda *s: torch.randn(s, device=dev, generator=g, dtype=dtype)  # noqa: E731
+    x, f = n(bt, L, D), n(bt, L, D)
+    init = torch.randn(bt, D, device=dev, generator=g)
+    out, last = ssm.gated_scan_fwd(x, f, None, init, return_last_state=True)
+    pick = torch.tensor([0, 1, 2 ** 20 - 1, 2 ** 20, bt // 2, bt - 2, bt - 1], device=dev)
+    r = lambda t: f64(t[pick].cpu())  # noqa: E731
+    o = oracle_fwd(r(x), r(f), None, r(init))
+    check("out", out[pick], o["out"], o["out_E"], HALF[dtype])
+    check("last", last[pick], o["last"], o["last_E"], 2.0 ** -24)
