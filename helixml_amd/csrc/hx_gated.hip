@@ -161,8 +161,9 @@ constexpr int kNoMap = 1, kGroupExit = 2, kGroupAbsent = 4;
 
 // The state that tile k of a chain starts from, in wave 0's lanes; `first` is the chain's own, (A, H) the tile's map. The
 // W waves look together, a share of the tiles and one group each: the maps of a group are all there about when the tile's own
-// is, and a chain of many tiles moves on by W groups, 8192 steps or 16384, a look. 1 x 42983 x 70 bf16 takes 26 us; with a
-// window of 8 tiles and an exit state for every tile it took 73.
+// is, and a chain of many tiles moves on by W groups a look: 16384 steps, or 8192 in the bf16 forward, whose blocks have
+// four waves (a window apart from the waves was not measured). 1 x 42983 x 70 bf16 takes 26 us; with a window of 8 tiles
+// and an exit state for every tile it took 73.
 template <int W>
 __device__ inline float entry_of(const Chain& c, int k, uint32_t col, int wave, int lane, float first, float A, float H,
                                  Looked<W>& seen) {

@@ -385,7 +385,8 @@ extern "C" int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int6
     //   more  the registers leave a CU 8 waves in every form, and a round of blocks takes up to 1.6 times as long with twice
     //       the tiles, so they are doubled where that saves a third of the rounds. 1 and 2 tiles: 60 x 4096 x 4096 12.3 and 9.7
     //       (2 rounds and 1), 24 x 8192 x 544 5.8 and 6.4 (1 and 1). 2 and 4: 64 x 8192 x 8192 28 and 22, 64 x 24576 x 8192 67
-    //       and 58 (3 and 2), 64 x 4096 x 4096 8.7 and 12.0 (1 and 1), 57 x 8950 x 7360 36.5 and 38.4 (3 and 2).
+    //       and 58 (3 and 2), 64 x 4096 x 4096 8.7 and 12.0 (1 and 1). Where the last round is nearly empty the rule misses:
+    //       57 x 8950 x 7360 gets four tiles (2 rounds against 3) at 38.4, 36.5 with two.
     const auto rounds = [&](int64_t t) { return ((tiles + t - 1) / t * ((M + kRowsAtOnce - 1) / kRowsAtOnce) * waves + 2047) / 2048; };
     const bool two = M > 16 ? 3 * rounds(2) <= 2 * rounds(1) : M > 8 ? tiles > 256 : tiles >= (M > 4 ? 1024 : 2048);
     const bool four = M > 16 ? 3 * rounds(4) <= 2 * rounds(2) : M > 8 && tiles > 512 && windows > 32;

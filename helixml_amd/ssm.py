@@ -247,8 +247,9 @@ def gated_scan_fwd(x, f, z=None, init_state=None, return_last_state=False, retur
     """Gated linear recurrence (hx_gated_scan_fwd): a = sigmoid(f), h_t = a_t h_{t-1} + (1 - a_t) x_t,
     out = h, times silu(z) where z is given. x, f, z: [batch, L, dim] fp32 or bf16; init_state: [batch, dim]
     fp32. Returns out, followed by the last state [batch, dim] fp32 and by the states that gated_scan_bwd
-    needs ([batch, ceil(L / GATED_CHUNK), dim] fp32) where asked for. ``workspace``: a uint8 device tensor of
-    at least gated_scan_workspace_size(...) bytes; allocated here when not given."""
+    needs ([batch, ceil(L / GATED_CHUNK), dim] fp32) where asked for. Nothing is recorded for
+    autograd (the results require no gradient, whatever the operands do): gated_scan_bwd gives the gradients.
+    ``workspace``: a uint8 device tensor of at least gated_scan_workspace_size(...) bytes; allocated here when not given."""
     if x.dim() != 3:
         raise ShapeMismatch(f"x: expected 3 dims [batch, seqlen, dim], got {list(x.shape)}")
     bt, L, dim = shape = x.shape
@@ -493,7 +494,7 @@ def w4_values(packed, scales, K):
 def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=None):
     """Y = X . W^T (+ bias)(, SiLU) with 4-bit weights (hx_linear_w4). X [M, K] bf16 (rows may be strided);
     packed, scales: what w4_quantize gives for W [N, K]; bias [N] fp32. act: bit 0 SiLU, bit 1 adds to
-    ``out`` [M, N] (rows may be strided), which has to be given then."""
+    ``out`` [M, N] (rows may be strided), which has to be given then. Any number of rows."""
     if X.dim() != 2 or packed.dim() != 2:
         raise ShapeMismatch(f"X, packed: expected 2 dims, got {list(X.shape)}, {list(packed.shape)}")
     M, K = X.shape
