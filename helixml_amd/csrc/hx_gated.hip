@@ -544,9 +544,8 @@ __global__ __launch_bounds__(256) void gated_step_kernel(int64_t n, float* state
         step_run<T, 1>(4 * runs + (t - runs), state, x, f, z, out);
 }
 
-// dst = src, or zero: what is left of a sequence without steps.
-__global__ __launch_bounds__(256) void gated_state_copy_kernel(int64_t n, const float* __restrict__ src,
-                                                               float* __restrict__ dst) {
+// dst = src, or zero: what is left of a sequence without steps. Both may be one buffer.
+__global__ __launch_bounds__(256) void gated_state_copy_kernel(int64_t n, const float* src, float* dst) {
     for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < n; o += (int64_t)gridDim.x * 256) dst[o] = src ? src[o] : 0.0f;
 }
 
