@@ -67,6 +67,7 @@ _BY_STATUS = {c.status: c for c in (ShapeMismatch, InvalidDimension, DeviceMisma
 
 HX_F32 = 0
 HX_BF16 = 1
+HX_I8 = 2
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -97,6 +98,11 @@ SIGNATURES = {
     "hx_gated_scan_bwd_workspace_size": [_i64, _i64, _i64, _int],
     "hx_gated_scan_bwd": [_i64, _i64, _i64, _int] + [_p] * 10 + [_p, _sz, _p],
     "hx_gated_state_update": [_i64, _i64, _int] + [_p] * 6,
+    "hx_decay_attention_workspace_size": [_i64] * 5 + [_int],
+    "hx_decay_attention_fwd": [_i64] * 8 + [_int, _p, _i64, _p, _i64, _p, _i64, _p, _f] + [_p] * 5 + [_sz, _p],
+    "hx_decay_attention_bwd_workspace_size": [_i64] * 8 + [_int],
+    "hx_decay_attention_bwd": [_i64] * 8 + [_int, _p, _i64, _p, _i64, _p, _i64, _p, _f] + [_p] * 9 + [_sz, _p],
+    "hx_decay_attention_step": [_i64] * 7 + [_int, _p, _p, _i64, _p, _i64, _p, _i64, _p, _f, _p, _p],
     "hx_s4_discretize": [_i64, _f, _p, _p, _p],
     "hx_s4_ref_workspace_size": [_i64, _i64, _i64],
     "hx_s4_ref_fwd": [_i64, _i64, _i64, _f] + [_p] * 7 + [_p, _sz, _p],
@@ -112,12 +118,15 @@ SIGNATURES = {
                             _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _int, _p, _sz, _p],
     "hx_w4_quantize": [_i64, _i64, _p, _p, _p],
     "hx_linear_w4": [_i64, _i64, _i64, _p, _i64, _p, _p, _p, _int, _int, _p, _i64, _p],
+    "hx_i8_quantize": [_i64, _i64, _p, _p, _p],
+    "hx_linear_i8": [_i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _int, _int, _p, _i64, _p],
     "hx_conv1d_silu": [_i64, _i64, _i64, _i64, _int, _p, _i64, _p, _p, _p, _p],
     "hx_selective_scan_dtproj_fwd": [_i64, _i64, _i64, _i64] + [_p] * 12,
     "hx_mamba_block_workspace_size": [_i64, _i64, _i64, _i64, _i64],
     "hx_mamba_block_fwd": [_i64] * 7 + [_p] * 12 + [_sz, _p],
     "hx_embedding_fwd": [_i64, _i64, _i64, _p, _p, _p, _p],
     "hx_rmsnorm_fwd": [_i64, _i64, _p, _p, _f, _int, _p, _p],
+    "hx_add_rmsnorm": [_i64, _i64, _int, _p, _i64, _int, _p, _i64, _p, _f, _p, _i64, _int, _p, _i64, _p, _p],
     "hx_conv1d_step": [_i64, _i64, _i64, _int, _p, _i64, _p, _p, _p, _p, _p],
     "hx_mamba_layer_workspace_size": [_i64] * 6,
     "hx_mamba_layer_fwd": [_i64] * 7 + [_p, _p, _f] + [_p] * 11 + [_p, _sz, _p],

@@ -1,0 +1,770 @@
+// hx_decay.hip — linear attention with one decay per head: whole sequences, their backward pass, one token.
+#include "hx_common.h"
+#include "hx_wave.h"
+
+namespace hx {
+namespace {
+
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------ the mathematics
+// Every pass over a sequence is one mixing of three operands, tokens counted in the pass's own direction:
+//   out_i = ps sum_{j <= i} w^(i-j) (a_i . b_j) c_j + es w^(i+e0) a_i S,     S the state before the first token,
+//   S' = w^n S + cs sum_j w^(n-1-j+1-e0) b_j c_j^T                          the state after n tokens
+// with w = e^g, g = log_decay[head]:
+//   out  a = q, b = k, c = v, forwards, e0 = 1        dq  a = do, b = v, c = k, forwards, e0 = 1 (its state is S^T)
+//   dv   a = k, b = q, c = do, backwards, e0 = 0      dk  a = v, b = do, c = q, backwards, e0 = 0 (S^T's adjoint)
+// Tokens are taken in chunks: inside a chunk the sum over j is two matrix products around the masked and weighted scores,
+// what came before enters through the state. Powers with a negative exponent are never formed, so no decay overflows.
+struct MixArgs {
+    const void *a, *b, *c;
+    int64_t lda, ldb, ldc;  // elements from one token to the next
+    int ga, gb, gc;         // heads that share one head of the operand
+    int64_t B, L, H;
+    int m, n, heads_out;  // channels of a and b, of c and the output
+    const float* log_decay;
+    const int32_t* lengths;
+    const float* entry;        // [B, H, segments or 1, dk dv]: the states before the first token (nullable: zero)
+    float* ends;               // the states after the last (nullable where there is an output)
+    int64_t state, segs;       // elements of a state, states of a (b, h) in entry and ends
+    int sm, sn;                // a state's strides along m and n
+    float ps, es, cs;
+    int e0, back;
+    void* out;
+    int64_t ldo;
+    int64_t seglen;  // tokens of a segment, whole chunks
+    int nseg, slices;
+};
+
+// w^x for x >= 0 as 2^(x l2); a decay of nothing (g = -inf) keeps w^0 = 1.
+__device__ inline float log2_decay(float g) {
+    const float l2 = g * kLog2e;
+    return l2 < -1e30f ? -1e30f : l2;
+}
+__device__ inline float power(float l2, int x) { return fast_exp2(l2 * (float)x); }
+// The decay of a state over x tokens as v -> v * a + v * b. Near 1 the difference from 1 is what is kept: a factor rounded to
+// 24 bits would repeat its error at every chunk, 3e-8 times the chunks that a state lives for.
+struct Decay {
+    float a, b;
+    __device__ Decay(float g, float x) {
+        const float y = g * x;  // -inf * 0 is a decay over nothing
+        const bool near = x == 0.0f || (y > -0.5f && y < 0.5f);
+        a = near ? 1.0f : __expf(y);
+        b = near ? (x == 0.0f ? 0.0f : expm1f(y)) : 0.0f;
+    }
+    // v decayed, and x added
+    __device__ float operator()(float v, float x) const { return fmaf(v, a, fmaf(v, b, x)); }
+};
+
+// ------------------------------------------------------------------ eight values a lane along a contraction of 32
+// Lane (r = lane % 16, u = lane / 16) of an operand holds row (or column) r and the contraction's places 8u..8u + 7: one bf16
+// instruction, or eight in fp32 that each contract over u. Any order of the places will do as long as both operands have it.
+template <typename T> struct Frag;
+template <> struct Frag<uint16_t> {
+    bf16x8 v;
+};
+template <> struct Frag<float> {
+    float v[8];
+};
+__device__ inline f32x4 mma(f32x4 acc, const Frag<uint16_t>& a, const Frag<uint16_t>& b) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, acc, 0, 0, 0);
+}
+__device__ inline f32x4 mma(f32x4 acc, const Frag<float>& a, const Frag<float>& b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc, 0, 0, 0);
+    return acc;
+}
+
+// fp32 values as a sum of PARTS operands of type T: bf16 keeps 8 bits a part (two leave 2^-17 of the value, three all of fp32's).
+template <typename T, int PARTS> struct Split;
+template <int PARTS> struct Split<float, PARTS> {
+    static constexpr int kParts = 1;
+    Frag<float> p[1];
+    Split() = default;
+    __device__ explicit Split(const float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[0].v[e] = x[e];
+    }
+};
+template <int PARTS> struct Split<uint16_t, PARTS> {
+    static constexpr int kParts = PARTS;
+    Frag<uint16_t> p[PARTS];
+    Split() = default;
+    __device__ explicit Split(const float (&x)[8]) {
+        float rest[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rest[e] = x[e];
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = pack_bf16x2(rest[2 * i], rest[2 * i + 1]);
+                rest[2 * i] -= __uint_as_float(w[i] << 16);
+                rest[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+            }
+            p[k].v = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+    }
+};
+
+// places 8u..8u + 7 of one row of a tile
+__device__ inline Frag<uint16_t> row_frag(const uint16_t* at) { return {*reinterpret_cast<const bf16x8*>(at)}; }
+__device__ inline Frag<float> row_frag(const float* at) {
+    Frag<float> f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(at + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[4 * i + e] = v[e];
+    }
+    return f;
+}
+// places 4u..4u + 3 of two neighbouring groups of 16: how a state's accumulators hold their rows
+__device__ inline Frag<uint16_t> pair_frag(const uint16_t* at) {
+    const uint2 x = *reinterpret_cast<const uint2*>(at), y = *reinterpret_cast<const uint2*>(at + 16);
+    return {__builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y))};
+}
+__device__ inline Frag<float> pair_frag(const float* at) {
+    Frag<float> f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(at + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[4 * i + e] = v[e];
+    }
+    return f;
+}
+// eight rows of one column of a tile
+template <int STRIDE>
+__device__ inline Frag<uint16_t> col_frag(const uint16_t* at) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = at[2 * i * STRIDE] | (uint32_t)at[(2 * i + 1) * STRIDE] << 16;
+    return {__builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]))};
+}
+template <int STRIDE>
+__device__ inline Frag<float> col_frag(const float* at) {
+    Frag<float> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = at[e * STRIDE];
+    return f;
+}
+__device__ inline float value(const Frag<uint16_t>& f, int e) {
+    const uint4 w = __builtin_bit_cast(uint4, f.v);
+    const uint32_t x = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
+    return __uint_as_float(e & 1 ? x & 0xffff0000u : x << 16);
+}
+__device__ inline float value(const Frag<float>& f, int e) { return f.v[e]; }
+
+__device__ inline bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+template <typename T>
+__device__ inline bool any_not_finite(const u32x4& w) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
+        if constexpr (sizeof(T) == 2) bad |= (w[i] & 0x7f80u) == 0x7f80u;
+    }
+    return bad;
+}
+
+// 16 bytes of a row of which `left` elements are there, zeros behind them
+template <typename T>
+__device__ inline u32x4 load_unit(const T* at, int left) {
+    constexpr int E = 16 / sizeof(T);
+    u32x4 v = {0, 0, 0, 0};
+    if (left >= E) {
+        __builtin_memcpy(&v, at, 16);
+    } else if (left > 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (e >= left) break;
+            if constexpr (sizeof(T) == 4)
+                v[e] = __float_as_uint(at[e]);
+            else
+                v[e / 2] |= (uint32_t)at[e] << (16 * (e & 1));
+        }
+    }
+    return v;
+}
+
+template <typename T, int ROWS, int COLS, int THREADS>
+struct Tile {  // rows by columns of T in LDS, 16 bytes apart from a multiple of all banks
+    static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kUnits = ROWS * COLS / E, kEach = (kUnits + THREADS - 1) / THREADS;
+    static constexpr int kBytes = ROWS * kStride * sizeof(T);
+    u32x4 reg[kEach];
+    // rows that are there (the first `valid`) of the pass's chunk; `step` is a token's stride in the pass's direction
+    __device__ void load(const T* first, int64_t step, int valid, int cols) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int u = threadIdx.x + i * THREADS, row = u / (COLS / E), col = u % (COLS / E) * E;
+            reg[i] = u < kUnits && row < valid ? load_unit(first + row * step + col, cols - col) : u32x4{0, 0, 0, 0};
+        }
+    }
+    __device__ bool store(T* tile) const {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int u = threadIdx.x + i * THREADS, row = u / (COLS / E), col = u % (COLS / E) * E;
+            if (u < kUnits) *reinterpret_cast<u32x4*>(tile + row * kStride + col) = reg[i];
+            bad |= any_not_finite<T>(reg[i]);
+        }
+        return bad;
+    }
+};
+
+template <typename T> constexpr int kPParts = sizeof(T) == 2 ? 2 : 1;
+
+// One segment of one (sequence, head) through NW waves, 16 columns of the output to each; MP >= m channels of a and b, C tokens
+// a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state.
+template <typename T, int MP, int C, int NW, bool OUT, typename TO>
+__global__ __launch_bounds__(64 * NW) void mix_kernel(const MixArgs p) {
+    constexpr int THREADS = 64 * NW, MT = MP / 16, NT = C / 16, KB = C / 32, E = 16 / sizeof(T);
+    using TileM = Tile<T, C, MP, THREADS>;
+    using TileN = Tile<T, C, 16 * NW, THREADS>;
+    constexpr int PS = C + E;  // stride of the scores
+    extern __shared__ __align__(16) char lds[];
+    T* const tb = (T*)lds;
+    T* const tc = (T*)(lds + TileM::kBytes);
+    T* const ta = (T*)(lds + TileM::kBytes + TileN::kBytes);
+    T* const tp = (T*)(lds + 2 * TileM::kBytes + TileN::kBytes);
+    __shared__ int bad_rows[2];  // whether c's tile holds values that are not finite, this chunk's and the next one's
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, u = lane >> 4;
+
+    int64_t id = blockIdx.x;
+    const int slice = (int)(id % p.slices);
+    id /= p.slices;
+    const int seg = (int)(id % p.nseg);
+    id /= p.nseg;
+    const int h = (int)(id % p.H);
+    const int64_t b = id / p.H;
+    int64_t len = p.L;
+    if (p.lengths) {
+        const int64_t given = p.lengths[b];
+        len = given < 0 ? 0 : given < len ? given : len;
+    }
+    const float g = p.log_decay[h], l2 = log2_decay(g);
+    const int n0 = slice * 16 * NW, cols = p.n - n0 < 16 * NW ? p.n - n0 : 16 * NW;
+    const int64_t t0 = seg * p.seglen, t1 = t0 + p.seglen < p.L ? t0 + p.seglen : p.L;
+    const int64_t end = t1 < len ? t1 : len;
+    // token t of the pass is token len - 1 - t of the sequence where it goes backwards
+    const T* const pa = (const T*)p.a + b * p.L * p.lda + h / p.ga * p.m;
+    const T* const pb = (const T*)p.b + b * p.L * p.ldb + h / p.gb * p.m;
+    const T* const pc = (const T*)p.c + b * p.L * p.ldc + h / p.gc * p.n + n0;
+    const int64_t sign = p.back ? -1 : 1;
+    const int64_t state_at = ((b * p.H + h) * p.segs + seg) * p.state;
+
+    // S[mt]: rows 16 mt + 4u..+3 of the state's column n0 + 16 wave + r
+    const int col = n0 + 16 * wave + r;
+    f32x4 S[MT];
+    const bool entered = OUT && p.entry != nullptr;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * mt + 4 * u + e;
+            S[mt][e] = entered && row < p.m && col < p.n ? p.entry[state_at + (int64_t)row * p.sm + (int64_t)col * p.sn] : 0.0f;
+        }
+    if constexpr (OUT) {  // score tiles above the diagonal stay zero
+        for (int i = threadIdx.x; i < kPParts<T> * C * PS; i += THREADS) tp[i] = 0;
+    }
+
+    TileM ra, rb;
+    TileN rc;
+    const auto load = [&](int64_t t) {
+        const int valid = (int)(end - t < C ? end - t : C);
+        const int64_t at = p.back ? len - 1 - t : t;
+        if (valid <= 0) return;
+        rb.load(pb + at * p.ldb, sign * p.ldb, valid, p.m);
+        rc.load(pc + at * p.ldc, sign * p.ldc, valid, cols);
+        if constexpr (OUT) ra.load(pa + at * p.lda, sign * p.lda, valid, p.m);
+    };
+    load(t0);
+    if (threadIdx.x == 0) bad_rows[0] = 0;
+    bool first = true;
+    int turn = 0;
+    for (int64_t t = t0; t < end; t += C, turn ^= 1) {
+        const int valid = (int)(end - t < C ? end - t : C);
+        __syncthreads();  // the last chunk's tiles are read
+        if (threadIdx.x == 0) bad_rows[turn ^ 1] = 0;
+        rb.store(tb);
+        if (rc.store(tc)) bad_rows[turn] = 1;
+        if constexpr (OUT) ra.store(ta);
+        load(t + C);
+        __syncthreads();
+        f32x4 O[NT];
+        if constexpr (OUT) {
+            // scores: rows j of b against rows i of a, tiles on and below the diagonal
+            for (int job = wave; job < NT * (NT + 1) / 2; job += NW) {
+                int it = 0;
+                while ((it + 1) * (it + 2) / 2 <= job) ++it;
+                const int jt = job - it * (it + 1) / 2;
+                f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < MP / 32; ++k)
+                    s = mma(s, row_frag(tb + (16 * jt + r) * TileM::kStride + 32 * k + 8 * u), row_frag(ta + (16 * it + r) * TileM::kStride + 32 * k + 8 * u));
+                const int i = 16 * it + r, j = 16 * jt + 4 * u;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = i >= j + e ? s[e] * (p.ps * power(l2, i - j - e)) : 0.0f;
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<f32x4*>(tp + i * PS + j) = f32x4{x[0], x[1], x[2], x[3]};
+                } else {
+                    const uint32_t h0 = pack_bf16x2(x[0], x[1]), h1 = pack_bf16x2(x[2], x[3]);
+                    *reinterpret_cast<uint2*>(tp + i * PS + j) = make_uint2(h0, h1);
+                    *reinterpret_cast<uint2*>(tp + C * PS + i * PS + j) =
+                        make_uint2(pack_bf16x2(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xffff0000u)),
+                                   pack_bf16x2(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xffff0000u)));
+                }
+            }
+            // what came before the chunk, through the state
+#pragma unroll
+            for (int it = 0; it < NT; ++it) O[it] = f32x4{0, 0, 0, 0};
+            if (entered || !first) {
+#pragma unroll
+                for (int k = 0; k < MT / 2; ++k) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = S[2 * k + e / 4][e % 4];
+                    const Split<T, 2> s(x);
+#pragma unroll
+                    for (int it = 0; it < NT; ++it) {
+                        const Frag<T> a = pair_frag(ta + (16 * it + r) * TileM::kStride + 32 * k + 4 * u);
+#pragma unroll
+                        for (int q = 0; q < s.kParts; ++q) O[it] = mma(O[it], s.p[q], a);
+                    }
+                }
+#pragma unroll
+                for (int it = 0; it < NT; ++it) {
+                    const float w = p.es * power(l2, 16 * it + r + p.e0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) O[it][e] *= w;
+                }
+            }
+            __syncthreads();  // the scores are there
+        }
+        Frag<T> c[KB];
+#pragma unroll
+        for (int k = 0; k < KB; ++k) c[k] = col_frag<TileN::kStride>(tc + (32 * k + 8 * u) * TileN::kStride + 16 * wave + r);
+        const bool bad = bad_rows[turn];
+        if constexpr (OUT) {
+            Frag<T> f[KB];
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                f[k] = c[k];
+                if (bad) {  // a masked score does not cancel what is not finite: such values are added by themselves below
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = not_finite(value(c[k], e)) ? 0.0f : value(c[k], e);
+                    f[k] = Split<T, 1>(x).p[0];
+                }
+            }
+#pragma unroll
+            for (int it = 0; it < NT; ++it)
+#pragma unroll
+                for (int k = 0; k <= it / 2; ++k)
+#pragma unroll
+                    for (int q = 0; q < kPParts<T>; ++q)
+                        O[it] = mma(O[it], f[k], row_frag(tp + q * C * PS + (16 * it + r) * PS + 32 * k + 8 * u));
+            if (bad) {
+                for (int j = 0; j < valid; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = Storage<T>::load(tc + j * TileN::kStride + 16 * wave + 4 * u + e);
+                        if (not_finite(v)) {
+#pragma unroll
+                            for (int it = 0; it < NT; ++it) {
+                                float s = Storage<T>::load(tp + (16 * it + r) * PS + j);
+                                if constexpr (sizeof(T) == 2) s += Storage<T>::load(tp + C * PS + (16 * it + r) * PS + j);
+                                if (16 * it + r >= j) O[it][e] += s * v;
+                            }
+                        }
+                    }
+            }
+            // rows 4u..+3 of the wave's columns, token 16 it + r
+            const int left = cols - 16 * wave - 4 * u;
+            TO* const po = (TO*)p.out + b * p.L * p.ldo + (int64_t)h * p.n + n0 + 16 * wave + 4 * u;
+#pragma unroll
+            for (int it = 0; it < NT; ++it) {
+                const int i = 16 * it + r;
+                if (i >= valid || left <= 0) continue;
+                TO* at = po + (p.back ? len - 1 - t - i : t + i) * p.ldo;
+                if (left >= 4) {
+                    if constexpr (sizeof(TO) == 4) {
+                        __builtin_memcpy(at, &O[it], 16);
+                    } else {
+                        const uint2 w = make_uint2(pack_bf16x2(O[it][0], O[it][1]), pack_bf16x2(O[it][2], O[it][3]));
+                        __builtin_memcpy(at, &w, 8);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (e < left) Storage<TO>::store(at + e, O[it][e]);
+                }
+            }
+        }
+        // the state after the chunk
+        if (p.ends || t + C < end) {
+            // the chunk's part is summed by itself, so that the state is rounded once a chunk
+            const Decay decay(g, (float)valid);
+            Split<T, 3> v[KB];
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int j = 32 * k + 8 * u + e;
+                    x[e] = j < valid ? value(c[k], e) * (p.cs * power(l2, valid - j - p.e0)) : 0.0f;
+                }
+                v[k] = Split<T, 3>(x);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    const Frag<T> a = col_frag<TileM::kStride>(tb + (32 * k + 8 * u) * TileM::kStride + 16 * mt + r);
+#pragma unroll
+                    for (int q = 0; q < v[k].kParts; ++q) s = mma(s, a, v[k].p[q]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[mt][e] = decay(S[mt][e], s[e]);
+            }
+        }
+        first = false;
+    }
+    if (p.ends) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * mt + 4 * u + e;
+                if (row < p.m && col < p.n) p.ends[state_at + (int64_t)row * p.sm + (int64_t)col * p.sn] = S[mt][e];
+            }
+    }
+    if constexpr (OUT) {  // rows behind a sequence's length
+        const int64_t from = t0 > end ? t0 : end;
+        TO* const po = (TO*)p.out + b * p.L * p.ldo + (int64_t)h * p.n + n0;
+        for (int64_t i = threadIdx.x; i < (t1 - from) * cols; i += THREADS)
+            Storage<TO>::store(po + (from + i / cols) * p.ldo + i % cols, 0.0f);
+    }
+}
+
+// Segments' end states, each from a zero state, to the states before them, in place; the last one's state to `last`.
+__global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_t seglen, int nseg, int64_t state,
+                                                    const float* __restrict__ log_decay, const int32_t* __restrict__ lengths,
+                                                    const float* __restrict__ init, float* __restrict__ ends, float* __restrict__ last) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= state) return;
+    const int64_t bh = blockIdx.y, b = bh / H;
+    int64_t len = L;
+    if (lengths) {
+        const int64_t given = lengths[b];
+        len = given < 0 ? 0 : given < L ? given : L;
+    }
+    const float g = log_decay[bh % H];
+    float cur = init ? init[bh * state + i] : 0.0f;
+    float* at = ends + bh * nseg * state + i;
+    const Decay whole(g, (float)seglen);
+    for (int s = 0; s < nseg; ++s, at += state) {
+        const int64_t left = len - s * seglen;
+        const float e = *at;
+        *at = cur;
+        if (left >= seglen)
+            cur = whole(cur, e);
+        else if (left > 0)
+            cur = Decay(g, (float)left)(cur, e);
+    }
+    if (last) last[bh * state + i] = cur;
+}
+
+// y[row][h][c] = sum over the heads of a group of x, in their order, rounded once
+template <typename T>
+__global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int heads, int group, int n, const float* __restrict__ x, T* __restrict__ y) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int64_t c = i % n, rh = i / n;
+    float s = 0.0f;
+    for (int k = 0; k < group; ++k) s += x[(rh * group + k) * n + c];
+    Storage<T>::store(y + i, s);
+}
+
+// ------------------------------------------------------------------ one token
+// S = e^g S + k v^T, out = scale q S: a state is read and written once. A block takes 64 columns of one (sequence, head): 16
+// threads hold four columns each of a row, 16 rows at a time; the rows' parts of q S are joined in LDS in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(256) void step_kernel(int64_t H, int dk, int dv, int gq, int gk, int gv, float* __restrict__ state,
+                                                   const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk,
+                                                   const T* __restrict__ v, int64_t ldv, const float* __restrict__ log_decay, float scale,
+                                                   T* __restrict__ out) {
+    const int64_t bh = blockIdx.x, b = bh / H, h = bh % H;
+    const int c0 = blockIdx.y * 64 + threadIdx.x % 16 * 4, row = threadIdx.x / 16;
+    const T *pq = q + b * ldq + h / gq * dk, *pk = k + b * ldk + h / gk * dk, *pv = v + b * ldv + h / gv * dv;
+    const Decay decay(log_decay[h], 1.0f);
+    const int left = dv - c0;
+    float vv[4], sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vv[e] = e < left ? Storage<T>::load(pv + c0 + e) : 0.0f;
+    float* s = state + bh * dk * dv + c0;
+    for (int m = row; m < dk; m += 16) {
+        const float qm = Storage<T>::load(pq + m), km = Storage<T>::load(pk + m);
+        float* at = s + (int64_t)m * dv;
+        if (left >= 4) {
+            f32x4 x;
+            __builtin_memcpy(&x, at, 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = decay(x[e], km * vv[e]);
+                sum[e] = fmaf(qm, x[e], sum[e]);
+            }
+            __builtin_memcpy(at, &x, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < left) {
+                    at[e] = decay(at[e], km * vv[e]);
+                    sum[e] = fmaf(qm, at[e], sum[e]);
+                }
+        }
+    }
+    __shared__ float part[16][64];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[row][threadIdx.x % 16 * 4 + e] = sum[e];
+    __syncthreads();
+    const int c = blockIdx.y * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && c < dv) {
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y += part[i][threadIdx.x];
+        Storage<T>::store(out + bh * dv + c, y * scale);
+    }
+}
+
+// ------------------------------------------------------------------ host
+constexpr int kMaxChannels = 256;
+int chunk_of(int dtype) { return dtype == HX_BF16 ? 64 : 32; }
+
+// Segments that a sequence is cut into where the (sequence, head) pairs leave compute units idle.
+int64_t segments_of(int64_t B, int64_t L, int64_t H, int dtype, int64_t* seglen) {
+    const int64_t C = chunk_of(dtype), chunks = (L + C - 1) / C, pairs = B * H;
+    int64_t want = pairs > 0 ? 1024 / pairs : 1;
+    const int64_t most = chunks / 4;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    const int64_t per = (chunks + want - 1) / want;
+    *seglen = (per > 0 ? per : 1) * C;
+    return chunks > 0 ? (chunks + per - 1) / per : 1;
+}
+
+struct Shape {
+    int64_t B, L, H, hq, hk, hv, dk, dv;
+    int dtype;
+};
+
+int check_shape(const char* what, const Shape& s) {
+    HX_REQUIRE(s.B >= 0 && s.L >= 0 && s.H >= 0 && s.hq >= 0 && s.hk >= 0 && s.hv >= 0 && s.dk >= 0 && s.dv >= 0, HX_ERR_INVALID_DIMENSION,
+               "%s: negative size", what);
+    HX_REQUIRE(s.dtype == HX_F32 || s.dtype == HX_BF16, HX_ERR_DTYPE_MISMATCH, "%s: dtype %d", what, s.dtype);
+    if (s.H == 0) return HX_OK;
+    HX_REQUIRE(s.hq > 0 && s.hk > 0 && s.hv > 0 && s.H % s.hq == 0 && s.H % s.hk == 0 && s.H % s.hv == 0, HX_ERR_SHAPE_MISMATCH,
+               "%s: q, k and v need heads that divide %lld (%lld, %lld, %lld)", what, (long long)s.H, (long long)s.hq, (long long)s.hk, (long long)s.hv);
+    HX_REQUIRE(s.dk > 0 && s.dv > 0, HX_ERR_INVALID_DIMENSION, "%s: a head without channels", what);
+    HX_REQUIRE(s.dk <= kMaxChannels && s.dv <= kMaxChannels, HX_ERR_UNSUPPORTED, "%s: at most %d channels a head", what, kMaxChannels);
+    HX_REQUIRE(s.B < (1 << 24) && s.H < (1 << 16) && s.B * s.H < (1 << 24) && s.L < ((int64_t)1 << 40) / (s.B > 0 ? s.B : 1), HX_ERR_UNSUPPORTED,
+               "%s: batch * heads below 2^24, heads below 2^16, batch * seqlen below 2^40", what);
+    return HX_OK;
+}
+
+template <typename T, int MP, int NW, bool OUT, typename TO>
+int launch_mix_of(MixArgs& p, hipStream_t stream) {
+    constexpr int C = sizeof(T) == 2 ? 64 : 32;
+    using TileM = Tile<T, C, MP, 64 * NW>;
+    using TileN = Tile<T, C, 16 * NW, 64 * NW>;
+    constexpr size_t bytes = (OUT ? 2 : 1) * TileM::kBytes + TileN::kBytes + (OUT ? kPParts<T> * C * (C + 16 / sizeof(T)) * sizeof(T) : 0);
+    const auto k = mix_kernel<T, MP, C, NW, OUT, TO>;
+    HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 16), HX_ERR_BACKEND, "decay_attention: %zu bytes of LDS not granted", bytes);
+    p.slices = (p.n + 16 * NW - 1) / (16 * NW);
+    const int64_t blocks = p.B * p.H * p.nseg * p.slices;
+    HX_REQUIRE(blocks < ((int64_t)1 << 32) / (64 * NW), HX_ERR_UNSUPPORTED, "decay_attention: too many blocks");
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * NW), bytes, stream, p);
+    HX_LAUNCH_CHECK();
+    return HX_OK;
+}
+template <typename T, bool OUT, typename TO>
+int launch_mix(MixArgs p, hipStream_t s) {
+    if (p.n > 64) {
+        if (p.m <= 64) return launch_mix_of<T, 64, 8, OUT, TO>(p, s);
+        if (p.m <= 128) return launch_mix_of<T, 128, 8, OUT, TO>(p, s);
+        return launch_mix_of<T, 256, 8, OUT, TO>(p, s);
+    }
+    if (p.m <= 64) return launch_mix_of<T, 64, 4, OUT, TO>(p, s);
+    if (p.m <= 128) return launch_mix_of<T, 128, 4, OUT, TO>(p, s);
+    return launch_mix_of<T, 256, 4, OUT, TO>(p, s);
+}
+
+// One pass: the segments' states and their chain where there is more than one, then the outputs. `init` and `last`: the states
+// before and after all tokens (nullable).
+int mix(MixArgs p, int dtype, bool out_f32, const float* init, float* last, float* states, hipStream_t s) {
+    if (p.nseg > 1) {
+        MixArgs e = p;
+        e.entry = nullptr;
+        e.ends = states;
+        e.segs = p.nseg;
+        int rc = dtype == HX_F32 ? launch_mix<float, false, float>(e, s) : launch_mix<uint16_t, false, uint16_t>(e, s);
+        if (rc != HX_OK) return rc;
+        const dim3 grid((unsigned)((p.state + 255) / 256), (unsigned)(p.B * p.H));
+        HX_REQUIRE(p.B * p.H < 65536, HX_ERR_UNSUPPORTED, "decay_attention: batch * heads below 2^16 for segments");
+        hipLaunchKernelGGL(chain_kernel, grid, dim3(256), 0, s, p.H, p.L, p.seglen, p.nseg, p.state, p.log_decay, p.lengths, init, states, last);
+        HX_LAUNCH_CHECK();
+        p.entry = states;
+        p.ends = nullptr;
+        p.segs = p.nseg;
+    } else {
+        p.entry = init;
+        p.ends = last;
+        p.segs = 1;
+    }
+    if (dtype == HX_F32) return launch_mix<float, true, float>(p, s);
+    return out_f32 ? launch_mix<uint16_t, true, float>(p, s) : launch_mix<uint16_t, true, uint16_t>(p, s);
+}
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+template <typename T>
+int group_sum(int64_t rows, int64_t H, int64_t heads, int64_t n, const float* x, void* y, hipStream_t s) {
+    const int64_t total = rows * heads * n, blocks = (total + 255) / 256;
+    HX_REQUIRE(blocks < ((int64_t)1 << 24), HX_ERR_UNSUPPORTED, "decay_attention: too many elements of shared heads");
+    hipLaunchKernelGGL(group_sum_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, total, (int)heads, (int)(H / heads), (int)n, x, (T*)y);
+    HX_LAUNCH_CHECK();
+    return HX_OK;
+}
+
+}  // namespace
+}  // namespace hx
+
+extern "C" size_t hx_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv, int dtype) {
+    using namespace hx;
+    if (check_shape("decay_attention", {batch, seqlen, heads, heads, heads, heads, dk, dv, dtype}) != HX_OK) return 0;
+    if (batch == 0 || heads == 0) return 0;
+    int64_t seglen;
+    const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen);
+    return nseg > 1 ? (size_t)(batch * heads * nseg * dk * dv * 4) : 0;
+}
+
+extern "C" int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads, int64_t k_heads, int64_t v_heads, int64_t dk,
+                                      int64_t dv, int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                      const float* log_decay, float scale, const int32_t* lengths, const float* init_state, void* out,
+                                      float* last_state, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace hx;
+    const Shape s{batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv, dtype};
+    int rc = check_shape("decay_attention_fwd", s);
+    if (rc != HX_OK || batch == 0 || heads == 0) return rc;
+    HX_REQUIRE(log_decay && (seqlen == 0 || (out && q && k && v)), HX_ERR_INVALID_INPUT, "decay_attention_fwd: NULL pointer");
+    HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_fwd: a stride is shorter than a token");
+    int64_t seglen;
+    const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen);
+    const size_t need = hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype);
+    HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), HX_ERR_INVALID_INPUT,
+               "decay_attention_fwd: workspace of %zu bytes (16-byte aligned) required", need);
+    MixArgs p{};
+    p.a = q, p.b = k, p.c = v;
+    p.lda = ldq, p.ldb = ldk, p.ldc = ldv;
+    p.ga = (int)(heads / q_heads), p.gb = (int)(heads / k_heads), p.gc = (int)(heads / v_heads);
+    p.B = batch, p.L = seqlen, p.H = heads;
+    p.m = (int)dk, p.n = (int)dv;
+    p.log_decay = log_decay, p.lengths = lengths;
+    p.state = dk * dv, p.sm = (int)dv, p.sn = 1;
+    p.ps = p.es = scale, p.cs = 1.0f, p.e0 = 1, p.back = 0;
+    p.out = out, p.ldo = heads * dv;
+    p.seglen = seglen, p.nseg = (int)nseg;
+    return mix(p, dtype, false, init_state, last_state, (float*)workspace, as_stream(stream));
+}
+
+// bytes of the fp32 gradients of an operand that heads share
+static size_t hx_shared_bytes(int64_t rows, int64_t H, int64_t heads, int64_t n) { return heads == H ? 0 : hx::round16((size_t)(rows * H * n * 4)); }
+
+extern "C" size_t hx_decay_attention_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads, int64_t k_heads,
+                                                        int64_t v_heads, int64_t dk, int64_t dv, int dtype) {
+    using namespace hx;
+    if (check_shape("decay_attention_bwd", {batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv, dtype}) != HX_OK) return 0;
+    if (batch == 0 || heads == 0) return 0;
+    const int64_t rows = batch * seqlen;
+    return round16(hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype)) + hx_shared_bytes(rows, heads, q_heads, dk) +
+           hx_shared_bytes(rows, heads, k_heads, dk) + hx_shared_bytes(rows, heads, v_heads, dv);
+}
+
+extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads, int64_t k_heads, int64_t v_heads, int64_t dk,
+                                      int64_t dv, int dtype, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                      const float* log_decay, float scale, const int32_t* lengths, const float* init_state, const void* dout,
+                                      const float* dlast, void* dq, void* dk_out, void* dv_out, float* dinit, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+    using namespace hx;
+    const Shape sh{batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv, dtype};
+    int rc = check_shape("decay_attention_bwd", sh);
+    if (rc != HX_OK || batch == 0 || heads == 0) return rc;
+    HX_REQUIRE(log_decay && (seqlen == 0 || (q && k && v && dout && dq && dk_out && dv_out)), HX_ERR_INVALID_INPUT, "decay_attention_bwd: NULL pointer");
+    HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_bwd: a stride is shorter than a token");
+    const size_t need = hx_decay_attention_bwd_workspace_size(batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv, dtype);
+    HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), HX_ERR_INVALID_INPUT,
+               "decay_attention_bwd: workspace of %zu bytes (16-byte aligned) required", need);
+    hipStream_t s = as_stream(stream);
+    int64_t seglen;
+    const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen), rows = batch * seqlen;
+    char* at = (char*)workspace;
+    float* const states = (float*)at;
+    at += round16(hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype));
+    MixArgs p{};
+    p.B = batch, p.L = seqlen, p.H = heads;
+    p.log_decay = log_decay, p.lengths = lengths;
+    p.state = dk * dv;
+    p.seglen = seglen, p.nseg = (int)nseg;
+    const int gq = (int)(heads / q_heads), gk = (int)(heads / k_heads), gv = (int)(heads / v_heads);
+    const int64_t ldo = heads * dv;
+    const auto pass = [&](const void* a, int64_t lda, int ga, const void* b, int64_t ldb, int gb, const void* c, int64_t ldc, int gc, bool transposed,
+                          bool back, const float* init, float* last, void* out, int64_t out_heads) -> int {
+        p.a = a, p.b = b, p.c = c, p.lda = lda, p.ldb = ldb, p.ldc = ldc, p.ga = ga, p.gb = gb, p.gc = gc;
+        const int64_t m = transposed ? dv : dk, n = transposed ? dk : dv;
+        p.m = (int)m, p.n = (int)n;
+        p.sm = transposed ? 1 : (int)dv, p.sn = transposed ? (int)dv : 1;
+        p.back = back, p.e0 = back ? 0 : 1;
+        p.ps = scale, p.es = back ? 1.0f : scale, p.cs = back ? scale : 1.0f;
+        const bool shared = out_heads != heads;
+        float* wide = (float*)at;
+        if (shared) at += hx_shared_bytes(rows, heads, out_heads, n);
+        p.out = shared ? wide : out;
+        p.ldo = heads * n;
+        int rc = mix(p, dtype, shared, init, last, states, s);
+        if (rc == HX_OK && shared && rows > 0)
+            rc = dtype == HX_F32 ? group_sum<float>(rows, heads, out_heads, n, wide, out, s) : group_sum<uint16_t>(rows, heads, out_heads, n, wide, out, s);
+        return rc;
+    };
+    rc = pass(dout, ldo, 1, v, ldv, gv, k, ldk, gk, true, false, init_state, nullptr, dq, q_heads);
+    if (rc == HX_OK) rc = pass(v, ldv, gv, dout, ldo, 1, q, ldq, gq, true, true, dlast, nullptr, dk_out, k_heads);
+    if (rc == HX_OK) rc = pass(k, ldk, gk, q, ldq, gq, dout, ldo, 1, false, true, dlast, dinit, dv_out, v_heads);
+    return rc;
+}
+
+extern "C" int hx_decay_attention_step(int64_t batch, int64_t heads, int64_t q_heads, int64_t k_heads, int64_t v_heads, int64_t dk, int64_t dv,
+                                       int dtype, float* state, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                       const float* log_decay, float scale, void* out, void* stream) {
+    using namespace hx;
+    const Shape s{batch, 1, heads, q_heads, k_heads, v_heads, dk, dv, dtype};
+    int rc = check_shape("decay_attention_step", s);
+    if (rc != HX_OK || batch == 0 || heads == 0) return rc;
+    HX_REQUIRE(log_decay && out && state && q && k && v, HX_ERR_INVALID_INPUT, "decay_attention_step: NULL pointer");
+    HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_step: a stride is shorter than a token");
+    const dim3 grid((unsigned)(batch * heads), (unsigned)((dv + 63) / 64));
+    const int gq = (int)(heads / q_heads), gk = (int)(heads / k_heads), gv = (int)(heads / v_heads);
+    if (dtype == HX_F32)
+        hipLaunchKernelGGL(step_kernel<float>, grid, dim3(256), 0, as_stream(stream), heads, (int)dk, (int)dv, gq, gk, gv, state, (const float*)q, ldq,
+                           (const float*)k, ldk, (const float*)v, ldv, log_decay, scale, (float*)out);
+    else
+        hipLaunchKernelGGL(step_kernel<uint16_t>, grid, dim3(256), 0, as_stream(stream), heads, (int)dk, (int)dv, gq, gk, gv, state, (const uint16_t*)q, ldq,
+                           (const uint16_t*)k, ldk, (const uint16_t*)v, ldv, log_decay, scale, (uint16_t*)out);
+    HX_LAUNCH_CHECK();
+    return HX_OK;
+}

@@ -56,6 +56,42 @@ def rmsnorm(x, weight, eps=1e-5, out_dtype=torch.float32, out=None, stream=None)
     return out
 
 
+@on_current_or_launch_stream
+def add_rmsnorm(x, weight=None, delta=None, eps=1e-5, out_dtype=torch.int8, resid=None, out=None, stream=None):
+    """The residual's addition, RMSNorm and rounding to 8 bits in one pass (hx_add_rmsnorm) over the last axis of x [rows, dim]
+    (fp32 or bf16): r = x + delta (fp32 or bf16; None: x) in x's type, y = r / sqrt(mean(r^2) + eps) * weight (fp32 [dim];
+    None: no norm, y = r). ``resid``: where r goes (``x`` itself for in place); not kept when None. Returns y of
+    out_dtype fp32 or bf16, or, for int8, (codes, scales): codes int8 [rows, dim] and one fp32 scale a row, which stand
+    for codes * scales, as linear_i8 takes them. Rows of x, delta, resid and ``out`` (y, or the codes) may be strided."""
+    if x.dim() != 2:
+        raise _ffi.ShapeMismatch(f"x: expected [rows, dim], got {list(x.shape)}")
+    if x.dtype not in _STORAGE:
+        raise _ffi.DTypeMismatch(f"x: {x.dtype} is neither float32 nor bfloat16")
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype != torch.int8 and out_dtype not in _STORAGE:
+        raise _ffi.DTypeMismatch(f"out_dtype {out_dtype} is none of int8, float32, bfloat16")
+    rows, dim = shape = x.shape
+    ldx = _rows(stream, x, "x", shape, x.dtype)
+    ldd = ldr = dim
+    if delta is not None:
+        if delta.dtype not in _STORAGE:
+            raise _ffi.DTypeMismatch(f"delta: {delta.dtype} is neither float32 nor bfloat16")
+        ldd = _rows(stream, delta, "delta", shape, delta.dtype)
+    if resid is not None:
+        ldr = _rows(stream, resid, "resid", shape, x.dtype)
+    _operands(stream, ("weight", weight, (dim,), torch.float32))
+    if out is None:
+        out, ldy = torch.empty(shape, device=x.device, dtype=out_dtype), dim
+    else:
+        ldy = _rows(stream, out, "out", shape, out_dtype)
+    scales = torch.empty((rows,), device=x.device, dtype=torch.float32) if out_dtype == torch.int8 else None
+    _ffi.call("hx_add_rmsnorm", rows, dim, _STORAGE[x.dtype], _ptr(x), ldx, _F32 if delta is None else _STORAGE[delta.dtype], _ptr(delta), ldd,
+              _ptr(weight), float(eps), _ptr(resid), ldr, _ffi.HX_I8 if scales is not None else _STORAGE[out_dtype], _ptr(out), ldy,
+              _ptr(scales), _stream(stream))
+    return out if scales is None else (out, scales)
+
+
 @on_launch_stream
 def conv1d_step(x, weight, bias, state, out=None, stream=None):
     """One recurrent step of the causal conv (hx_conv1d_step); x [batch, dim] (rows may be

@@ -322,6 +322,125 @@ def gated_state_update(state, x, f, z=None, out=None, stream=None):
     return out
 
 
+def _tokens(launch, t, name, shape, dtype):
+    """Checks a [batch, seqlen, heads, channels] operand whose tokens may be strided (a slice of a projection's output); the
+    elements from one token to the next."""
+    if not t.is_cuda:
+        raise InvalidInput(f"{name} must be a device tensor")
+    if t.shape != shape:
+        raise ShapeMismatch(f"{name}: expected {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise DTypeMismatch(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.device != launch.device:
+        _on_stream_device(launch, **{name: t})
+    if t.is_contiguous():
+        return shape[2] * shape[3]
+    bt, L, heads, n = shape
+    sb, st, sh, sn = t.stride()
+    ld = st if L > 1 else sb if bt > 1 else heads * n  # an axis of one has no stride: torch may report any
+    if (n > 1 and sn != 1) or (heads > 1 and sh != n) or ld < heads * n or (bt > 1 and sb != L * ld):
+        raise InvalidInput(f"{name} needs adjacent channels and heads, and one stride for all tokens")
+    return ld
+
+
+def _decay_heads(launch, q, k, v, log_decay, dims):
+    """Checks what every form of the attention takes: (batch, seqlen or 1, heads, q_heads, k_heads, v_heads, dk, dv), the
+    storage type's code and the three token strides."""
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+        raise ShapeMismatch(f"q, k, v: expected {dims} dims, got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    if log_decay.dim() != 1:
+        raise ShapeMismatch(f"log_decay: expected [heads], got {list(log_decay.shape)}")
+    st = q.dtype
+    if st not in _STORAGE:
+        raise DTypeMismatch(f"q: storage dtype {st} is neither float32 nor bfloat16")
+    if dims == 3:  # one token of every sequence
+        q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
+    bt, L, hq, dk = q.shape
+    hk, (hv, dv) = k.shape[2], v.shape[2:]
+    heads = log_decay.shape[0]
+    _operands(launch, ("log_decay", log_decay, (heads,), torch.float32))
+    ld = (_tokens(launch, q, "q", (bt, L, hq, dk), st), _tokens(launch, k, "k", (bt, L, hk, dk), st),
+          _tokens(launch, v, "v", (bt, L, hv, dv), st))
+    return (bt, L, heads, hq, hk, hv, dk, dv), _STORAGE[st], ld
+
+
+def _scratch(name, given, device, *sizes):
+    need = int(getattr(_ffi.lib(), name)(*sizes))
+    if need and given is None:
+        given = torch.empty(need, device=device, dtype=torch.uint8)
+    elif given is not None and not given.is_contiguous():
+        raise InvalidInput("workspace must be contiguous")
+    return (None, 0) if given is None else (given, given.numel() * given.element_size())
+
+
+@on_current_or_launch_stream
+def decay_attention_fwd(q, k, v, log_decay, scale=1.0, lengths=None, init_state=None, return_last_state=False, out=None,
+                        workspace=None, stream=None):
+    """Linear attention with one decay a head (hx_decay_attention_fwd): S_i = e^g S_{i-1} + k_i v_i^T, out_i = scale q_i^T S_i,
+    g = log_decay[head], a constant of the head. q: [batch, L, q_heads, dk], k: [batch, L, k_heads, dk], v: [batch, L, v_heads, dv]
+    fp32 or bf16, each with heads that divide log_decay's (fp32 [heads]) and are shared by groups of them; tokens may be
+    strided. lengths: int32 [batch], tokens of each sequence (all when None; rows of ``out`` behind them are zero).
+    init_state: [batch, heads, dk, dv] fp32. Returns out [batch, L, heads, dv], followed by the last state where asked for.
+    Nothing is recorded for autograd: decay_attention_bwd gives the gradients. ``workspace``: a uint8 device
+    tensor of at least decay_attention_workspace_size(...) bytes; allocated here when not given."""
+    sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 4)
+    bt, L, heads, hq, hk, hv, dk, dv = sizes
+    f32, state = torch.float32, (bt, heads, dk, dv)
+    _operands(stream, ("lengths", lengths, (bt,), torch.int32), ("init_state", init_state, state, f32), ("out", out, (bt, L, heads, dv), q.dtype))
+    if workspace is not None:
+        _on_stream_device(stream, workspace=workspace)
+    if out is None:
+        out = torch.empty((bt, L, heads, dv), device=q.device, dtype=q.dtype)
+    last = torch.empty(state, device=q.device, dtype=f32) if return_last_state else None
+    workspace, nbytes = _scratch("hx_decay_attention_workspace_size", workspace, q.device, bt, L, heads, dk, dv, code)
+    _ffi.call("hx_decay_attention_fwd", *sizes, code, _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay), float(scale),
+              _ptr(lengths), _ptr(init_state), _ptr(out), _ptr(last), _ptr(workspace), nbytes, _stream(stream))
+    return (out, last) if return_last_state else out
+
+
+@on_current_or_launch_stream
+def decay_attention_bwd(q, k, v, log_decay, dout, scale=1.0, lengths=None, init_state=None, dlast=None, workspace=None, stream=None):
+    """Gradients of decay_attention_fwd (hx_decay_attention_bwd): (dq, dk, dv, dinit) from dout [batch, L, heads, dv] and dlast
+    [batch, heads, dk, dv] fp32 (the last state's gradient; None: zero). The other arguments are the forward's. dq, dk, dv
+    have q's type and the operands' shapes (a shared head's is the sum over its group), dinit is fp32."""
+    sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 4)
+    bt, L, heads, hq, hk, hv, dk, dv = sizes
+    f32, state = torch.float32, (bt, heads, dk, dv)
+    _operands(stream, ("lengths", lengths, (bt,), torch.int32), ("init_state", init_state, state, f32), ("dlast", dlast, state, f32),
+              ("dout", dout, (bt, L, heads, dv), q.dtype))
+    if workspace is not None:
+        _on_stream_device(stream, workspace=workspace)
+    dq, dkeys, dvalues = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+    dinit = torch.empty(state, device=q.device, dtype=f32)
+    workspace, nbytes = _scratch("hx_decay_attention_bwd_workspace_size", workspace, q.device, *sizes, code)
+    _ffi.call("hx_decay_attention_bwd", *sizes, code, _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay), float(scale),
+              _ptr(lengths), _ptr(init_state), _ptr(dout), _ptr(dlast), _ptr(dq), _ptr(dkeys), _ptr(dvalues), _ptr(dinit),
+              _ptr(workspace), nbytes, _stream(stream))
+    return dq, dkeys, dvalues, dinit
+
+
+def decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype=torch.float32, backward=False, q_heads=None, k_heads=None,
+                                   v_heads=None) -> int:
+    """Bytes of scratch that decay_attention_fwd (or decay_attention_bwd, where shared heads count) needs."""
+    if not backward:
+        return int(_ffi.lib().hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, _STORAGE[dtype]))
+    own = (heads if n is None else n for n in (q_heads, k_heads, v_heads))
+    return int(_ffi.lib().hx_decay_attention_bwd_workspace_size(batch, seqlen, heads, *own, dk, dv, _STORAGE[dtype]))
+
+
+@on_current_or_launch_stream
+def decay_attention_step(state, q, k, v, log_decay, scale=1.0, out=None, stream=None):
+    """One token of that attention for every sequence (hx_decay_attention_step); advances ``state`` [batch, heads, dk, dv] fp32 in
+    place. q: [batch, q_heads, dk], k: [batch, k_heads, dk], v: [batch, v_heads, dv] (rows may be strided); out [batch, heads, dv]."""
+    (bt, _, heads, hq, hk, hv, dk, dv), code, ld = _decay_heads(stream, q, k, v, log_decay, 3)
+    _operands(stream, ("state", state, (bt, heads, dk, dv), torch.float32), ("out", out, (bt, heads, dv), q.dtype))
+    if out is None:
+        out = torch.empty((bt, heads, dv), device=q.device, dtype=q.dtype)
+    _ffi.call("hx_decay_attention_step", bt, heads, hq, hk, hv, dk, dv, code, _ptr(state), _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2],
+              _ptr(log_decay), float(scale), _ptr(out), _stream(stream))
+    return out
+
+
 def s4_discretize(a_real, a_imag, dt=0.1, device=None):
     """S4Block::discretize's decay (crates/nn/src/ssm.rs:113-120) through hx_s4_discretize:
     a = expf(a_real*dt) * cosf(a_imag*dt) computed on the host with the reference's libm, returned
@@ -525,6 +644,75 @@ def linear_w4(X, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out
         return out
     # a single row has no stride: torch may report any
     _ffi.call("hx_linear_w4", M, N, K, _ptr(X), X.stride(0) if M > 1 else K, _ptr(packed), _ptr(scales), _ptr(bias),
+              int(act), _STORAGE[out.dtype], _ptr(out), out.stride(0) if M > 1 else N, _stream(stream))
+    return out
+
+
+I8_ROWS = 64 * 65535  # of X that one hx_linear_i8 takes
+
+
+def _i8_pieces(N, K):
+    """Shape of packed 8-bit weights (include/helix_hip.h, "8-bit integer weights"): pieces of 16 rows by 64 columns."""
+    return -(-N // 16), -(-K // 64), 4, 16, 16
+
+
+def i8_quantize(W, device=None):
+    """Rounds a weight [N, K] to 8 bits with one scale an output channel (hx_i8_quantize): (packed, scales), int8
+    [ceil(N / 16), ceil(K / 64), 4, 16, 16] and fp32 [N] on ``device`` (W's own when None). Runs on the host, once per
+    weight; W is read back if it lives on the device."""
+    if W.dim() != 2:
+        raise ShapeMismatch(f"W: expected [N, K], got {list(W.shape)}")
+    N, K = W.shape
+    w = np.ascontiguousarray(W.detach().float().cpu().numpy())
+    packed, scales = np.zeros(_i8_pieces(N, K), np.int8), np.zeros(N, np.float32)
+    _ffi.call("hx_i8_quantize", N, K, w.ctypes.data, packed.ctypes.data, scales.ctypes.data)
+    device = W.device if device is None else device
+    return torch.from_numpy(packed).to(device), torch.from_numpy(scales).to(device)
+
+
+def i8_values(packed, scales, K):
+    """What packed 8-bit weights stand for: a float32 numpy array [N, K]."""
+    q, s = packed.cpu().numpy(), scales.cpu().numpy()
+    rows = q.transpose(0, 3, 1, 2, 4).reshape(q.shape[0] * 16, q.shape[1] * 64)
+    return rows[: s.shape[0], :K].astype(np.float32) * s[:, None]
+
+
+@on_current_or_launch_stream
+def linear_i8(X, x_scales, packed, scales, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=None):
+    """Y = X . W^T (+ bias)(, SiLU) with activations and weights in 8 bits (hx_linear_i8). X [M, K] int8 (rows may be strided)
+    with a scale a row x_scales fp32 [M], as lm.add_rmsnorm gives them; packed, scales: what i8_quantize gives for W [N, K]; bias
+    [N] fp32. act: bit 0 SiLU, bit 1 adds to ``out`` [M, N] (rows may be strided), which has to be given then."""
+    if X.dim() != 2 or scales.dim() != 1:
+        raise ShapeMismatch(f"X, scales: expected [M, K] and [N], got {list(X.shape)}, {list(scales.shape)}")
+    M, K = X.shape
+    N = scales.shape[0]
+    if X.dtype != torch.int8:
+        raise DTypeMismatch("linear_i8: X must be int8")
+    if K > 1 and X.stride(1) != 1:
+        raise InvalidInput("linear_i8: X needs unit column stride")
+    _operands(stream, ("x_scales", x_scales, (M,), torch.float32), ("packed", packed, _i8_pieces(N, K), torch.int8),
+              ("scales", scales, (N,), torch.float32), ("bias", bias, (N,), torch.float32))
+    if out is None:
+        if act & 2:
+            raise InvalidInput("linear_i8: act bit 1 adds to out, which is not given")
+        if out_dtype not in _STORAGE:
+            raise DTypeMismatch(f"out_dtype {out_dtype} is neither float32 nor bfloat16")
+        out = torch.empty((M, N), device=X.device, dtype=out_dtype)
+    elif tuple(out.shape) != (M, N):
+        raise ShapeMismatch(f"out: expected {[M, N]}, got {list(out.shape)}")
+    elif out.dtype not in _STORAGE:
+        raise DTypeMismatch(f"out: {out.dtype} is neither float32 nor bfloat16")
+    elif N > 1 and out.stride(1) != 1:
+        raise InvalidInput("linear_i8: out needs unit column stride")
+    if not X.is_cuda or not out.is_cuda:
+        raise InvalidInput("X and out must be device tensors")
+    _on_stream_device(stream, X=X, out=out)
+    if M > I8_ROWS:  # a row's result does not depend on the rows beside it, so they are cut anywhere
+        for i in range(0, M, I8_ROWS):
+            linear_i8.__wrapped__(X[i: i + I8_ROWS], x_scales[i: i + I8_ROWS], packed, scales, bias, act, out=out[i: i + I8_ROWS], stream=stream)
+        return out
+    # a single row has no stride: torch may report any
+    _ffi.call("hx_linear_i8", M, N, K, _ptr(X), X.stride(0) if M > 1 else K, _ptr(x_scales), _ptr(packed), _ptr(scales), _ptr(bias),
               int(act), _STORAGE[out.dtype], _ptr(out), out.stride(0) if M > 1 else N, _stream(stream))
     return out
 

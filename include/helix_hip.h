@@ -49,8 +49,9 @@ typedef enum {
 
 /* Storage dtypes. Arithmetic and recurrent state are always fp32.
  * (tensor_core::DType has no BF16, crates/tensor-core/src/dtype.rs:8-37; HX_BF16 is the
- * storage format the north-star config 3 asks for.) */
-typedef enum { HX_F32 = 0, HX_BF16 = 1 } hx_dtype;
+ * storage format the north-star config 3 asks for.) HX_I8: 8-bit integers with a scale a row, only
+ * where an entry point says so. */
+typedef enum { HX_F32 = 0, HX_BF16 = 1, HX_I8 = 2 } hx_dtype;
 
 /* ------------------------------------------------------------------ runtime */
 /* Library version, (major << 16) | (minor << 8) | patch. */
@@ -194,6 +195,59 @@ int hx_gated_scan_bwd(int64_t batch, int64_t seqlen, int64_t dim, int dtype, con
 int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, const void* x,
                           const void* f, const void* z, void* out, void* stream);
 
+/* ------------------------------------------------------------------ linear attention with a decay per head */
+/* A recurrence whose state is a matrix per head, over whole sequences (tokens i of a head, state [dk, dv]):
+ *   S_i = e^g S_{i-1} + k_i v_i^T;   out_i = scale * q_i^T S_i;   g = log_decay[head]
+ * the matrix member of the family (the reference's recurrences, crates/nn/src/ssm.rs:138-186, carry a
+ * state per channel). g is a constant of the head, -inf (nothing is kept) and 0 (everything is) among
+ * them; it has no gradient here.
+ * q: [batch, seqlen, q_heads, dk], k: [batch, seqlen, k_heads, dk], v: [batch, seqlen, v_heads, dv] of
+ * `dtype` with ldq, ldk, ldv elements from one token to the next (so they can be slices of one
+ * projection's output; a token's heads follow each other). q_heads, k_heads and v_heads each divide
+ * `heads`: head h reads head h / (heads / q_heads) of q, and so on (k and v shared by groups of queries,
+ * or q and k shared as a state-space block shares B and C). out: [batch, seqlen, heads, dv] of `dtype`.
+ * log_decay: [heads] fp32. init_state (nullable: zero), last_state (nullable): [batch, heads, dk, dv]
+ * fp32, which may be one buffer. lengths (nullable: seqlen): int32 [batch], clamped to [0, seqlen]; what
+ * lies behind a sequence's length is not read, its rows of out are zero, and last_state is the state
+ * after its last token (init_state for none).
+ * Tokens are taken in chunks through the matrix cores with fp32 sums (bf16 operands that are not stored
+ * as bf16 are split into two or three bf16 parts), the same bits on every call; an infinite value may
+ * become NaN, but nothing reaches the tokens before it. dk and dv 1..256, batch * heads < 2^24, heads <
+ * 2^16, batch * seqlen < 2^40. workspace: hx_decay_attention_workspace_size(...) bytes of device memory
+ * (0 where no sequence is cut into segments), 16-byte aligned; it holds nothing between calls, and one
+ * call uses it at a time. */
+size_t hx_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk,
+                                         int64_t dv, int dtype);
+int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads,
+                           int64_t k_heads, int64_t v_heads, int64_t dk, int64_t dv, int dtype,
+                           const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                           int64_t ldv, const float* log_decay, float scale, const int32_t* lengths,
+                           const float* init_state, void* out, float* last_state, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* Its backward pass. With G_i = e^g G_{i+1} + scale * q_i dout_i^T, dlast added at the last token:
+ *   dq_i = scale * S_i dout_i;  dk_i = G_i v_i;  dv_i = G_i^T k_i;  dinit = e^g G_0 (dlast for no tokens)
+ * dout: [batch, seqlen, heads, dv]; dq, dk_out, dv_out: like q, k and v but contiguous, all of `dtype`
+ * (a shared head's gradient is the sum over its group, rounded once; rows behind a length are zero).
+ * dlast (nullable: zero), dinit (nullable: not wanted): [batch, heads, dk, dv] fp32, which may be one
+ * buffer. The states are formed again. workspace as above. */
+size_t hx_decay_attention_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t heads,
+                                             int64_t q_heads, int64_t k_heads, int64_t v_heads,
+                                             int64_t dk, int64_t dv, int dtype);
+int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads,
+                           int64_t k_heads, int64_t v_heads, int64_t dk, int64_t dv, int dtype,
+                           const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                           int64_t ldv, const float* log_decay, float scale, const int32_t* lengths,
+                           const float* init_state, const void* dout, const float* dlast, void* dq,
+                           void* dk_out, void* dv_out, float* dinit, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* One token of it for every sequence: state [batch, heads, dk, dv] fp32 is advanced in place; q, k, v as
+ * above with seqlen 1 (ldq, ldk, ldv elements from one sequence to the next), out [batch, heads, dv]. */
+int hx_decay_attention_step(int64_t batch, int64_t heads, int64_t q_heads, int64_t k_heads,
+                            int64_t v_heads, int64_t dk, int64_t dv, int dtype, float* state,
+                            const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                            int64_t ldv, const float* log_decay, float scale, void* out,
+                            void* stream);
+
 /* ------------------------------------------------------------------ S4 recurrences */
 /* nn::ssm::S4Block::discretize(dt)'s real decay (crates/nn/src/ssm.rs:113-120) on HOST arrays:
  * a[n] = expf(a_real[n]*dt) * cosf(a_imag[n]*dt), each product rounded to f32 first, with the
@@ -312,6 +366,28 @@ int hx_linear_w4(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, co
                  const void* scales, const float* bias, int act, int out_dtype, void* Y,
                  int64_t ldy, void* stream);
 
+/* 8-bit integer weights with one scale per output channel: w[n][k] = code * scales[n], code in -127..127.
+ * `packed` holds pieces of 16 rows by HX_I8_COLS columns, ceil(N / 16) * ceil(K / HX_I8_COLS) of 1024
+ * bytes, those of the same 16 rows one after the other: a piece's byte 256 c + 16 r + j is row r, column
+ * 16 c + j of it, which is the order in which the matrix instruction's lanes hold it. Rows from N on and
+ * columns from K on are zero. */
+#define HX_I8_COLS 64
+/* Rounds weights w [N, K] (the Linear layout, row stride K) to that format, all three on the HOST: a
+ * row's scale is its largest magnitude / 127 (0 for a row of zeros), elements round to the nearest code,
+ * ties to the even one. A weight that is not finite is refused (HX_ERR_INVALID_INPUT). Done once per
+ * weight. */
+int hx_i8_quantize(int64_t N, int64_t K, const float* w, void* packed, float* scales);
+/* Y = X . W^T (+ bias)(, SiLU) with activations and weights in 8 bits, the nn::Linear layout
+ * (crates/nn/src/lib.rs:120-134): X [M, K] int8 (row stride ldx) with one scale a row x_scales [M] (what
+ * hx_add_rmsnorm gives with HX_I8), packed (16-byte aligned) and scales as above, bias [N] fp32
+ * (nullable), Y [M, N] of out_dtype HX_F32 or HX_BF16 (row stride ldy); act as in hx_gemm_bf16 (bit 0
+ * SiLU, bit 1 Y = Y + result). Products are summed exactly in 32-bit integers and scaled once, so a
+ * row's result does not depend on the rows beside it. Any M, N, K and any alignment of X and Y (K < 2^17, N <
+ * 2^28, M up to 64 * 65535, else HX_ERR_UNSUPPORTED). */
+int hx_linear_i8(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const float* x_scales,
+                 const void* packed, const float* scales, const float* bias, int act, int out_dtype,
+                 void* Y, int64_t ldy, void* stream);
+
 /* Causal depthwise conv1d over time + bias + SiLU (the Mamba block's conv, kernel `width` <= 4):
  * y[b,t,d] = silu(bias[d] + sum_j weight[d,j] * x[b, t-width+1+j, d]) with zero padding.
  * x: [batch, seqlen, dim] with row stride ldx (so it can be the x half of in_proj's output);
@@ -366,6 +442,21 @@ int hx_embedding_fwd(int64_t n_tokens, int64_t vocab, int64_t dim, const int32_t
  * epsilon per row from U[eps, eps + 1e-8) (lib.rs:262); this uses eps itself. */
 int hx_rmsnorm_fwd(int64_t rows, int64_t dim, const float* x, const float* weight, float eps,
                    int out_dtype, void* y, void* stream);
+
+/* The residual's addition, RMSNorm and rounding to 8 bits in one pass over rows of x [rows, dim]:
+ *   r = x + delta (rounded to x's type);  y = r / sqrt(mean(r^2) + eps) * weight
+ * dtype: x's and resid's; delta (nullable: none) of delta_dtype; both HX_F32 or HX_BF16. resid (nullable:
+ * not wanted) receives r and may be x or delta itself. weight [dim] fp32 (nullable: no norm, y = r).
+ * out_dtype HX_F32 or HX_BF16: y as such. HX_I8: codes of 8 bits with one scale a row, scales [rows]
+ * fp32, which stand for code * scale:
+ *   code = round(127 p / max|p|), ties to even, p = r * weight (the norm cancels);  scale = max|y| / 127
+ * (0, with codes 0, for a row of zeros; NaN, with codes 0, for one that holds what is not finite). Sums,
+ * products and codes are formed in 64 bits, so the codes are the definition's own. ldx, ldd, ldr, ldy:
+ * elements from one row to the next. nn::RMSNorm::forward (crates/nn/src/lib.rs:258-285) is its case
+ * without delta. Fewer than 2^22 rows (2^24 of up to 2048 elements). */
+int hx_add_rmsnorm(int64_t rows, int64_t dim, int dtype, const void* x, int64_t ldx, int delta_dtype,
+                   const void* delta, int64_t ldd, const float* weight, float eps, void* resid,
+                   int64_t ldr, int out_dtype, void* y, int64_t ldy, float* scales, void* stream);
 
 /* One recurrent step of the causal conv: y[b][d] = silu(bias[d] + sum_{j<w-1} weight[d][j] *
  * state[b][j][d] + weight[d][w-1] * x[b][d]), then state shifts in x. state [batch][w-1][dim]
