@@ -383,7 +383,7 @@ int hx_i8_quantize(int64_t N, int64_t K, const float* w, void* packed, float* sc
  * (nullable), Y [M, N] of out_dtype HX_F32 or HX_BF16 (row stride ldy); act as in hx_gemm_bf16 (bit 0
  * SiLU, bit 1 Y = Y + result). Products are summed exactly in 32-bit integers and scaled once, so a
  * row's result does not depend on the rows beside it. Any M, N, K and any alignment of X and Y (K < 2^17, N <
- * 2^28, M up to 64 * 65535, else HX_ERR_UNSUPPORTED). */
+ * 2^26, M up to 64 * 65535, else HX_ERR_UNSUPPORTED). */
 int hx_linear_i8(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const float* x_scales,
                  const void* packed, const float* scales, const float* bias, int act, int out_dtype,
                  void* Y, int64_t ldy, void* stream);
