@@ -137,13 +137,19 @@ __device__ inline Frag<float> pair_frag(const float* at) {
     }
     return f;
 }
-// eight rows of one column of a tile
+// Eight rows of one column of a tile: rows 8u.. of column r, `at` being what col_at gives for the tile's first row and column.
+// bf16 comes through the LDS's transposing read: of 16 lanes each names four neighbours of a row, four lanes to a row, and gets
+// four rows of its own column.
+template <typename T, int STRIDE>
+__device__ inline int col_at(int r, int u) {
+    return sizeof(T) == 2 ? (8 * u + r / 4) * STRIDE + r % 4 * 4 : 8 * u * STRIDE + r;
+}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 template <int STRIDE>
 __device__ inline Frag<uint16_t> col_frag(const uint16_t* at) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = at[2 * i * STRIDE] | (uint32_t)at[(2 * i + 1) * STRIDE] << 16;
-    return {__builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]))};
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * STRIDE));
+    return {__builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7))};
 }
 template <int STRIDE>
 __device__ inline Frag<float> col_frag(const float* at) {
@@ -160,6 +166,18 @@ __device__ inline float value(const Frag<uint16_t>& f, int e) {
 __device__ inline float value(const Frag<float>& f, int e) { return f.v[e]; }
 
 __device__ inline bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+__device__ inline Frag<uint16_t> finite_only(const Frag<uint16_t>& f) {
+    uint4 w = __builtin_bit_cast(uint4, f.v);
+    const auto keep = [](uint32_t x) {
+        return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+    };
+    return {__builtin_bit_cast(bf16x8, make_uint4(keep(w.x), keep(w.y), keep(w.z), keep(w.w)))};
+}
+__device__ inline Frag<float> finite_only(Frag<float> f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = not_finite(f.v[e]) ? 0.0f : f.v[e];
+    return f;
+}
 template <typename T>
 __device__ inline bool any_not_finite(const u32x4& w) {
     bool bad = false;
@@ -171,60 +189,96 @@ __device__ inline bool any_not_finite(const u32x4& w) {
     return bad;
 }
 
-// 16 bytes of a row of which `left` elements are there, zeros behind them
+// A row's elements from one of them on: 16 bytes moved down by `by` elements, zeros behind them.
 template <typename T>
-__device__ inline u32x4 load_unit(const T* at, int left) {
-    constexpr int E = 16 / sizeof(T);
-    u32x4 v = {0, 0, 0, 0};
-    if (left >= E) {
-        __builtin_memcpy(&v, at, 16);
-    } else if (left > 0) {
+__device__ inline u32x4 moved(const u32x4& v, int by) {
+    const uint32_t bits = 8 * sizeof(T) * by;
+    uint32_t w[8] = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (e >= left) break;
-            if constexpr (sizeof(T) == 4)
-                v[e] = __float_as_uint(at[e]);
-            else
-                v[e / 2] |= (uint32_t)at[e] << (16 * (e & 1));
-        }
+    for (int i = 0; i < 6; ++i) w[i] = bits & 64 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = bits & 32 ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], bits & 31);
     }
-    return v;
+    return u32x4{w[0], w[1], w[2], w[3]};
 }
 
-template <typename T, int ROWS, int COLS, int THREADS>
-struct Tile {  // rows by columns of T in LDS, 16 bytes apart from a multiple of all banks
-    static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kUnits = ROWS * COLS / E, kEach = (kUnits + THREADS - 1) / THREADS;
-    static constexpr int kBytes = ROWS * kStride * sizeof(T);
+// Rows by columns of T in LDS, 16 bytes apart from a multiple of all banks, and the registers through which a chunk of them comes
+// from global memory: a thread has the same 16 bytes of every few rows. Loads go out without a branch, rows and columns that are
+// not there reading ones that are; columns behind a row's end are never written to LDS and keep the zeros that it starts with.
+// WHOLE: rows end with a whole 16 bytes. Else the last 16 bytes end with the row and are moved into place.
+template <typename T, int ROWS, int COLS, int THREADS, bool WHOLE>
+struct Tile {
+    static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kPerRow = COLS / E, kStep = THREADS / kPerRow;
+    static constexpr int kEach = (ROWS + kStep - 1) / kStep, kBytes = ROWS * kStride * (int)sizeof(T);
+    static_assert(THREADS % kPerRow == 0, "a thread's column is the same in all rows");
     u32x4 reg[kEach];
-    // rows that are there (the first `valid`) of the pass's chunk; `step` is a token's stride in the pass's direction
-    __device__ void load(const T* first, int64_t step, int valid, int cols) {
+    int row, col, by, n;  // `by`: elements that what is loaded stands too early
+    bool in;
+    // columns c0.. of rows of n
+    __device__ void begin(int c0, int width) {
+        row = threadIdx.x / kPerRow;
+        n = width;
+        const int want = c0 + threadIdx.x % kPerRow * E, most = WHOLE || n >= E ? n - E : 0;
+        in = want < n;
+        col = want < most ? want : most;
+        by = want - col;
+    }
+    // Rows shift.. of the tile are tokens of a chunk, `valid` = ROWS - shift of them, the first (or, backwards, the last) at `first`.
+    __device__ void load(const T* first, int64_t ld, int shift, bool back) {
+        const int valid = ROWS - shift;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int u = threadIdx.x + i * THREADS, row = u / (COLS / E), col = u % (COLS / E) * E;
-            reg[i] = u < kUnits && row < valid ? load_unit(first + row * step + col, cols - col) : u32x4{0, 0, 0, 0};
+            int k = row + i * kStep - shift;
+            k = k < 0 ? 0 : k >= valid ? valid - 1 : k;
+            const uint32_t off = (uint32_t)((back ? valid - 1 - k : k) * (int)ld + col);
+            if (WHOLE || n >= E) {
+                __builtin_memcpy(&reg[i], first + off, 16);
+            } else {
+                T v[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = first[off + (e < n ? e : n - 1)];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = e < n ? v[e] : 0;
+                __builtin_memcpy(&reg[i], v, 16);
+            }
         }
     }
-    __device__ bool store(T* tile) const {
-        bool bad = false;
+    __device__ void store(T* tile, int shift) {
+        if constexpr (!WHOLE) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) reg[i] = moved<T>(reg[i], by);
+        }
+        if (!in) return;
+        T* const to = tile + row * kStride + threadIdx.x % kPerRow * E;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int u = threadIdx.x + i * THREADS, row = u / (COLS / E), col = u % (COLS / E) * E;
-            if (u < kUnits) *reinterpret_cast<u32x4*>(tile + row * kStride + col) = reg[i];
-            bad |= any_not_finite<T>(reg[i]);
+            const u32x4 v = row + i * kStep >= shift ? reg[i] : u32x4{0, 0, 0, 0};
+            if (ROWS % kStep == 0 || row + i * kStep < ROWS) *reinterpret_cast<u32x4*>(to + i * kStep * kStride) = v;
         }
-        return bad;
+    }
+    __device__ bool bad(int shift) const {
+        bool b = false;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) b |= any_not_finite<T>(reg[i]) && row + i * kStep >= shift;
+        return b && in;
     }
 };
 
 template <typename T> constexpr int kPParts = sizeof(T) == 2 ? 2 : 1;
+// waves to a SIMD that a kernel's LDS leaves room for, as its register bound
+template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT ? (MP > 128 ? 2 : 3) : MP > 128 ? (NW == 8 ? 2 : 1) : NW == 8 ? 2 : MP > 64 ? 2 : 3;
 
 // One segment of one (sequence, head) through NW waves, 16 columns of the output to each; MP >= m channels of a and b, C tokens
-// a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state.
-template <typename T, int MP, int C, int NW, bool OUT, typename TO>
-__global__ __launch_bounds__(64 * NW) void mix_kernel(const MixArgs p) {
+// a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state. A segment's last chunk that
+// is not whole stands at its tile's end, zeros before it, where its weights are a whole chunk's.
+template <typename T, int MP, int C, int NW, bool WHOLE, bool OUT, typename TO>
+__global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_kernel(const MixArgs p) {
     constexpr int THREADS = 64 * NW, MT = MP / 16, NT = C / 16, KB = C / 32, E = 16 / sizeof(T);
-    using TileM = Tile<T, C, MP, THREADS>;
-    using TileN = Tile<T, C, 16 * NW, THREADS>;
+    using TileM = Tile<T, C, MP, THREADS, WHOLE>;
+    using TileN = Tile<T, C, 16 * NW, THREADS, WHOLE>;
     constexpr int PS = C + E;  // stride of the scores
     extern __shared__ __align__(16) char lds[];
     T* const tb = (T*)lds;
@@ -235,143 +289,173 @@ __global__ __launch_bounds__(64 * NW) void mix_kernel(const MixArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, u = lane >> 4;
 
-    int64_t id = blockIdx.x;
-    const int slice = (int)(id % p.slices);
-    id /= p.slices;
-    const int seg = (int)(id % p.nseg);
-    id /= p.nseg;
-    const int h = (int)(id % p.H);
-    const int64_t b = id / p.H;
+    uint32_t id = blockIdx.x;
+    const int slice = (int)(id % (uint32_t)p.slices);
+    id /= (uint32_t)p.slices;
+    const int seg = (int)(id % (uint32_t)p.nseg);
+    id /= (uint32_t)p.nseg;
+    const int h = (int)(id % (uint32_t)p.H);
+    const int64_t b = id / (uint32_t)p.H;
     int64_t len = p.L;
     if (p.lengths) {
         const int64_t given = p.lengths[b];
         len = given < 0 ? 0 : given < len ? given : len;
     }
     const float g = p.log_decay[h], l2 = log2_decay(g);
-    const int n0 = slice * 16 * NW, cols = p.n - n0 < 16 * NW ? p.n - n0 : 16 * NW;
+    const int n0 = slice * 16 * NW;
     const int64_t t0 = seg * p.seglen, t1 = t0 + p.seglen < p.L ? t0 + p.seglen : p.L;
     const int64_t end = t1 < len ? t1 : len;
+    const bool back = p.back != 0;
+
+    // columns behind a row's end stay zero, and so do score tiles above the diagonal
+    constexpr int kAll = (OUT ? 2 : 1) * TileM::kBytes + TileN::kBytes + (OUT ? kPParts<T> * C * PS * (int)sizeof(T) : 0);
+    for (int i = threadIdx.x; i < kAll / 16; i += THREADS) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+
     // token t of the pass is token len - 1 - t of the sequence where it goes backwards
-    const T* const pa = (const T*)p.a + b * p.L * p.lda + h / p.ga * p.m;
-    const T* const pb = (const T*)p.b + b * p.L * p.ldb + h / p.gb * p.m;
-    const T* const pc = (const T*)p.c + b * p.L * p.ldc + h / p.gc * p.n + n0;
-    const int64_t sign = p.back ? -1 : 1;
-    const int64_t state_at = ((b * p.H + h) * p.segs + seg) * p.state;
-
-    // S[mt]: rows 16 mt + 4u..+3 of the state's column n0 + 16 wave + r
-    const int col = n0 + 16 * wave + r;
-    f32x4 S[MT];
-    const bool entered = OUT && p.entry != nullptr;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * mt + 4 * u + e;
-            S[mt][e] = entered && row < p.m && col < p.n ? p.entry[state_at + (int64_t)row * p.sm + (int64_t)col * p.sn] : 0.0f;
-        }
-    if constexpr (OUT) {  // score tiles above the diagonal stay zero
-        for (int i = threadIdx.x; i < kPParts<T> * C * PS; i += THREADS) tp[i] = 0;
-    }
-
     TileM ra, rb;
     TileN rc;
+    ra.begin(0, p.m);
+    rb.begin(0, p.m);
+    rc.begin(n0, p.n);
+    const T* const pa = (const T*)p.a + b * p.L * p.lda + h / p.ga * p.m;
+    const T* const pb = (const T*)p.b + b * p.L * p.ldb + h / p.gb * p.m;
+    const T* const pc = (const T*)p.c + b * p.L * p.ldc + h / p.gc * p.n;
     const auto load = [&](int64_t t) {
-        const int valid = (int)(end - t < C ? end - t : C);
-        const int64_t at = p.back ? len - 1 - t : t;
-        if (valid <= 0) return;
-        rb.load(pb + at * p.ldb, sign * p.ldb, valid, p.m);
-        rc.load(pc + at * p.ldc, sign * p.ldc, valid, cols);
-        if constexpr (OUT) ra.load(pa + at * p.lda, sign * p.lda, valid, p.m);
+        const int shift = end - t < C ? (int)(C - (end - t)) : 0;
+        const int64_t first = back ? len - t - (C - shift) : t;  // the chunk's lowest token
+        rb.load(pb + first * p.ldb, p.ldb, shift, back);
+        rc.load(pc + first * p.ldc, p.ldc, shift, back);
+        if constexpr (OUT) ra.load(pa + first * p.lda, p.lda, shift, back);
     };
-    load(t0);
+    if (t0 < end) load(t0);
+
+    // S[mt]: rows 16 mt + 4u..+3 of the state's column n0 + 16 wave + r
+    const int64_t state_at = ((b * p.H + h) * p.segs + seg) * p.state;
+    const int col = n0 + 16 * wave + r, col_in = (col < p.n ? col : p.n - 1) * p.sn;
+    f32x4 S[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) S[mt] = f32x4{0, 0, 0, 0};
+    if (OUT && p.entry) {
+        const float* const from = p.entry + state_at + col_in;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * mt + 4 * u + e;
+                const float v = from[(row < p.m ? row : p.m - 1) * p.sm];
+                S[mt][e] = row < p.m && col < p.n ? v : 0.0f;
+            }
+    }
+
+    // Weights of a lane's places: scores on and off the diagonal, tokens' part of the state.
+    float near[4], off[4], left[KB * 8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int d = r - 4 * u - e;
+        near[e] = p.ps * power(l2, d < 0 ? 0 : d);
+        off[e] = p.ps * power(l2, 16 + d);
+    }
+#pragma unroll
+    for (int i = 0; i < KB * 8; ++i) left[i] = p.cs * power(l2, C - (32 * (i / 8) + 8 * u + i % 8) - p.e0);
+
+    // places of a lane's fragments in the tiles
+    const int row_m = r * TileM::kStride + 8 * u, pair_m = r * TileM::kStride + 4 * u, row_p = r * PS + 8 * u;
+    const T* const col_b = tb + col_at<T, TileM::kStride>(r, u);
+    const T* const col_c = tc + col_at<T, TileN::kStride>(r, u) + 16 * wave;
+    const int more = p.n - n0 - 16 * wave - 4 * u;  // columns from this lane's first of the output on
+    TO* const po = (TO*)p.out + b * p.L * p.ldo + (int64_t)h * p.n + n0 + 16 * wave;
+
     if (threadIdx.x == 0) bad_rows[0] = 0;
-    bool first = true;
     int turn = 0;
+#pragma unroll 1
     for (int64_t t = t0; t < end; t += C, turn ^= 1) {
-        const int valid = (int)(end - t < C ? end - t : C);
-        __syncthreads();  // the last chunk's tiles are read
+        const int shift = end - t < C ? (int)(C - (end - t)) : 0;
+        lds_barrier();  // the last chunk's tiles are read
         if (threadIdx.x == 0) bad_rows[turn ^ 1] = 0;
-        rb.store(tb);
-        if (rc.store(tc)) bad_rows[turn] = 1;
-        if constexpr (OUT) ra.store(ta);
-        load(t + C);
-        __syncthreads();
+        rb.store(tb, shift);
+        rc.store(tc, shift);
+        if constexpr (OUT) {
+            ra.store(ta, shift);
+            if (rc.bad(shift)) bad_rows[turn] = 1;
+        }
+        if (t + C < end) load(t + C);
+        lds_barrier();
         f32x4 O[NT];
         if constexpr (OUT) {
             // scores: rows j of b against rows i of a, tiles on and below the diagonal
-            for (int job = wave; job < NT * (NT + 1) / 2; job += NW) {
-                int it = 0;
-                while ((it + 1) * (it + 2) / 2 <= job) ++it;
-                const int jt = job - it * (it + 1) / 2;
+#pragma unroll
+            for (int n = 0; n < (NT * (NT + 1) / 2 + NW - 1) / NW; ++n) {
+                const int job = wave + n * NW;
+                if (job >= NT * (NT + 1) / 2) break;
+                const int it = job < 1 ? 0 : job < 3 ? 1 : job < 6 ? 2 : 3, jt = job - it * (it + 1) / 2;
                 f32x4 s = {0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < MP / 32; ++k)
-                    s = mma(s, row_frag(tb + (16 * jt + r) * TileM::kStride + 32 * k + 8 * u), row_frag(ta + (16 * it + r) * TileM::kStride + 32 * k + 8 * u));
-                const int i = 16 * it + r, j = 16 * jt + 4 * u;
+                    s = mma(s, row_frag(tb + 16 * jt * TileM::kStride + row_m + 32 * k), row_frag(ta + 16 * it * TileM::kStride + row_m + 32 * k));
+                const float far = power(l2, 16 * (it > jt ? it - jt - 1 : 0));
                 float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = i >= j + e ? s[e] * (p.ps * power(l2, i - j - e)) : 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = s[e] * (it == jt ? near[e] : off[e] * far);
+                    x[e] = it > jt || r >= 4 * u + e ? x[e] : 0.0f;
+                }
+                T* const to = tp + (16 * it + r) * PS + 16 * jt + 4 * u;
                 if constexpr (sizeof(T) == 4) {
-                    *reinterpret_cast<f32x4*>(tp + i * PS + j) = f32x4{x[0], x[1], x[2], x[3]};
+                    *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
                 } else {
                     const uint32_t h0 = pack_bf16x2(x[0], x[1]), h1 = pack_bf16x2(x[2], x[3]);
-                    *reinterpret_cast<uint2*>(tp + i * PS + j) = make_uint2(h0, h1);
-                    *reinterpret_cast<uint2*>(tp + C * PS + i * PS + j) =
+                    *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
+                    *reinterpret_cast<uint2*>(to + C * PS) =
                         make_uint2(pack_bf16x2(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xffff0000u)),
                                    pack_bf16x2(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xffff0000u)));
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             // what came before the chunk, through the state
 #pragma unroll
             for (int it = 0; it < NT; ++it) O[it] = f32x4{0, 0, 0, 0};
-            if (entered || !first) {
 #pragma unroll
-                for (int k = 0; k < MT / 2; ++k) {
-                    float x[8];
+            for (int k = 0; k < MT / 2; ++k) {
+                float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = S[2 * k + e / 4][e % 4];
-                    const Split<T, 2> s(x);
-#pragma unroll
-                    for (int it = 0; it < NT; ++it) {
-                        const Frag<T> a = pair_frag(ta + (16 * it + r) * TileM::kStride + 32 * k + 4 * u);
-#pragma unroll
-                        for (int q = 0; q < s.kParts; ++q) O[it] = mma(O[it], s.p[q], a);
-                    }
-                }
+                for (int e = 0; e < 8; ++e) x[e] = S[2 * k + e / 4][e % 4];
+                const Split<T, 2> s(x);
 #pragma unroll
                 for (int it = 0; it < NT; ++it) {
-                    const float w = p.es * power(l2, 16 * it + r + p.e0);
+                    const Frag<T> a = pair_frag(ta + 16 * it * TileM::kStride + pair_m + 32 * k);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) O[it][e] *= w;
+                    for (int q = 0; q < s.kParts; ++q) O[it] = mma(O[it], s.p[q], a);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __syncthreads();  // the scores are there
+#pragma unroll
+            for (int it = 0; it < NT; ++it) {
+                const int i = 16 * it + r - shift;
+                const float w = p.es * power(l2, (i < 0 ? 0 : i) + p.e0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) O[it][e] *= w;
+            }
+            lds_barrier();  // the scores are there
         }
         Frag<T> c[KB];
 #pragma unroll
-        for (int k = 0; k < KB; ++k) c[k] = col_frag<TileN::kStride>(tc + (32 * k + 8 * u) * TileN::kStride + 16 * wave + r);
-        const bool bad = bad_rows[turn];
+        for (int k = 0; k < KB; ++k) c[k] = col_frag<TileN::kStride>(col_c + 32 * k * TileN::kStride);
         if constexpr (OUT) {
-            Frag<T> f[KB];
+            // A masked score does not cancel what is not finite: such values are left out here and added by themselves below.
+            const bool bad = bad_rows[turn];
+            if (bad) {
 #pragma unroll
-            for (int k = 0; k < KB; ++k) {
-                f[k] = c[k];
-                if (bad) {  // a masked score does not cancel what is not finite: such values are added by themselves below
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = not_finite(value(c[k], e)) ? 0.0f : value(c[k], e);
-                    f[k] = Split<T, 1>(x).p[0];
-                }
+                for (int k = 0; k < KB; ++k) c[k] = finite_only(c[k]);
             }
 #pragma unroll
             for (int it = 0; it < NT; ++it)
 #pragma unroll
                 for (int k = 0; k <= it / 2; ++k)
 #pragma unroll
-                    for (int q = 0; q < kPParts<T>; ++q)
-                        O[it] = mma(O[it], f[k], row_frag(tp + q * C * PS + (16 * it + r) * PS + 32 * k + 8 * u));
+                    for (int q = 0; q < kPParts<T>; ++q) O[it] = mma(O[it], c[k], row_frag(tp + q * C * PS + 16 * it * PS + row_p + 32 * k));
             if (bad) {
-                for (int j = 0; j < valid; ++j)
+#pragma unroll 1
+                for (int j = shift; j < C; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float v = Storage<T>::load(tc + j * TileN::kStride + 16 * wave + 4 * u + e);
@@ -384,73 +468,77 @@ __global__ __launch_bounds__(64 * NW) void mix_kernel(const MixArgs p) {
                             }
                         }
                     }
+#pragma unroll
+                for (int k = 0; k < KB; ++k) c[k] = col_frag<TileN::kStride>(col_c + 32 * k * TileN::kStride);
             }
-            // rows 4u..+3 of the wave's columns, token 16 it + r
-            const int left = cols - 16 * wave - 4 * u;
-            TO* const po = (TO*)p.out + b * p.L * p.ldo + (int64_t)h * p.n + n0 + 16 * wave + 4 * u;
+            __builtin_amdgcn_sched_barrier(0);
+            // rows 4u..+3 of the wave's columns, row 16 it + r of the tile
+            TO* const first = po + (back ? len - t - (C - shift) : t) * p.ldo;  // the chunk's lowest token
 #pragma unroll
             for (int it = 0; it < NT; ++it) {
-                const int i = 16 * it + r;
-                if (i >= valid || left <= 0) continue;
-                TO* at = po + (p.back ? len - 1 - t - i : t + i) * p.ldo;
-                if (left >= 4) {
+                const int i = 16 * it + r - shift;
+                TO* const to = first + (uint32_t)((back ? C - shift - 1 - i : i) * (int)p.ldo + 4 * u);
+                if (i < 0 || more <= 0) continue;
+                if (WHOLE || more >= 4) {
                     if constexpr (sizeof(TO) == 4) {
-                        __builtin_memcpy(at, &O[it], 16);
+                        __builtin_memcpy(to, &O[it], 16);
                     } else {
-                        const uint2 w = make_uint2(pack_bf16x2(O[it][0], O[it][1]), pack_bf16x2(O[it][2], O[it][3]));
-                        __builtin_memcpy(at, &w, 8);
+                        // hidden from the compiler, which else carries all tiles through wide vectors (168 registers and 496 bytes spilled
+                        // for 143 and none)
+                        float x[4] = {O[it][0], O[it][1], O[it][2], O[it][3]};
+                        asm("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+                        const uint2 w = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+                        __builtin_memcpy(to, &w, 8);
                     }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 3; ++e)
-                        if (e < left) Storage<TO>::store(at + e, O[it][e]);
+                        if (e < more) Storage<TO>::store(to + e, O[it][e]);
                 }
             }
         }
-        // the state after the chunk
+        // The state after the chunk: the chunk's part is summed by itself, so that the state is rounded once a chunk.
         if (p.ends || t + C < end) {
-            // the chunk's part is summed by itself, so that the state is rounded once a chunk
-            const Decay decay(g, (float)valid);
+            const Decay decay(g, (float)(C - shift));
             Split<T, 3> v[KB];
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int j = 32 * k + 8 * u + e;
-                    x[e] = j < valid ? value(c[k], e) * (p.cs * power(l2, valid - j - p.e0)) : 0.0f;
-                }
+                for (int e = 0; e < 8; ++e) x[e] = value(c[k], e) * left[8 * k + e];
                 v[k] = Split<T, 3>(x);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 f32x4 s = {0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < KB; ++k) {
-                    const Frag<T> a = col_frag<TileM::kStride>(tb + (32 * k + 8 * u) * TileM::kStride + 16 * mt + r);
+                    const Frag<T> a = col_frag<TileM::kStride>(col_b + 32 * k * TileM::kStride + 16 * mt);
 #pragma unroll
                     for (int q = 0; q < v[k].kParts; ++q) s = mma(s, a, v[k].p[q]);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[mt][e] = decay(S[mt][e], s[e]);
+                if (mt % 2) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        first = false;
     }
-    if (p.ends) {
+    if (p.ends && col < p.n) {
+        float* const to = p.ends + state_at + col_in;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = 16 * mt + 4 * u + e;
-                if (row < p.m && col < p.n) p.ends[state_at + (int64_t)row * p.sm + (int64_t)col * p.sn] = S[mt][e];
+                if (row < p.m) to[row * p.sm] = S[mt][e];
             }
     }
     if constexpr (OUT) {  // rows behind a sequence's length
-        const int64_t from = t0 > end ? t0 : end;
-        TO* const po = (TO*)p.out + b * p.L * p.ldo + (int64_t)h * p.n + n0;
-        for (int64_t i = threadIdx.x; i < (t1 - from) * cols; i += THREADS)
-            Storage<TO>::store(po + (from + i / cols) * p.ldo + i % cols, 0.0f);
+        const int64_t behind = t0 > end ? t0 : end;
+        const int cols = p.n - n0 < 16 * NW ? p.n - n0 : 16 * NW;
+        TO* const to = (TO*)p.out + b * p.L * p.ldo + (int64_t)h * p.n + n0;
+        for (int64_t i = threadIdx.x; i < (t1 - behind) * cols; i += THREADS) Storage<TO>::store(to + (behind + i / cols) * p.ldo + i % cols, 0.0f);
     }
 }
 
@@ -470,14 +558,21 @@ __global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_
     float cur = init ? init[bh * state + i] : 0.0f;
     float* at = ends + bh * nseg * state + i;
     const Decay whole(g, (float)seglen);
-    for (int s = 0; s < nseg; ++s, at += state) {
-        const int64_t left = len - s * seglen;
-        const float e = *at;
-        *at = cur;
-        if (left >= seglen)
-            cur = whole(cur, e);
-        else if (left > 0)
-            cur = Decay(g, (float)left)(cur, e);
+    constexpr int kAhead = 8;  // segments whose states are on their way at once
+    for (int s0 = 0; s0 < nseg; s0 += kAhead, at += kAhead * state) {
+        float e[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) e[k] = s0 + k < nseg ? at[k * state] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (s0 + k >= nseg) break;
+            at[k * state] = cur;
+            const int64_t left = len - (s0 + k) * seglen;
+            if (left >= seglen)
+                cur = whole(cur, e[k]);
+            else if (left > 0)
+                cur = Decay(g, (float)left)(cur, e[k]);
+        }
     }
     if (last) last[bh * state + i] = cur;
 }
@@ -546,6 +641,7 @@ __global__ __launch_bounds__(256) void step_kernel(int64_t H, int dk, int dv, in
 
 // ------------------------------------------------------------------ host
 constexpr int kMaxChannels = 256;
+constexpr int64_t kMaxStride = 1 << 23;  // elements from one token to the next: a chunk's offsets take 32 bits
 int chunk_of(int dtype) { return dtype == HX_BF16 ? 64 : 32; }
 
 // Segments that a sequence is cut into where the (sequence, head) pairs leave compute units idle.
@@ -572,6 +668,7 @@ int check_shape(const char* what, const Shape& s) {
     if (s.H == 0) return HX_OK;
     HX_REQUIRE(s.hq > 0 && s.hk > 0 && s.hv > 0 && s.H % s.hq == 0 && s.H % s.hk == 0 && s.H % s.hv == 0, HX_ERR_SHAPE_MISMATCH,
                "%s: q, k and v need heads that divide %lld (%lld, %lld, %lld)", what, (long long)s.H, (long long)s.hq, (long long)s.hk, (long long)s.hv);
+    HX_REQUIRE(s.H * (s.dk > s.dv ? s.dk : s.dv) < kMaxStride, HX_ERR_UNSUPPORTED, "%s: tokens of fewer than 2^23 elements", what);
     HX_REQUIRE(s.dk > 0 && s.dv > 0, HX_ERR_INVALID_DIMENSION, "%s: a head without channels", what);
     HX_REQUIRE(s.dk <= kMaxChannels && s.dv <= kMaxChannels, HX_ERR_UNSUPPORTED, "%s: at most %d channels a head", what, kMaxChannels);
     HX_REQUIRE(s.B < (1 << 24) && s.H < (1 << 16) && s.B * s.H < (1 << 24) && s.L < ((int64_t)1 << 40) / (s.B > 0 ? s.B : 1), HX_ERR_UNSUPPORTED,
@@ -579,13 +676,13 @@ int check_shape(const char* what, const Shape& s) {
     return HX_OK;
 }
 
-template <typename T, int MP, int NW, bool OUT, typename TO>
+template <typename T, int MP, int NW, bool WHOLE, bool OUT, typename TO>
 int launch_mix_of(MixArgs& p, hipStream_t stream) {
     constexpr int C = sizeof(T) == 2 ? 64 : 32;
-    using TileM = Tile<T, C, MP, 64 * NW>;
-    using TileN = Tile<T, C, 16 * NW, 64 * NW>;
+    using TileM = Tile<T, C, MP, 64 * NW, WHOLE>;
+    using TileN = Tile<T, C, 16 * NW, 64 * NW, WHOLE>;
     constexpr size_t bytes = (OUT ? 2 : 1) * TileM::kBytes + TileN::kBytes + (OUT ? kPParts<T> * C * (C + 16 / sizeof(T)) * sizeof(T) : 0);
-    const auto k = mix_kernel<T, MP, C, NW, OUT, TO>;
+    const auto k = mix_kernel<T, MP, C, NW, WHOLE, OUT, TO>;
     HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 16), HX_ERR_BACKEND, "decay_attention: %zu bytes of LDS not granted", bytes);
     p.slices = (p.n + 16 * NW - 1) / (16 * NW);
     const int64_t blocks = p.B * p.H * p.nseg * p.slices;
@@ -594,16 +691,21 @@ int launch_mix_of(MixArgs& p, hipStream_t stream) {
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
+template <typename T, bool WHOLE, bool OUT, typename TO>
+int launch_mix_as(MixArgs& p, hipStream_t s) {
+    if (p.n > 64) {
+        if (p.m <= 64) return launch_mix_of<T, 64, 8, WHOLE, OUT, TO>(p, s);
+        if (p.m <= 128) return launch_mix_of<T, 128, 8, WHOLE, OUT, TO>(p, s);
+        return launch_mix_of<T, 256, 8, WHOLE, OUT, TO>(p, s);
+    }
+    if (p.m <= 64) return launch_mix_of<T, 64, 4, WHOLE, OUT, TO>(p, s);
+    if (p.m <= 128) return launch_mix_of<T, 128, 4, WHOLE, OUT, TO>(p, s);
+    return launch_mix_of<T, 256, 4, WHOLE, OUT, TO>(p, s);
+}
 template <typename T, bool OUT, typename TO>
 int launch_mix(MixArgs p, hipStream_t s) {
-    if (p.n > 64) {
-        if (p.m <= 64) return launch_mix_of<T, 64, 8, OUT, TO>(p, s);
-        if (p.m <= 128) return launch_mix_of<T, 128, 8, OUT, TO>(p, s);
-        return launch_mix_of<T, 256, 8, OUT, TO>(p, s);
-    }
-    if (p.m <= 64) return launch_mix_of<T, 64, 4, OUT, TO>(p, s);
-    if (p.m <= 128) return launch_mix_of<T, 128, 4, OUT, TO>(p, s);
-    return launch_mix_of<T, 256, 4, OUT, TO>(p, s);
+    constexpr int E = 16 / sizeof(T);
+    return p.m % E == 0 && p.n % E == 0 ? launch_mix_as<T, true, OUT, TO>(p, s) : launch_mix_as<T, false, OUT, TO>(p, s);
 }
 
 // One pass: the segments' states and their chain where there is more than one, then the outputs. `init` and `last`: the states
@@ -665,6 +767,7 @@ extern "C" int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t hea
     if (rc != HX_OK || batch == 0 || heads == 0) return rc;
     HX_REQUIRE(log_decay && (seqlen == 0 || (out && q && k && v)), HX_ERR_INVALID_INPUT, "decay_attention_fwd: NULL pointer");
     HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_fwd: a stride is shorter than a token");
+    HX_REQUIRE(ldq < kMaxStride && ldk < kMaxStride && ldv < kMaxStride, HX_ERR_UNSUPPORTED, "decay_attention_fwd: strides below 2^23 elements");
     int64_t seglen;
     const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen);
     const size_t need = hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype);
@@ -708,6 +811,7 @@ extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t hea
     if (rc != HX_OK || batch == 0 || heads == 0) return rc;
     HX_REQUIRE(log_decay && (seqlen == 0 || (q && k && v && dout && dq && dk_out && dv_out)), HX_ERR_INVALID_INPUT, "decay_attention_bwd: NULL pointer");
     HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_bwd: a stride is shorter than a token");
+    HX_REQUIRE(ldq < kMaxStride && ldk < kMaxStride && ldv < kMaxStride, HX_ERR_UNSUPPORTED, "decay_attention_bwd: strides below 2^23 elements");
     const size_t need = hx_decay_attention_bwd_workspace_size(batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv, dtype);
     HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), HX_ERR_INVALID_INPUT,
                "decay_attention_bwd: workspace of %zu bytes (16-byte aligned) required", need);
@@ -757,6 +861,7 @@ extern "C" int hx_decay_attention_step(int64_t batch, int64_t heads, int64_t q_h
     if (rc != HX_OK || batch == 0 || heads == 0) return rc;
     HX_REQUIRE(log_decay && out && state && q && k && v, HX_ERR_INVALID_INPUT, "decay_attention_step: NULL pointer");
     HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_step: a stride is shorter than a token");
+    HX_REQUIRE(ldq < kMaxStride && ldk < kMaxStride && ldv < kMaxStride, HX_ERR_UNSUPPORTED, "decay_attention_step: strides below 2^23 elements");
     const dim3 grid((unsigned)(batch * heads), (unsigned)((dv + 63) / 64));
     const int gq = (int)(heads / q_heads), gk = (int)(heads / k_heads), gv = (int)(heads / v_heads);
     if (dtype == HX_F32)
