@@ -26,16 +26,24 @@ struct MixArgs {
     int m, n, heads_out;  // channels of a and b, of c and the output
     const float* log_decay;
     const int32_t* lengths;
-    const float* entry;        // [B, H, segments or 1, dk dv]: the states before the first token (nullable: zero)
-    float* ends;               // the states after the last (nullable where there is an output)
-    int64_t state, segs;       // elements of a state, states of a (b, h) in entry and ends
+    const float* init;   // [B, H, dk, dv]: the states before the first token (nullable: zero)
+    float* last;         // the states after the last one (nullable)
+    float* parts;        // [B, H, segments, dk, dv]: what each segment gives from a zero state, or, chained, the states before segments
+    int chained;
+    int64_t state;       // elements of a state
     int sm, sn;                // a state's strides along m and n
     float ps, es, cs;
     int e0, back;
     void* out;
     int64_t ldo;
     int64_t seglen;  // tokens of a segment, whole chunks
-    int nseg, slices;
+    int nseg;
+};
+// Passes of one kind that go out as one launch, their blocks side by side: what they share they find in the L2.
+constexpr int kMaxPasses = 3;
+struct MixPasses {
+    MixArgs p[kMaxPasses];
+    int count, slices;
 };
 
 // w^x for x >= 0 as 2^(x l2); a decay of nothing (g = -inf) keeps w^0 = 1.
@@ -178,17 +186,6 @@ __device__ inline Frag<float> finite_only(Frag<float> f) {
     for (int e = 0; e < 8; ++e) f.v[e] = not_finite(f.v[e]) ? 0.0f : f.v[e];
     return f;
 }
-template <typename T>
-__device__ inline bool any_not_finite(const u32x4& w) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
-        if constexpr (sizeof(T) == 2) bad |= (w[i] & 0x7f80u) == 0x7f80u;
-    }
-    return bad;
-}
-
 // A row's elements from one of them on: 16 bytes moved down by `by` elements, zeros behind them.
 template <typename T>
 __device__ inline u32x4 moved(const u32x4& v, int by) {
@@ -226,23 +223,31 @@ struct Tile {
         col = want < most ? want : most;
         by = want - col;
     }
-    // Rows shift.. of the tile are tokens of a chunk, `valid` = ROWS - shift of them, the first (or, backwards, the last) at `first`.
+    __device__ void unit(int i, const T* at, uint32_t off) {
+        if (WHOLE || n >= E) {
+            __builtin_memcpy(&reg[i], at + off, 16);
+        } else {
+            T v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = at[off + (e < n ? e : n - 1)];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = e < n ? v[e] : 0;
+            __builtin_memcpy(&reg[i], v, 16);
+        }
+    }
+    // Rows shift.. of the tile are tokens of a chunk, ROWS - shift of them, the first (or, backwards, the last) at `first`.
     __device__ void load(const T* first, int64_t ld, int shift, bool back) {
-        const int valid = ROWS - shift;
+        if (shift == 0 && ROWS % kStep == 0) {  // one offset, and places that are the same for all threads
+            const uint32_t off = (uint32_t)((back ? kStep - 1 - row : row) * (int)ld + col);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            int k = row + i * kStep - shift;
-            k = k < 0 ? 0 : k >= valid ? valid - 1 : k;
-            const uint32_t off = (uint32_t)((back ? valid - 1 - k : k) * (int)ld + col);
-            if (WHOLE || n >= E) {
-                __builtin_memcpy(&reg[i], first + off, 16);
-            } else {
-                T v[E];
+            for (int i = 0; i < kEach; ++i) unit(i, first + (back ? kEach - 1 - i : i) * kStep * ld, off);
+        } else {
+            const int valid = ROWS - shift;
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = first[off + (e < n ? e : n - 1)];
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = e < n ? v[e] : 0;
-                __builtin_memcpy(&reg[i], v, 16);
+            for (int i = 0; i < kEach; ++i) {
+                int k = row + i * kStep - shift;
+                k = k < 0 ? 0 : k >= valid ? valid - 1 : k;
+                unit(i, first, (uint32_t)((back ? valid - 1 - k : k) * (int)ld + col));
             }
         }
     }
@@ -251,19 +256,35 @@ struct Tile {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) reg[i] = moved<T>(reg[i], by);
         }
+        if (shift) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (row + i * kStep < shift) reg[i] = u32x4{0, 0, 0, 0};
+        }
         if (!in) return;
         T* const to = tile + row * kStride + threadIdx.x % kPerRow * E;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const u32x4 v = row + i * kStep >= shift ? reg[i] : u32x4{0, 0, 0, 0};
-            if (ROWS % kStep == 0 || row + i * kStep < ROWS) *reinterpret_cast<u32x4*>(to + i * kStep * kStride) = v;
-        }
+        for (int i = 0; i < kEach; ++i)
+            if (ROWS % kStep == 0 || row + i * kStep < ROWS) *reinterpret_cast<u32x4*>(to + i * kStep * kStride) = reg[i];
     }
-    __device__ bool bad(int shift) const {
-        bool b = false;
+    // after store(): whether a value that was stored is not finite
+    __device__ bool bad() const {
+        if constexpr (sizeof(T) == 2) {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 most = {0, 0};  // of the exponents
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) b |= any_not_finite<T>(reg[i]) && row + i * kStep >= shift;
-        return b && in;
+            for (int i = 0; i < kEach; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, reg[i][k] & 0x7f807f80u));
+            return in && (most[0] == 0x7f80 || most[1] == 0x7f80);
+        } else {
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = max(most, reg[i][k] & 0x7f800000u);
+            return in && most == 0x7f800000u;
+        }
     }
 };
 
@@ -275,7 +296,7 @@ template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT 
 // a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state. A segment's last chunk that
 // is not whole stands at its tile's end, zeros before it, where its weights are a whole chunk's.
 template <typename T, int MP, int C, int NW, bool WHOLE, bool OUT, typename TO>
-__global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_kernel(const MixArgs p) {
+__global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_kernel(const MixPasses all) {
     constexpr int THREADS = 64 * NW, MT = MP / 16, NT = C / 16, KB = C / 32, E = 16 / sizeof(T);
     using TileM = Tile<T, C, MP, THREADS, WHOLE>;
     using TileN = Tile<T, C, 16 * NW, THREADS, WHOLE>;
@@ -289,27 +310,31 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, u = lane >> 4;
 
-    uint32_t id = blockIdx.x;
-    const int slice = (int)(id % (uint32_t)p.slices);
-    id /= (uint32_t)p.slices;
-    const int seg = (int)(id % (uint32_t)p.nseg);
-    id /= (uint32_t)p.nseg;
+    // Passes and slices of the same (sequence, head, segment) eight blocks apart, on one die; then the heads of the same tokens,
+    // whose rows are neighbours in memory.
+    const uint32_t inner = (uint32_t)(all.count * all.slices), tasks = gridDim.x / inner;
+    uint32_t id = blockIdx.x, which = id % inner;
+    if (tasks % 8 == 0) {
+        which = id / 8 % inner;
+        id = id / (8 * inner) * 8 + id % 8;
+    } else {
+        id /= inner;
+    }
+    const MixArgs& p = all.p[which / (uint32_t)all.slices];
+    const int slice = (int)(which % (uint32_t)all.slices);
     const int h = (int)(id % (uint32_t)p.H);
-    const int64_t b = id / (uint32_t)p.H;
+    id /= (uint32_t)p.H;
+    const int seg = (int)(id % (uint32_t)p.nseg);
+    const int64_t b = id / (uint32_t)p.nseg;
     int64_t len = p.L;
     if (p.lengths) {
         const int64_t given = p.lengths[b];
         len = given < 0 ? 0 : given < len ? given : len;
     }
-    const float g = p.log_decay[h], l2 = log2_decay(g);
     const int n0 = slice * 16 * NW;
     const int64_t t0 = seg * p.seglen, t1 = t0 + p.seglen < p.L ? t0 + p.seglen : p.L;
     const int64_t end = t1 < len ? t1 : len;
     const bool back = p.back != 0;
-
-    // columns behind a row's end stay zero, and so do score tiles above the diagonal
-    constexpr int kAll = (OUT ? 2 : 1) * TileM::kBytes + TileN::kBytes + (OUT ? kPParts<T> * C * PS * (int)sizeof(T) : 0);
-    for (int i = threadIdx.x; i < kAll / 16; i += THREADS) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
 
     // token t of the pass is token len - 1 - t of the sequence where it goes backwards
     TileM ra, rb;
@@ -329,26 +354,66 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
     };
     if (t0 < end) load(t0);
 
+    // Columns behind a row's end stay zero, and so do the score tiles above the diagonal that a product over 32 tokens meets.
+    if (!WHOLE || p.m < MP || p.n - n0 < 16 * NW) {
+        constexpr int kTiles = (OUT ? 2 : 1) * TileM::kBytes + TileN::kBytes;
+        for (int i = threadIdx.x; i < kTiles / 16; i += THREADS) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    }
+    if constexpr (OUT) {
+        for (int i = threadIdx.x; i < kPParts<T> * (NT / 2) * 256; i += THREADS) {
+            const int row = i / 16 % 16, t = i / 256 % (NT / 2) * 32, part = i / (NT / 2 * 256);
+            tp[part * C * PS + (t + row) * PS + t + 16 + i % 16] = 0;
+        }
+    }
+    const float g = p.log_decay[h], l2 = log2_decay(g);
+
     // S[mt]: rows 16 mt + 4u..+3 of the state's column n0 + 16 wave + r
-    const int64_t state_at = ((b * p.H + h) * p.segs + seg) * p.state;
+    const int64_t state_at = (b * p.H + h) * p.state;
     const int col = n0 + 16 * wave + r, col_in = (col < p.n ? col : p.n - 1) * p.sn;
     f32x4 S[MT];
+    const auto each = [&](const float* from, const auto& take) {  // a state's part of this lane, 16 rows at a time
+        from += col_in;
+        const bool down = p.sm == 1 && p.m % 4 == 0;  // rows are neighbours
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            f32x4 x;
+            const int row = 16 * mt + 4 * u;
+            if (down) {
+                __builtin_memcpy(&x, from + (row < p.m ? row : p.m - 4), 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = from[(row + e < p.m ? row + e : p.m - 1) * p.sm];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = row + e < p.m && col < p.n ? x[e] : 0.0f;
+            take(mt, x);
+        }
+    };
+    const float* const first = !OUT ? nullptr : p.chained ? p.parts + state_at * p.nseg + seg * p.state : p.init ? p.init + state_at : nullptr;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) S[mt] = f32x4{0, 0, 0, 0};
-    if (OUT && p.entry) {
-        const float* const from = p.entry + state_at + col_in;
+    if (first) each(first, [&](int mt, const f32x4& x) { S[mt] = x; });
+    if (OUT && !p.chained) {  // few segments: those before this one, in turn
+        const Decay whole(g, (float)p.seglen);
+#pragma unroll 1
+        for (int k = 0; k < seg; ++k) {
+            const int64_t there = len - k * p.seglen;
+            if (there <= 0) break;
+            const Decay decay = there >= p.seglen ? whole : Decay(g, (float)there);
+            each(p.parts + state_at * p.nseg + k * p.state, [&](int mt, const f32x4& x) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * mt + 4 * u + e;
-                const float v = from[(row < p.m ? row : p.m - 1) * p.sm];
-                S[mt][e] = row < p.m && col < p.n ? v : 0.0f;
-            }
+                for (int e = 0; e < 4; ++e) S[mt][e] = decay(S[mt][e], x[e]);
+            });
+        }
     }
+    float* const ends = !OUT ? p.parts + state_at * p.nseg + seg * p.state : seg == p.nseg - 1 && p.last ? p.last + state_at : nullptr;
 
-    // Weights of a lane's places: scores on and off the diagonal, tokens' part of the state.
-    float near[4], off[4], left[KB * 8];
+    // Weights of a lane's places: scores on and off the diagonal, tokens' part of the state, the state's part of outputs. The last
+    // and the state's decay are another chunk's only where that is not whole.
+    float near[4], off[4], left[KB * 8], entry[NT];
+    Decay decay(g, (float)C);
+#pragma unroll
+    for (int it = 0; it < NT; ++it) entry[it] = p.es * power(l2, 16 * it + r + p.e0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int d = r - 4 * u - e;
@@ -370,13 +435,21 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
 #pragma unroll 1
     for (int64_t t = t0; t < end; t += C, turn ^= 1) {
         const int shift = end - t < C ? (int)(C - (end - t)) : 0;
+        if (shift) {
+            decay = Decay(g, (float)(C - shift));
+#pragma unroll
+            for (int it = 0; it < NT; ++it) {
+                const int i = 16 * it + r - shift;
+                entry[it] = p.es * power(l2, (i < 0 ? 0 : i) + p.e0);
+            }
+        }
         lds_barrier();  // the last chunk's tiles are read
         if (threadIdx.x == 0) bad_rows[turn ^ 1] = 0;
         rb.store(tb, shift);
         rc.store(tc, shift);
         if constexpr (OUT) {
             ra.store(ta, shift);
-            if (rc.bad(shift)) bad_rows[turn] = 1;
+            if (rc.bad()) bad_rows[turn] = 1;
         }
         if (t + C < end) load(t + C);
         lds_barrier();
@@ -429,12 +502,9 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int it = 0; it < NT; ++it) {
-                const int i = 16 * it + r - shift;
-                const float w = p.es * power(l2, (i < 0 ? 0 : i) + p.e0);
+            for (int it = 0; it < NT; ++it)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) O[it][e] *= w;
-            }
+                for (int e = 0; e < 4; ++e) O[it][e] *= entry[it];
             lds_barrier();  // the scores are there
         }
         Frag<T> c[KB];
@@ -498,8 +568,7 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
             }
         }
         // The state after the chunk: the chunk's part is summed by itself, so that the state is rounded once a chunk.
-        if (p.ends || t + C < end) {
-            const Decay decay(g, (float)(C - shift));
+        if (ends || t + C < end) {
             Split<T, 3> v[KB];
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
@@ -524,8 +593,8 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
             }
         }
     }
-    if (p.ends && col < p.n) {
-        float* const to = p.ends + state_at + col_in;
+    if (ends && col < p.n) {
+        float* const to = ends + col_in;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -542,10 +611,13 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
     }
 }
 
-// Segments' end states, each from a zero state, to the states before them, in place; the last one's state to `last`.
-__global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_t seglen, int nseg, int64_t state,
-                                                    const float* __restrict__ log_decay, const int32_t* __restrict__ lengths,
-                                                    const float* __restrict__ init, float* __restrict__ ends, float* __restrict__ last) {
+// Many segments' parts to the states before them, in place: of one or two passes.
+struct ChainArgs {
+    const float* init[2];
+    float* parts[2];
+};
+__global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_t seglen, int nseg, int64_t state, const float* __restrict__ log_decay,
+                                                    const int32_t* __restrict__ lengths, const ChainArgs passes) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= state) return;
     const int64_t bh = blockIdx.y, b = bh / H;
@@ -555,10 +627,11 @@ __global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_
         len = given < 0 ? 0 : given < L ? given : L;
     }
     const float g = log_decay[bh % H];
+    const float* const init = passes.init[blockIdx.z];
     float cur = init ? init[bh * state + i] : 0.0f;
-    float* at = ends + bh * nseg * state + i;
+    float* at = passes.parts[blockIdx.z] + bh * nseg * state + i;
     const Decay whole(g, (float)seglen);
-    constexpr int kAhead = 8;  // segments whose states are on their way at once
+    constexpr int kAhead = 8;  // segments whose parts are on their way at once
     for (int s0 = 0; s0 < nseg; s0 += kAhead, at += kAhead * state) {
         float e[kAhead];
 #pragma unroll
@@ -574,18 +647,26 @@ __global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_
                 cur = Decay(g, (float)left)(cur, e[k]);
         }
     }
-    if (last) last[bh * state + i] = cur;
 }
 
-// y[row][h][c] = sum over the heads of a group of x, in their order, rounded once
-template <typename T>
-__global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int heads, int group, int n, const float* __restrict__ x, T* __restrict__ y) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// y[row][h][c] = sum over the heads of a group of x, in their order, rounded once; V neighbouring columns a thread
+template <typename T, int V>
+__global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int group, int n, const float* __restrict__ x, T* __restrict__ y) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (i >= total) return;
-    const int64_t c = i % n, rh = i / n;
-    float s = 0.0f;
-    for (int k = 0; k < group; ++k) s += x[(rh * group + k) * n + c];
-    Storage<T>::store(y + i, s);
+    const int64_t rh = (uint64_t)i / (uint32_t)n;
+    const float* at = x + rh * (group - 1) * n + i;
+    Run<V, float> s = Run<V, float>::load(at);
+#pragma unroll 4
+    for (int k = 1; k < group; ++k) {
+        const Run<V, float> o = Run<V, float>::load(at + (int64_t)k * n);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s.v[e] += o.v[e];
+    }
+    Run<V, T> r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) Storage<T>::store(&r.v[e], s.v[e]);
+    r.store(y + i);
 }
 
 // ------------------------------------------------------------------ one token
@@ -644,17 +725,22 @@ constexpr int kMaxChannels = 256;
 constexpr int64_t kMaxStride = 1 << 23;  // elements from one token to the next: a chunk's offsets take 32 bits
 int chunk_of(int dtype) { return dtype == HX_BF16 ? 64 : 32; }
 
-// Segments that a sequence is cut into where the (sequence, head) pairs leave compute units idle.
-int64_t segments_of(int64_t B, int64_t L, int64_t H, int dtype, int64_t* seglen) {
-    const int64_t C = chunk_of(dtype), chunks = (L + C - 1) / C, pairs = B * H;
-    int64_t want = pairs > 0 ? 1024 / pairs : 1;
-    const int64_t most = chunks / 4;
+// Segments that a sequence is cut into where the (sequence, head) pairs leave compute units idle: as many blocks as are
+// resident at once, each of two chunks at least.
+int64_t segments_of(int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv, int dtype, bool backward, int64_t* seglen) {
+    const int64_t C = chunk_of(dtype), chunks = (L + C - 1) / C, pairs = B * H, wide = dk > dv ? dk : dv;
+    const int64_t target = wide > 64 ? 512 : dtype == HX_F32 ? 1024 : backward ? 512 : 768;
+    int64_t want = pairs > 0 ? target / pairs : 1;
+    const int64_t most = chunks / 2;
     if (want > most) want = most;
     if (want < 1) want = 1;
     const int64_t per = (chunks + want - 1) / want;
     *seglen = (per > 0 ? per : 1) * C;
     return chunks > 0 ? (chunks + per - 1) / per : 1;
 }
+// Up to this many, an output's block goes through the segments before it by itself (not where the last one's state takes the
+// first one's buffer, which another block may yet read).
+constexpr int kFewSegments = 8;
 
 struct Shape {
     int64_t B, L, H, hq, hk, hv, dk, dv;
@@ -677,70 +763,66 @@ int check_shape(const char* what, const Shape& s) {
 }
 
 template <typename T, int MP, int NW, bool WHOLE, bool OUT, typename TO>
-int launch_mix_of(MixArgs& p, hipStream_t stream) {
+int launch_mix_of(MixPasses& a, hipStream_t stream) {
     constexpr int C = sizeof(T) == 2 ? 64 : 32;
     using TileM = Tile<T, C, MP, 64 * NW, WHOLE>;
     using TileN = Tile<T, C, 16 * NW, 64 * NW, WHOLE>;
     constexpr size_t bytes = (OUT ? 2 : 1) * TileM::kBytes + TileN::kBytes + (OUT ? kPParts<T> * C * (C + 16 / sizeof(T)) * sizeof(T) : 0);
     const auto k = mix_kernel<T, MP, C, NW, WHOLE, OUT, TO>;
     HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 16), HX_ERR_BACKEND, "decay_attention: %zu bytes of LDS not granted", bytes);
-    p.slices = (p.n + 16 * NW - 1) / (16 * NW);
-    const int64_t blocks = p.B * p.H * p.nseg * p.slices;
+    const MixArgs& p = a.p[0];
+    a.slices = (p.n + 16 * NW - 1) / (16 * NW);
+    const int64_t blocks = p.B * p.H * p.nseg * a.slices * a.count;
     HX_REQUIRE(blocks < ((int64_t)1 << 32) / (64 * NW), HX_ERR_UNSUPPORTED, "decay_attention: too many blocks");
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * NW), bytes, stream, p);
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * NW), bytes, stream, a);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
 template <typename T, bool WHOLE, bool OUT, typename TO>
-int launch_mix_as(MixArgs& p, hipStream_t s) {
+int launch_mix_as(MixPasses& a, hipStream_t s) {
+    const MixArgs& p = a.p[0];
     if (p.n > 64) {
-        if (p.m <= 64) return launch_mix_of<T, 64, 8, WHOLE, OUT, TO>(p, s);
-        if (p.m <= 128) return launch_mix_of<T, 128, 8, WHOLE, OUT, TO>(p, s);
-        return launch_mix_of<T, 256, 8, WHOLE, OUT, TO>(p, s);
+        if (p.m <= 64) return launch_mix_of<T, 64, 8, WHOLE, OUT, TO>(a, s);
+        if (p.m <= 128) return launch_mix_of<T, 128, 8, WHOLE, OUT, TO>(a, s);
+        return launch_mix_of<T, 256, 8, WHOLE, OUT, TO>(a, s);
     }
-    if (p.m <= 64) return launch_mix_of<T, 64, 4, WHOLE, OUT, TO>(p, s);
-    if (p.m <= 128) return launch_mix_of<T, 128, 4, WHOLE, OUT, TO>(p, s);
-    return launch_mix_of<T, 256, 4, WHOLE, OUT, TO>(p, s);
+    if (p.m <= 64) return launch_mix_of<T, 64, 4, WHOLE, OUT, TO>(a, s);
+    if (p.m <= 128) return launch_mix_of<T, 128, 4, WHOLE, OUT, TO>(a, s);
+    return launch_mix_of<T, 256, 4, WHOLE, OUT, TO>(a, s);
 }
 template <typename T, bool OUT, typename TO>
-int launch_mix(MixArgs p, hipStream_t s) {
+int launch_mix(MixPasses& a, hipStream_t s) {
     constexpr int E = 16 / sizeof(T);
-    return p.m % E == 0 && p.n % E == 0 ? launch_mix_as<T, true, OUT, TO>(p, s) : launch_mix_as<T, false, OUT, TO>(p, s);
+    return a.p[0].m % E == 0 && a.p[0].n % E == 0 ? launch_mix_as<T, true, OUT, TO>(a, s) : launch_mix_as<T, false, OUT, TO>(a, s);
 }
 
-// One pass: the segments' states and their chain where there is more than one, then the outputs. `init` and `last`: the states
-// before and after all tokens (nullable).
-int mix(MixArgs p, int dtype, bool out_f32, const float* init, float* last, float* states, hipStream_t s) {
-    if (p.nseg > 1) {
-        MixArgs e = p;
-        e.entry = nullptr;
-        e.ends = states;
-        e.segs = p.nseg;
-        int rc = dtype == HX_F32 ? launch_mix<float, false, float>(e, s) : launch_mix<uint16_t, false, uint16_t>(e, s);
-        if (rc != HX_OK) return rc;
-        const dim3 grid((unsigned)((p.state + 255) / 256), (unsigned)(p.B * p.H));
-        HX_REQUIRE(p.B * p.H < 65536, HX_ERR_UNSUPPORTED, "decay_attention: batch * heads below 2^16 for segments");
-        hipLaunchKernelGGL(chain_kernel, grid, dim3(256), 0, s, p.H, p.L, p.seglen, p.nseg, p.state, p.log_decay, p.lengths, init, states, last);
-        HX_LAUNCH_CHECK();
-        p.entry = states;
-        p.ends = nullptr;
-        p.segs = p.nseg;
-    } else {
-        p.entry = init;
-        p.ends = last;
-        p.segs = 1;
-    }
-    if (dtype == HX_F32) return launch_mix<float, true, float>(p, s);
-    return out_f32 ? launch_mix<uint16_t, true, float>(p, s) : launch_mix<uint16_t, true, uint16_t>(p, s);
+// What the segments of one or two passes give (b c^T each), and, where there are many, the states before them.
+int segment_states(MixPasses a, int dtype, hipStream_t s) {
+    const int rc = dtype == HX_F32 ? launch_mix<float, false, float>(a, s) : launch_mix<uint16_t, false, uint16_t>(a, s);
+    if (rc != HX_OK || !a.p[0].chained) return rc;
+    const MixArgs& p = a.p[0];
+    HX_REQUIRE(p.B * p.H < 65536, HX_ERR_UNSUPPORTED, "decay_attention: batch * heads below 2^16 for segments");
+    ChainArgs c{};
+    for (int i = 0; i < a.count; ++i) c.init[i] = a.p[i].init, c.parts[i] = a.p[i].parts;
+    const dim3 grid((unsigned)((p.state + 255) / 256), (unsigned)(p.B * p.H), (unsigned)a.count);
+    hipLaunchKernelGGL(chain_kernel, grid, dim3(256), 0, s, p.H, p.L, p.seglen, p.nseg, p.state, p.log_decay, p.lengths, c);
+    HX_LAUNCH_CHECK();
+    return HX_OK;
+}
+
+// The outputs of passes that have their sizes in common.
+int outputs(MixPasses a, int dtype, bool out_f32, hipStream_t s) {
+    if (dtype == HX_F32) return launch_mix<float, true, float>(a, s);
+    return out_f32 ? launch_mix<uint16_t, true, float>(a, s) : launch_mix<uint16_t, true, uint16_t>(a, s);
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 template <typename T>
 int group_sum(int64_t rows, int64_t H, int64_t heads, int64_t n, const float* x, void* y, hipStream_t s) {
-    const int64_t total = rows * heads * n, blocks = (total + 255) / 256;
+    const int64_t total = rows * heads * n, each = n % 4 == 0 ? 4 : 1, blocks = (total / each + 255) / 256;
     HX_REQUIRE(blocks < ((int64_t)1 << 24), HX_ERR_UNSUPPORTED, "decay_attention: too many elements of shared heads");
-    hipLaunchKernelGGL(group_sum_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, total, (int)heads, (int)(H / heads), (int)n, x, (T*)y);
+    hipLaunchKernelGGL((each == 4 ? group_sum_kernel<T, 4> : group_sum_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, s, total, (int)(H / heads), (int)n, x, (T*)y);
     HX_LAUNCH_CHECK();
     return HX_OK;
 }
@@ -748,13 +830,17 @@ int group_sum(int64_t rows, int64_t H, int64_t heads, int64_t n, const float* x,
 }  // namespace
 }  // namespace hx
 
+// bytes of the segments' states of one direction (0 where no sequence is cut)
+static size_t hx_state_bytes(int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv, int dtype, bool backward) {
+    int64_t seglen;
+    const int64_t nseg = hx::segments_of(B, L, H, dk, dv, dtype, backward, &seglen);
+    return nseg > 1 ? hx::round16((size_t)(B * H * nseg * dk * dv * 4)) : 0;
+}
+
 extern "C" size_t hx_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv, int dtype) {
     using namespace hx;
     if (check_shape("decay_attention", {batch, seqlen, heads, heads, heads, heads, dk, dv, dtype}) != HX_OK) return 0;
-    if (batch == 0 || heads == 0) return 0;
-    int64_t seglen;
-    const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen);
-    return nseg > 1 ? (size_t)(batch * heads * nseg * dk * dv * 4) : 0;
+    return batch == 0 || heads == 0 ? 0 : hx_state_bytes(batch, seqlen, heads, dk, dv, dtype, false);
 }
 
 extern "C" int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads, int64_t k_heads, int64_t v_heads, int64_t dk,
@@ -769,22 +855,30 @@ extern "C" int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t hea
     HX_REQUIRE(ldq >= q_heads * dk && ldk >= k_heads * dk && ldv >= v_heads * dv, HX_ERR_INVALID_INPUT, "decay_attention_fwd: a stride is shorter than a token");
     HX_REQUIRE(ldq < kMaxStride && ldk < kMaxStride && ldv < kMaxStride, HX_ERR_UNSUPPORTED, "decay_attention_fwd: strides below 2^23 elements");
     int64_t seglen;
-    const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen);
-    const size_t need = hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype);
+    const int64_t nseg = segments_of(batch, seqlen, heads, dk, dv, dtype, false, &seglen);
+    const size_t need = hx_state_bytes(batch, seqlen, heads, dk, dv, dtype, false);
     HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), HX_ERR_INVALID_INPUT,
                "decay_attention_fwd: workspace of %zu bytes (16-byte aligned) required", need);
-    MixArgs p{};
+    MixPasses all{};
+    all.count = 1;
+    MixArgs& p = all.p[0];
     p.a = q, p.b = k, p.c = v;
     p.lda = ldq, p.ldb = ldk, p.ldc = ldv;
     p.ga = (int)(heads / q_heads), p.gb = (int)(heads / k_heads), p.gc = (int)(heads / v_heads);
     p.B = batch, p.L = seqlen, p.H = heads;
     p.m = (int)dk, p.n = (int)dv;
     p.log_decay = log_decay, p.lengths = lengths;
+    p.init = init_state, p.last = last_state, p.parts = (float*)workspace;
+    p.chained = nseg > kFewSegments || (nseg > 1 && last_state && last_state == init_state);
     p.state = dk * dv, p.sm = (int)dv, p.sn = 1;
     p.ps = p.es = scale, p.cs = 1.0f, p.e0 = 1, p.back = 0;
     p.out = out, p.ldo = heads * dv;
     p.seglen = seglen, p.nseg = (int)nseg;
-    return mix(p, dtype, false, init_state, last_state, (float*)workspace, as_stream(stream));
+    if (nseg > 1) {
+        rc = segment_states(all, dtype, as_stream(stream));
+        if (rc != HX_OK) return rc;
+    }
+    return outputs(all, dtype, false, as_stream(stream));
 }
 
 // bytes of the fp32 gradients of an operand that heads share
@@ -796,7 +890,7 @@ extern "C" size_t hx_decay_attention_bwd_workspace_size(int64_t batch, int64_t s
     if (check_shape("decay_attention_bwd", {batch, seqlen, heads, q_heads, k_heads, v_heads, dk, dv, dtype}) != HX_OK) return 0;
     if (batch == 0 || heads == 0) return 0;
     const int64_t rows = batch * seqlen;
-    return round16(hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype)) + hx_shared_bytes(rows, heads, q_heads, dk) +
+    return 2 * hx_state_bytes(batch, seqlen, heads, dk, dv, dtype, true) + hx_shared_bytes(rows, heads, q_heads, dk) +
            hx_shared_bytes(rows, heads, k_heads, dk) + hx_shared_bytes(rows, heads, v_heads, dv);
 }
 
@@ -817,39 +911,75 @@ extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t hea
                "decay_attention_bwd: workspace of %zu bytes (16-byte aligned) required", need);
     hipStream_t s = as_stream(stream);
     int64_t seglen;
-    const int64_t nseg = segments_of(batch, seqlen, heads, dtype, &seglen), rows = batch * seqlen;
+    const int64_t nseg = segments_of(batch, seqlen, heads, dk, dv, dtype, true, &seglen), rows = batch * seqlen;
+    const size_t state_bytes = hx_state_bytes(batch, seqlen, heads, dk, dv, dtype, true);
     char* at = (char*)workspace;
-    float* const states = (float*)at;
-    at += round16(hx_decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype));
-    MixArgs p{};
-    p.B = batch, p.L = seqlen, p.H = heads;
-    p.log_decay = log_decay, p.lengths = lengths;
-    p.state = dk * dv;
-    p.seglen = seglen, p.nseg = (int)nseg;
+    float *const before = (float*)at, *const behind = (float*)(at + state_bytes);  // states before segments, their adjoints behind
+    at += 2 * state_bytes;
     const int gq = (int)(heads / q_heads), gk = (int)(heads / k_heads), gv = (int)(heads / v_heads);
-    const int64_t ldo = heads * dv;
-    const auto pass = [&](const void* a, int64_t lda, int ga, const void* b, int64_t ldb, int gb, const void* c, int64_t ldc, int gc, bool transposed,
-                          bool back, const float* init, float* last, void* out, int64_t out_heads) -> int {
-        p.a = a, p.b = b, p.c = c, p.lda = lda, p.ldb = ldb, p.ldc = ldc, p.ga = ga, p.gb = gb, p.gc = gc;
-        const int64_t m = transposed ? dv : dk, n = transposed ? dk : dv;
-        p.m = (int)m, p.n = (int)n;
+    struct Operand {
+        const void* p;
+        int64_t ld;
+        int group;
+    };
+    const Operand Q{q, ldq, gq}, K{k, ldk, gk}, V{v, ldv, gv}, D{dout, heads * dv, 1};
+    const bool in_place = dinit && dinit == dlast, chained = nseg > kFewSegments || (nseg > 1 && in_place);
+    const auto mixing = [&](const Operand& a, const Operand& b, const Operand& c, bool transposed, bool back, float* last) {
+        MixArgs p{};
+        p.B = batch, p.L = seqlen, p.H = heads;
+        p.log_decay = log_decay, p.lengths = lengths;
+        p.init = back ? dlast : init_state, p.last = last, p.parts = back ? behind : before, p.chained = chained;
+        p.state = dk * dv;
+        p.seglen = seglen, p.nseg = (int)nseg;
+        p.a = a.p, p.b = b.p, p.c = c.p, p.lda = a.ld, p.ldb = b.ld, p.ldc = c.ld, p.ga = a.group, p.gb = b.group, p.gc = c.group;
+        p.m = (int)(transposed ? dv : dk), p.n = (int)(transposed ? dk : dv);
         p.sm = transposed ? 1 : (int)dv, p.sn = transposed ? (int)dv : 1;
         p.back = back, p.e0 = back ? 0 : 1;
         p.ps = scale, p.es = back ? 1.0f : scale, p.cs = back ? scale : 1.0f;
-        const bool shared = out_heads != heads;
-        float* wide = (float*)at;
-        if (shared) at += hx_shared_bytes(rows, heads, out_heads, n);
-        p.out = shared ? wide : out;
-        p.ldo = heads * n;
-        int rc = mix(p, dtype, shared, init, last, states, s);
-        if (rc == HX_OK && shared && rows > 0)
-            rc = dtype == HX_F32 ? group_sum<float>(rows, heads, out_heads, n, wide, out, s) : group_sum<uint16_t>(rows, heads, out_heads, n, wide, out, s);
-        return rc;
+        return p;
     };
-    rc = pass(dout, ldo, 1, v, ldv, gv, k, ldk, gk, true, false, init_state, nullptr, dq, q_heads);
-    if (rc == HX_OK) rc = pass(v, ldv, gv, dout, ldo, 1, q, ldq, gq, true, true, dlast, nullptr, dk_out, k_heads);
-    if (rc == HX_OK) rc = pass(k, ldk, gk, q, ldq, gq, dout, ldo, 1, false, true, dlast, dinit, dv_out, v_heads);
-    return rc;
+    if (nseg > 1) {
+        MixPasses both{};
+        both.count = 2;
+        both.p[0] = mixing(Q, K, V, false, false, nullptr);
+        both.p[1] = mixing(K, Q, D, false, true, nullptr);
+        rc = segment_states(both, dtype, s);
+        if (rc != HX_OK) return rc;
+    }
+    // dq, dk and dv as they are to be, or in 32 bits and head by head where heads share an operand. Passes with the same sizes
+    // and type go out together; where dinit's buffer is dlast's, the pass that writes it goes last.
+    struct Gradient {
+        MixArgs p;
+        void* out;
+        int64_t heads;
+    };
+    Gradient grads[3] = {{mixing(D, V, K, true, false, nullptr), dq, q_heads}, {mixing(V, D, Q, true, true, nullptr), dk_out, k_heads},
+                         {mixing(K, Q, D, false, true, dinit), dv_out, v_heads}};
+    bool wide[3];
+    for (int i = 0; i < 3; ++i) {
+        Gradient& x = grads[i];
+        wide[i] = x.heads != heads;
+        x.p.out = wide[i] ? (void*)at : x.out;
+        x.p.ldo = heads * x.p.n;
+        if (wide[i]) at += hx_shared_bytes(rows, heads, x.heads, x.p.n);
+    }
+    for (int i = 0; i < 3;) {
+        MixPasses all{};
+        int j = i;
+        for (; j < 3 && grads[j].p.m == grads[i].p.m && grads[j].p.n == grads[i].p.n && wide[j] == wide[i] && !(j == 2 && j > i && in_place); ++j)
+            all.p[all.count++] = grads[j].p;
+        rc = outputs(all, dtype, wide[i], s);
+        if (rc != HX_OK) return rc;
+        i = j;
+    }
+    for (int i = 0; i < 3 && rows > 0; ++i)
+        if (wide[i]) {
+            const int64_t n = grads[i].p.n;
+            rc = dtype == HX_F32 ? group_sum<float>(rows, heads, grads[i].heads, n, (const float*)grads[i].p.out, grads[i].out, s)
+                                 : group_sum<uint16_t>(rows, heads, grads[i].heads, n, (const float*)grads[i].p.out, grads[i].out, s);
+            if (rc != HX_OK) return rc;
+        }
+    return HX_OK;
 }
 
 extern "C" int hx_decay_attention_step(int64_t batch, int64_t heads, int64_t q_heads, int64_t k_heads, int64_t v_heads, int64_t dk, int64_t dv,
