@@ -19,63 +19,110 @@ struct NormArgs {
     float* scales;
 };
 
-// With r = x + delta as it is stored and p = r w (exact in 64 bits: two numbers of 24), a row is p / rms(r). In 8 bits its codes
-// are round(127 p / max |p|), whatever the norm, and its scale is max |p| / (127 rms). All of it is formed in 64 bits: the
-// codes are those of the definition, not of one order of summing, and the rate (half of fp32's) leaves memory the bound.
+// With r = x + delta as it is stored and p = r w, a row is p / rms(r). In 8 bits its codes are round(127 p / max |p|), whatever the
+// norm, and its scale is max |p| / (127 rms). The squares are summed in 64 bits, and the codes are those of the definition, not of
+// one order of rounding: 127 p / max |p| in 32 bits is off by less than 4e-5 steps, so what lies further than 1e-4 from a border
+// is decided by it, and the rest (one element in five thousand) by the exact products, which 64 bits hold (two numbers of 24).
+// The largest of the exact products is sought among the elements that are the largest in 32 bits. Rows whose products leave 32
+// bits' range take 64 throughout. 32768 x 2048 fp32 with a bf16 delta: 64 bits for every element and a wave a row 207 us,
+// a block of four waves a row, 2 x 4 elements a lane (58 registers for 145), 153 (4.8 TB/s).
 struct RowSums {
     double squares;
-    uint64_t top;  // the largest |p|: the bits of numbers without a sign order as they do, with NaN above all
-    __device__ void add(double r, double p) {
-        squares = fma(r, r, squares);
-        const uint64_t bits = (uint64_t)__double_as_longlong(fabs(p));
+    uint32_t top;  // the largest |p| in 32 bits: the bits of numbers without a sign order as they do, with NaN above all
+    __device__ void add(float r, float w) {
+        squares = fma((double)r, (double)r, squares);
+        const uint32_t bits = __float_as_uint(r * w) & 0x7fffffffu;
         top = bits > top ? bits : top;
     }
     __device__ void join(const RowSums& o) {
         squares += o.squares;
         top = o.top > top ? o.top : top;
     }
+    __device__ bool common() const { return top >= 0x0d800000u && top < 0x71800000u; }  // 2^-100 and 2^100
 };
 
-__device__ inline RowSums over_wave(RowSums s) {
+// over the THREADS of a row, the same in all of them
+template <int THREADS>
+__device__ inline RowSums over_row(RowSums v, RowSums* part) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        RowSums o;
-        o.squares = __shfl_xor(s.squares, off, 64);
-        o.top = (uint64_t)__shfl_xor((unsigned long long)s.top, off, 64);
-        s.join(o);
+    for (int off = 32; off > 0; off >>= 1) v.join({__shfl_xor(v.squares, off, 64), (uint32_t)__shfl_xor((int)v.top, off, 64)});
+    if constexpr (THREADS > 64) {
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / 64; ++i) v.join(part[i]);
     }
-    return s;
+    return v;
+}
+// |p| in 64 bits, as the integer that orders as it does
+__device__ inline unsigned long long exact_bits(float r, float w) { return (unsigned long long)__double_as_longlong(fabs((double)r * (double)w)); }
+// Where one of four elements is the row's largest in 32 bits (or all are to be looked at), the largest of their exact products.
+__device__ inline void find_top(const float (&r)[4], const float (&w)[4], const RowSums& s, unsigned long long* top) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t bits = __float_as_uint(r[e] * w[e]) & 0x7fffffffu;
+        most = bits > most ? bits : most;
+    }
+    if (most == s.top || !s.common()) {
+        unsigned long long v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned long long bits = exact_bits(r[e], w[e]);
+            v = bits > v ? bits : v;
+        }
+        atomicMax(top, v);  // whichever order they come in
+    }
+}
+__device__ inline double inverse_rms(const RowSums& s, const NormArgs& p) {
+    return p.weight ? 1.0 / sqrt(s.squares / (double)p.dim + (double)p.eps) : 1.0;
 }
 
 enum Kind { kF32 = HX_F32, kBf16 = HX_BF16, kI8 = HX_I8 };
 
-// What a row's elements are multiplied with, and its scale.
+// What four elements become. For codes: the largest |p| exactly and 127 over it in 32 bits (0 where that does not serve).
 struct RowFactor {
-    double m, top;
-    float scale;
-    bool bad;
-    template <int KIND>
-    static __device__ RowFactor of(const RowSums& s, const NormArgs& p) {
+    double top, inv;
+    float m32;
+    bool zero, fast;
+    __device__ static RowFactor of_codes(const RowSums& s, unsigned long long top) {
         RowFactor f;
-        const double inv = p.weight ? 1.0 / sqrt(s.squares / (double)p.dim + (double)p.eps) : 1.0;
-        f.top = __longlong_as_double((long long)s.top);
-        f.bad = s.top >= 0x7ff0000000000000ull || !(inv <= 1.7e308);
-        if constexpr (KIND == kI8) {
-            f.m = f.bad || f.top == 0.0 ? 0.0 : 127.0 / f.top;
-            f.scale = f.bad ? __uint_as_float(0x7fc00000u) : (float)(f.top * inv / 127.0);
-        } else {
-            f.m = inv;
-        }
+        f.top = __longlong_as_double((long long)top);
+        f.zero = top == 0 || top >= 0x7ff0000000000000ull;
+        f.fast = s.common();
+        f.m32 = 127.0f / __uint_as_float(s.top);
+        f.inv = 0.0;
         return f;
     }
-    __device__ int code(double p) const {
-        if (bad) return 0;
-        const double t = p * m;
-        double q = rint(t);
-        if (fabs(fabs(t - q) - 0.5) < 1e-9) q = rint(p * 127.0 / top);  // a tie of p itself, not of the rounded factor's
-        return (int)q;
+    __device__ static RowFactor of_values(const RowSums& s, const NormArgs& p) {
+        RowFactor f{};
+        f.inv = inverse_rms(s, p);
+        f.m32 = (float)f.inv;
+        f.fast = s.common();
+        return f;
+    }
+    __device__ uint32_t codes(const float (&r)[4], const float (&w)[4]) const {
+        int q[4];
+        bool border = !fast;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float t = r[e] * w[e] * m32, whole = rintf(t);
+            border |= fabsf(t - whole) > 0.4999f;
+            q[e] = (int)whole;
+        }
+        if (border) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = zero ? 0 : (int)rint((double)r[e] * (double)w[e] * 127.0 / top);
+        }
+        return (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)q[3] << 24;
     }
 };
+// a row's scale; NaN where it holds what is not finite (a NaN among the products is above all numbers in `top`)
+__device__ inline float scale_of(const RowSums& s, unsigned long long top, const NormArgs& p) {
+    const double inv = inverse_rms(s, p);
+    return top >= 0x7ff0000000000000ull || !(inv <= 1.7e308) ? __uint_as_float(0x7fc00000u) : (float)(__longlong_as_double((long long)top) * inv / 127.0);
+}
 
 template <int N, typename T>
 __device__ inline void load_run(const T* at, int64_t left, float (&v)[N]) {
@@ -132,15 +179,15 @@ template <int KIND>
 __device__ inline void store_y(const NormArgs& p, const RowFactor& f, int64_t row, int64_t c, const float (&r)[4], const float (&w)[4]) {
     const int64_t at = row * p.ldy + c, left = p.dim - c;
     if constexpr (KIND == kI8) {
-        int8_t q[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = (int8_t)f.code((double)r[e] * (double)w[e]);
-        store_run<4>((int8_t*)p.y + at, left, q);
+        const uint32_t q = f.codes(r, w);
+        int8_t v[4];
+        __builtin_memcpy(v, &q, 4);
+        store_run<4>((int8_t*)p.y + at, left, v);
     } else {
         using T = std::conditional_t<KIND == kF32, float, uint16_t>;
         T v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = as_stored<T>((float)((double)r[e] * (double)w[e] * f.m));
+        for (int e = 0; e < 4; ++e) v[e] = as_stored<T>(KIND == kBf16 && f.fast ? r[e] * w[e] * f.m32 : (float)((double)r[e] * (double)w[e] * f.inv));
         store_run<4>((T*)p.y + at, left, v);
     }
 }
@@ -148,7 +195,7 @@ __device__ inline void store_y(const NormArgs& p, const RowFactor& f, int64_t ro
 // A row in the registers of THREADS threads, 4 NV elements each: read once, written once.
 template <typename TX, int KIND, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_kernel(const NormArgs p) {
-    constexpr int kBlock = THREADS < 256 ? 256 : THREADS, kWaves = THREADS / 64;
+    constexpr int kBlock = THREADS < 256 ? 256 : THREADS;
     const int64_t row = (int64_t)blockIdx.x * (kBlock / THREADS) + threadIdx.x / THREADS;
     const int at = threadIdx.x % THREADS;
     if (THREADS == 64 && row >= p.rows) return;
@@ -169,24 +216,38 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_kernel(cons
         const int64_t c = (int64_t)(i * THREADS + at) * 4;
         if (p.resid) store_sum<TX>(p, row, c, r[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s.add(r[i][e], (double)r[i][e] * (double)w[i][e]);
+        for (int e = 0; e < 4; ++e) s.add(r[i][e], w[i][e]);
     }
-    s = over_wave(s);
-    if constexpr (kWaves > 1) {
-        __shared__ RowSums part[kWaves];
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
-        __syncthreads();
-        s = part[0];
+    __shared__ RowSums sums[kBlock / 64];
+    __shared__ unsigned long long tops[kBlock / THREADS];
+    unsigned long long* const top = tops + threadIdx.x / THREADS;
+    if (at == 0) *top = 0;
+    s = over_row<THREADS>(s, sums);
+    if constexpr (KIND == kI8) {
+        const auto meet = [] {  // of a row's threads
+            if constexpr (THREADS > 64) {
+                __syncthreads();
+            } else {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
+                __builtin_amdgcn_wave_barrier();
+            }
+        };
+        meet();
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i) s.join(part[i]);
+        for (int i = 0; i < NV; ++i) find_top(r[i], w[i], s, top);
+        meet();
+        const RowFactor f = RowFactor::of_codes(s, *top);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store_y<KIND>(p, f, row, (int64_t)(i * THREADS + at) * 4, r[i], w[i]);
+        if (at == 0) p.scales[row] = scale_of(s, *top, p);
+    } else {
+        const RowFactor f = RowFactor::of_values(s, p);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store_y<KIND>(p, f, row, (int64_t)(i * THREADS + at) * 4, r[i], w[i]);
     }
-    const RowFactor f = RowFactor::of<KIND>(s, p);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) store_y<KIND>(p, f, row, (int64_t)(i * THREADS + at) * 4, r[i], w[i]);
-    if (KIND == kI8 && at == 0) p.scales[row] = f.scale;
 }
 
-// Rows of any width: two passes, the second from what the first stored where it stored anything.
+// Rows of any width: passes over the row, the later ones from what the first stored where it stored anything.
 template <typename TX, int KIND>
 __global__ __launch_bounds__(1024) void wide_row_kernel(const NormArgs p) {
     const int64_t row = blockIdx.x;
@@ -204,26 +265,34 @@ __global__ __launch_bounds__(1024) void wide_row_kernel(const NormArgs p) {
         weights(c, w);
         if (p.resid) store_sum<TX>(p, row, c, r);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s.add(r[e], (double)r[e] * (double)w[e]);
+        for (int e = 0; e < 4; ++e) s.add(r[e], w[e]);
     }
-    s = over_wave(s);
-    __shared__ RowSums part[16];
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
-    __syncthreads();
-    s = part[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) s.join(part[i]);
-    const RowFactor f = RowFactor::of<KIND>(s, p);
-    for (int64_t c = threadIdx.x * 4; c < p.dim; c += 4096) {
-        float r[4], w[4];
+    __shared__ RowSums sums[16];
+    __shared__ unsigned long long top;
+    if (threadIdx.x == 0) top = 0;
+    s = over_row<1024>(s, sums);
+    const auto again = [&](int64_t c, float (&r)[4], float (&w)[4]) {
         if (p.resid)
             load_run<4>((const TX*)p.resid + row * p.ldr + c, p.dim - c, r);
         else
             load_sum<TX>(p, row, c, r);
         weights(c, w);
+    };
+    if constexpr (KIND == kI8) {
+        for (int64_t c = threadIdx.x * 4; c < p.dim; c += 4096) {
+            float r[4], w[4];
+            again(c, r, w);
+            find_top(r, w, s, &top);
+        }
+        __syncthreads();
+    }
+    const RowFactor f = KIND == kI8 ? RowFactor::of_codes(s, top) : RowFactor::of_values(s, p);
+    for (int64_t c = threadIdx.x * 4; c < p.dim; c += 4096) {
+        float r[4], w[4];
+        again(c, r, w);
         store_y<KIND>(p, f, row, c, r, w);
     }
-    if (KIND == kI8 && threadIdx.x == 0) p.scales[row] = f.scale;
+    if (KIND == kI8 && threadIdx.x == 0) p.scales[row] = scale_of(s, top, p);
 }
 
 template <typename TX, int KIND>
@@ -232,13 +301,13 @@ int launch_rows(const NormArgs& p, hipStream_t s) {
     if (p.dim <= 512)
         hipLaunchKernelGGL((row_kernel<TX, KIND, 64, 2>), four, dim3(256), 0, s, p);
     else if (p.dim <= 1024)
-        hipLaunchKernelGGL((row_kernel<TX, KIND, 64, 4>), four, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((row_kernel<TX, KIND, 256, 1>), one, dim3(256), 0, s, p);
     else if (p.dim <= 2048)
-        hipLaunchKernelGGL((row_kernel<TX, KIND, 64, 8>), four, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((row_kernel<TX, KIND, 256, 2>), one, dim3(256), 0, s, p);
     else if (p.dim <= 4096)
         hipLaunchKernelGGL((row_kernel<TX, KIND, 256, 4>), one, dim3(256), 0, s, p);
     else if (p.dim <= 8192)
-        hipLaunchKernelGGL((row_kernel<TX, KIND, 256, 8>), one, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((row_kernel<TX, KIND, 1024, 2>), one, dim3(1024), 0, s, p);
     else if (p.dim <= 16384)
         hipLaunchKernelGGL((row_kernel<TX, KIND, 1024, 4>), one, dim3(1024), 0, s, p);
     else
@@ -266,8 +335,8 @@ extern "C" int hx_add_rmsnorm(int64_t rows, int64_t dim, int dtype, const void* 
     HX_REQUIRE(x && y && (out_dtype != HX_I8 || scales), HX_ERR_INVALID_INPUT, "add_rmsnorm: NULL pointer");
     HX_REQUIRE(ldx >= dim && ldy >= dim && (!delta || ldd >= dim) && (!resid || ldr >= dim), HX_ERR_INVALID_INPUT,
                "add_rmsnorm: a stride is shorter than a row");
-    HX_REQUIRE(rows < (1 << 22) || (dim <= 2048 && rows < (1 << 24)), HX_ERR_UNSUPPORTED,
-               "add_rmsnorm: fewer than 2^24 rows of up to 2048 elements, 2^22 of more");
+    HX_REQUIRE(rows < (1 << 22) || (dim <= 4096 && rows < (1 << 24)), HX_ERR_UNSUPPORTED,
+               "add_rmsnorm: fewer than 2^24 rows of up to 4096 elements, 2^22 of more");
     const NormArgs p{rows, dim, x, delta, ldx, ldd, delta ? delta_dtype : -1, weight, eps, resid, ldr, y, ldy, scales};
     return dtype == HX_F32 ? launch_kind<float>(p, out_dtype, as_stream(stream)) : launch_kind<uint16_t>(p, out_dtype, as_stream(stream));
 }

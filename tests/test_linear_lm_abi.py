@@ -81,7 +81,7 @@ def test_norm_refusals():
     assert norm(rows=0) == 0 and norm(dim=0) == 0
     assert norm(x=None) == INPUT and norm(y=None) == INPUT and norm(scales=None) == INPUT
     assert norm(ldx=7) == INPUT and norm(ldy=7) == INPUT and norm(delta=P, ldd=7) == INPUT and norm(resid=P, ldr=7) == INPUT
-    assert norm(rows=1 << 40) == UNSUPPORTED and norm(rows=1 << 23, dim=4096, ldx=4096, ldy=4096) == UNSUPPORTED
+    assert norm(rows=1 << 40) == UNSUPPORTED and norm(rows=1 << 23, dim=4100, ldx=4100, ldy=4100) == UNSUPPORTED
 
 
 def linear(M=2, N=8, K=8, X=P, ldx=8, sx=P, packed=P, scales=P, bias=None, act=0, out_dtype=0, Y=P, ldy=8):
