@@ -66,7 +66,14 @@ __device__ inline void store_outputs(const I8Args& p, TO* to, int64_t left, floa
             else
                 w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
         }
-        __builtin_memcpy(to, w, sizeof(w));
+        if constexpr (sizeof(w) == 16) {  // outputs stream out past what the other tiles still read
+            typedef uint32_t anywhere __attribute__((ext_vector_type(4), aligned(2)));
+            anywhere v4;
+            __builtin_memcpy(&v4, w, 16);
+            __builtin_nontemporal_store(v4, (anywhere*)to);
+        } else {
+            __builtin_memcpy(to, w, sizeof(w));
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -325,19 +332,30 @@ __global__ __launch_bounds__(256) void linear_i8_tiles_kernel(const I8Args p, co
                 acc[t / TN][t % TN] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[t / TN], b[t % TN], acc[t / TN][t % TN], 0, 0, 0);
         }
     }
-    __syncthreads();  // the ring's memory is free
-    // slabs of 32 rows by 64 outputs through LDS rows of the wave's own, and out as rows
+    // Slabs of 32 rows by 64 outputs through LDS rows of the wave's own, and out as rows. The scales are all asked for ahead: with
+    // few waves to a SIMD a load between slabs is waited for in full (256 wide, 8191 x 8192 x 2048: 193 -> 175 us).
     constexpr int E = 16 / sizeof(TO), kLanes = 64 / E, kRows = 64 / kLanes;  // elements a lane, lanes a row, rows at a time
     int* const st = (int*)lds + wave * (32 * 68);
     const int c = lane % kLanes * E;
+    float sx[TM][32 / kRows];
 #pragma unroll
-    for (int jj = 0; jj < TN / 2; ++jj) {
-        const int64_t n = n0 + wn * 32 * TN + 64 * jj + c;
-        Finish fin[E];
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) fin[e] = Finish::of(p, n + e);
+        for (int h = 0; h < 32 / kRows; ++h) {
+            const int64_t m = m0 + wm * 32 * TM + 32 * i + h * kRows + lane / kLanes;
+            sx[i][h] = p.sx[m < p.M ? m : p.M - 1];
+        }
+    Finish fin[TN / 2][E];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
+    for (int jj = 0; jj < TN / 2; ++jj)
+#pragma unroll
+        for (int e = 0; e < E; ++e) fin[jj][e] = Finish::of(p, n0 + wn * 32 * TN + 64 * jj + c + e);
+    __syncthreads();  // the ring's memory is free
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int jj = 0; jj < TN / 2; ++jj) {
+            const int64_t n = n0 + wn * 32 * TN + 64 * jj + c;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -349,9 +367,8 @@ __global__ __launch_bounds__(256) void linear_i8_tiles_kernel(const I8Args p, co
                 const int row = h * kRows + lane / kLanes;
                 const int64_t m = m0 + wm * 32 * TM + 32 * i + row;
                 float v[E];
-                const float sx = p.sx[m < p.M ? m : p.M - 1];
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = fin[e](p, st[row * 68 + c + e], sx);
+                for (int e = 0; e < E; ++e) v[e] = fin[jj][e](p, st[row * 68 + c + e], sx[i][h]);
                 if (m < p.M && n < p.N) store_outputs<E>(p, (TO*)p.Y + m * p.ldy + n, p.N - n, v);
             }
             __builtin_amdgcn_wave_barrier();
@@ -390,13 +407,21 @@ int launch_tiles(const I8Args& p, hipStream_t s) {
 template <typename TO>
 int launch_i8(const I8Args& p, hipStream_t s) {
     const auto tiles = [&](int64_t side) { return ((p.M + side - 1) / side) * ((p.N + side - 1) / side); };
-    if (aligned(p.X, 16) && p.ldx % 16 == 0 && p.ldx < (1 << 22) && tiles(256) < (1 << 23)) {
-        if (tiles(256) >= 256) return launch_tiles<4, TO>(p, s);
-        if (p.M > 128 && tiles(128) >= 256) return launch_tiles<2, TO>(p, s);
+    // Many rows: tiles of 128 where there are enough for half the chip, two blocks to a CU, so that one's outputs are written while the
+    // other multiplies; tiles of 256 from K 4096 on. 128 and 256 wide, in us: 8192 x 8192 x 2048 177 and 178, x 4096 361 and
+    // 306, 4096 x 4096 x 8192 143 and 118, 13479 x 13976 x 272 to fp32 286 and 357. Tiles of 128 and few rows' kernel: 1024 x 2048 x
+    // 2048 14.6 and 15.7 (128 tiles), 512 x 2048 x 2048 14.1 and 10.5 (64 tiles).
+    if (aligned(p.X, 16) && p.ldx % 16 == 0 && p.ldx < (1 << 22) && tiles(128) < (1 << 23)) {
+        if (p.K >= 4096 && tiles(256) >= 256) return launch_tiles<4, TO>(p, s);
+        if (p.M > 128 && tiles(128) >= 128) return launch_tiles<2, TO>(p, s);
     }
-    if (p.M <= 16) return launch_rows<1, 1, TO>(p, s);
-    if (p.M <= 32) return launch_rows<1, 2, TO>(p, s);
-    if (p.M <= 64) return launch_rows<1, 4, TO>(p, s);
+    // Few rows, a block's outputs by rows: 16 x 16 where blocks are wanting, 32 x 32, 32 x 64 where there are more of them than are
+    // resident. 16 x 16, 32 x 32 and 32 x 64: 48 x 2048 x 8192 9.4, 8.5 and 12.0; 32 x 2048 x 8192 6.8, 8.1 and 11.8; 48 x 8192 x
+    // 2048 8.1, 7.4 and 8.1; 256 x 1024 x 8192 13.9, 9.5 and 12.3; 1024 x 2048 x 2048 23.8, 15.7 and 18.0; 4096 x 4096 x 8192 597,
+    // 320 and 267.
+    const int64_t outs = (p.N + 15) / 16;
+    if (p.M <= 16 || (p.M <= 32 && outs <= 128)) return launch_rows<1, 1, TO>(p, s);
+    if (outs * ((p.M + 63) / 64) < 4096) return launch_rows<2, 2, TO>(p, s);
     return launch_rows<2, 4, TO>(p, s);
 }
 
