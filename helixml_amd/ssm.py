@@ -323,19 +323,21 @@ def gated_state_update(state, x, f, z=None, out=None, stream=None):
 
 
 def _tokens(launch, t, name, shape, dtype):
-    """Checks a [batch, seqlen, heads, channels] operand whose tokens may be strided (a slice of a projection's output); the
-    elements from one token to the next."""
+    """Checks a [batch, seqlen, heads, channels] operand (one token: without seqlen) whose tokens may be strided, as a slice of a
+    projection's output is; the elements from one token to the next."""
+    heads, n = shape[-2:]
+    if t.shape == shape and t.dtype == dtype and t.device == launch.device and t.is_contiguous():
+        return heads * n
     if not t.is_cuda:
         raise InvalidInput(f"{name} must be a device tensor")
     if t.shape != shape:
         raise ShapeMismatch(f"{name}: expected {list(shape)}, got {list(t.shape)}")
     if t.dtype != dtype:
         raise DTypeMismatch(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.device != launch.device:
-        _on_stream_device(launch, **{name: t})
-    if t.is_contiguous():
-        return shape[2] * shape[3]
-    bt, L, heads, n = shape
+    _on_stream_device(launch, **{name: t})
+    if len(shape) == 3:
+        t = t.unsqueeze(1)
+    bt, L = t.shape[:2]
     sb, st, sh, sn = t.stride()
     ld = st if L > 1 else sb if bt > 1 else heads * n  # an axis of one has no stride: torch may report any
     if (n > 1 and sn != 1) or (heads > 1 and sh != n) or ld < heads * n or (bt > 1 and sb != L * ld):
@@ -344,24 +346,21 @@ def _tokens(launch, t, name, shape, dtype):
 
 
 def _decay_heads(launch, q, k, v, log_decay, dims):
-    """Checks what every form of the attention takes: (batch, seqlen or 1, heads, q_heads, k_heads, v_heads, dk, dv), the
-    storage type's code and the three token strides."""
-    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
-        raise ShapeMismatch(f"q, k, v: expected {dims} dims, got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
-    if log_decay.dim() != 1:
-        raise ShapeMismatch(f"log_decay: expected [heads], got {list(log_decay.shape)}")
+    """Checks what every form of the attention takes: the leading sizes (batch, and seqlen but for one token), (heads, q_heads,
+    k_heads, v_heads, dk, dv), the storage type's code and the three token strides."""
+    qs, ks, vs, gs = q.shape, k.shape, v.shape, log_decay.shape
+    if len(qs) != dims or len(ks) != dims or len(vs) != dims:
+        raise ShapeMismatch(f"q, k, v: expected {dims} dims, got {list(qs)}, {list(ks)}, {list(vs)}")
+    if len(gs) != 1:
+        raise ShapeMismatch(f"log_decay: expected [heads], got {list(gs)}")
     st = q.dtype
     if st not in _STORAGE:
         raise DTypeMismatch(f"q: storage dtype {st} is neither float32 nor bfloat16")
-    if dims == 3:  # one token of every sequence
-        q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
-    bt, L, hq, dk = q.shape
-    hk, (hv, dv) = k.shape[2], v.shape[2:]
-    heads = log_decay.shape[0]
-    _operands(launch, ("log_decay", log_decay, (heads,), torch.float32))
-    ld = (_tokens(launch, q, "q", (bt, L, hq, dk), st), _tokens(launch, k, "k", (bt, L, hk, dk), st),
-          _tokens(launch, v, "v", (bt, L, hv, dv), st))
-    return (bt, L, heads, hq, hk, hv, dk, dv), _STORAGE[st], ld
+    *lead, hq, dk = qs
+    lead, hk, (hv, dv) = tuple(lead), ks[-2], vs[-2:]
+    _operands(launch, ("log_decay", log_decay, gs, torch.float32))
+    ld = (_tokens(launch, q, "q", qs, st), _tokens(launch, k, "k", (*lead, hk, dk), st), _tokens(launch, v, "v", (*lead, hv, dv), st))
+    return lead, (gs[0], hq, hk, hv, dk, dv), _STORAGE[st], ld
 
 
 def _scratch(name, given, device, *sizes):
@@ -383,8 +382,8 @@ def decay_attention_fwd(q, k, v, log_decay, scale=1.0, lengths=None, init_state=
     init_state: [batch, heads, dk, dv] fp32. Returns out [batch, L, heads, dv], followed by the last state where asked for.
     Nothing is recorded for autograd: decay_attention_bwd gives the gradients. ``workspace``: a uint8 device
     tensor of at least decay_attention_workspace_size(...) bytes; allocated here when not given."""
-    sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 4)
-    bt, L, heads, hq, hk, hv, dk, dv = sizes
+    (bt, L), sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 4)
+    heads, hq, hk, hv, dk, dv = sizes
     f32, state = torch.float32, (bt, heads, dk, dv)
     _operands(stream, ("lengths", lengths, (bt,), torch.int32), ("init_state", init_state, state, f32), ("out", out, (bt, L, heads, dv), q.dtype))
     if workspace is not None:
@@ -393,7 +392,7 @@ def decay_attention_fwd(q, k, v, log_decay, scale=1.0, lengths=None, init_state=
         out = torch.empty((bt, L, heads, dv), device=q.device, dtype=q.dtype)
     last = torch.empty(state, device=q.device, dtype=f32) if return_last_state else None
     workspace, nbytes = _scratch("hx_decay_attention_workspace_size", workspace, q.device, bt, L, heads, dk, dv, code)
-    _ffi.call("hx_decay_attention_fwd", *sizes, code, _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay), float(scale),
+    _ffi.call("hx_decay_attention_fwd", bt, L, *sizes, code, _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay), float(scale),
               _ptr(lengths), _ptr(init_state), _ptr(out), _ptr(last), _ptr(workspace), nbytes, _stream(stream))
     return (out, last) if return_last_state else out
 
@@ -403,8 +402,8 @@ def decay_attention_bwd(q, k, v, log_decay, dout, scale=1.0, lengths=None, init_
     """Gradients of decay_attention_fwd (hx_decay_attention_bwd): (dq, dk, dv, dinit) from dout [batch, L, heads, dv] and dlast
     [batch, heads, dk, dv] fp32 (the last state's gradient; None: zero). The other arguments are the forward's. dq, dk, dv
     have q's type and the operands' shapes (a shared head's is the sum over its group), dinit is fp32."""
-    sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 4)
-    bt, L, heads, hq, hk, hv, dk, dv = sizes
+    (bt, L), sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 4)
+    heads, hq, hk, hv, dk, dv = sizes
     f32, state = torch.float32, (bt, heads, dk, dv)
     _operands(stream, ("lengths", lengths, (bt,), torch.int32), ("init_state", init_state, state, f32), ("dlast", dlast, state, f32),
               ("dout", dout, (bt, L, heads, dv), q.dtype))
@@ -412,8 +411,8 @@ def decay_attention_bwd(q, k, v, log_decay, dout, scale=1.0, lengths=None, init_
         _on_stream_device(stream, workspace=workspace)
     dq, dkeys, dvalues = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
     dinit = torch.empty(state, device=q.device, dtype=f32)
-    workspace, nbytes = _scratch("hx_decay_attention_bwd_workspace_size", workspace, q.device, *sizes, code)
-    _ffi.call("hx_decay_attention_bwd", *sizes, code, _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay), float(scale),
+    workspace, nbytes = _scratch("hx_decay_attention_bwd_workspace_size", workspace, q.device, bt, L, *sizes, code)
+    _ffi.call("hx_decay_attention_bwd", bt, L, *sizes, code, _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay), float(scale),
               _ptr(lengths), _ptr(init_state), _ptr(dout), _ptr(dlast), _ptr(dq), _ptr(dkeys), _ptr(dvalues), _ptr(dinit),
               _ptr(workspace), nbytes, _stream(stream))
     return dq, dkeys, dvalues, dinit
@@ -432,12 +431,13 @@ def decay_attention_workspace_size(batch, seqlen, heads, dk, dv, dtype=torch.flo
 def decay_attention_step(state, q, k, v, log_decay, scale=1.0, out=None, stream=None):
     """One token of that attention for every sequence (hx_decay_attention_step); advances ``state`` [batch, heads, dk, dv] fp32 in
     place. q: [batch, q_heads, dk], k: [batch, k_heads, dk], v: [batch, v_heads, dv] (rows may be strided); out [batch, heads, dv]."""
-    (bt, _, heads, hq, hk, hv, dk, dv), code, ld = _decay_heads(stream, q, k, v, log_decay, 3)
+    (bt,), sizes, code, ld = _decay_heads(stream, q, k, v, log_decay, 3)
+    heads, _, _, _, dk, dv = sizes
     _operands(stream, ("state", state, (bt, heads, dk, dv), torch.float32), ("out", out, (bt, heads, dv), q.dtype))
     if out is None:
-        out = torch.empty((bt, heads, dv), device=q.device, dtype=q.dtype)
-    _ffi.call("hx_decay_attention_step", bt, heads, hq, hk, hv, dk, dv, code, _ptr(state), _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2],
-              _ptr(log_decay), float(scale), _ptr(out), _stream(stream))
+        out = torch.empty((bt, heads, dv), device=stream.device, dtype=q.dtype)
+    _ffi.call("hx_decay_attention_step", bt, *sizes, code, _ptr(state), _ptr(q), ld[0], _ptr(k), ld[1], _ptr(v), ld[2], _ptr(log_decay),
+              float(scale), _ptr(out), _stream(stream))
     return out
 
 

@@ -132,7 +132,7 @@ def test_quantize_refusals():
 
 
 class Launch:
-    device = torch.device("cpu")
+    device = torch.device("cuda:0")
     cuda_stream = 0
 
 
