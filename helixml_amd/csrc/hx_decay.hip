@@ -290,7 +290,7 @@ struct Tile {
 
 template <typename T> constexpr int kPParts = sizeof(T) == 2 ? 2 : 1;
 // waves to a SIMD that a kernel's LDS leaves room for, as its register bound
-template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT ? (MP > 128 ? 2 : 3) : MP > 128 ? (NW == 8 ? 2 : 1) : NW == 8 ? 2 : MP > 64 ? 2 : 3;
+template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT ? (MP > 128 ? 2 : 3) : MP > 128 ? (NW == 8 ? 2 : 1) : NW == 8 ? 2 : MP > 64 ? 2 : sizeof(T) == 4 ? 4 : 3;
 
 // One segment of one (sequence, head) through NW waves, 16 columns of the output to each; MP >= m channels of a and b, C tokens
 // a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state. A segment's last chunk that
@@ -310,20 +310,18 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, u = lane >> 4;
 
-    // Passes and slices of the same (sequence, head, segment) eight blocks apart, on one die; then the heads of the same tokens,
-    // whose rows are neighbours in memory.
-    const uint32_t inner = (uint32_t)(all.count * all.slices), tasks = gridDim.x / inner;
-    uint32_t id = blockIdx.x, which = id % inner;
-    if (tasks % 8 == 0) {
-        which = id / 8 % inner;
-        id = id / (8 * inner) * 8 + id % 8;
-    } else {
-        id /= inner;
-    }
+    // Consecutive blocks go to different dies. A die takes all heads of its segments, whose rows are neighbours in memory (a head's own
+    // rows stand a whole token apart, which meets few of an L2's channels: 1 x 65536 x 16 x 64 fp32 343 -> 315 us), and passes and
+    // slices of a head one after the other.
+    const uint32_t inner = (uint32_t)(all.count * all.slices), heads = (uint32_t)all.p[0].H, groups = gridDim.x / (inner * heads);
+    const uint32_t dies = groups % 8 == 0 ? 8 : groups % 4 == 0 ? 4 : groups % 2 == 0 ? 2 : 1, die = blockIdx.x % dies;
+    uint32_t id = blockIdx.x / dies;
+    const uint32_t which = id % inner;
+    id /= inner;
     const MixArgs& p = all.p[which / (uint32_t)all.slices];
     const int slice = (int)(which % (uint32_t)all.slices);
-    const int h = (int)(id % (uint32_t)p.H);
-    id /= (uint32_t)p.H;
+    const int h = (int)(id % heads);
+    id = id / heads * dies + die;
     const int seg = (int)(id % (uint32_t)p.nseg);
     const int64_t b = id / (uint32_t)p.nseg;
     int64_t len = p.L;
@@ -736,7 +734,8 @@ int64_t segments_of(int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv, int
     if (want < 1) want = 1;
     const int64_t per = (chunks + want - 1) / want;
     *seglen = (per > 0 ? per : 1) * C;
-    return chunks > 0 ? (chunks + per - 1) / per : 1;
+    const int64_t nseg = chunks > 0 ? (chunks + per - 1) / per : 1;
+    return nseg >= 8 ? (nseg + 7) / 8 * 8 : nseg;  // whole rounds of dies, the last ones perhaps without tokens
 }
 // Up to this many, an output's block goes through the segments before it by itself (not where the last one's state takes the
 // first one's buffer, which another block may yet read).
