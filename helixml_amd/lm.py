@@ -8,7 +8,8 @@ that model, pre-norm with a residual stream:
     x = embed[tokens]                                    (fp32 residual stream)
     for each layer: x += MambaBlock(RMSNorm(x))          (hx_mamba_layer_fwd / _decode)
     logits = RMSNorm_f(x) . W_head^T                     (hx_rmsnorm_fwd + hx_gemm_bf16, or
-                                                          hx_linear_w4 after quantize_head)
+                                                          hx_linear_w4, or hx_add_rmsnorm + hx_linear_i8,
+                                                          after quantize_head)
     what a decode step does to them before a token is chosen       (hx_logits_adjust)
 
 ``prefill`` runs whole sequences and returns the per-layer decode state (the scan's last state
@@ -23,8 +24,8 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _ffi
-from .ssm import (_STORAGE, _on_stream_device, _operands, _ptr, _stream, keep_for_stream,
-                  linear_w4, on_current_or_launch_stream, on_launch_stream, w4_quantize, w4_values)
+from .ssm import (_STORAGE, _on_stream_device, _operands, _ptr, _stream, i8_quantize, i8_values, keep_for_stream,
+                  linear_i8, linear_w4, on_current_or_launch_stream, on_launch_stream, w4_quantize, w4_values)
 
 _F32, _BF16 = _ffi.HX_F32, _ffi.HX_BF16
 
@@ -218,28 +219,52 @@ class ByteLM:
             ))
         self.norm_f = torch.ones(dm, dtype=f32, device=self.device)
         self.w_head = lin(vocab, dm)
-        self._head4 = None
+        self._rounded = None  # (bits, pair, the weights it is of, their version)
         self._ws: Optional[torch.Tensor] = None
 
     # ------------------------------------------------------------------ helpers
-    def quantize_head(self):
-        """Rounds the head's weights to 4 bits with group scales (ssm.w4_quantize): from then on prefill and decode
-        alike read them through hx_linear_w4, whose rows do not depend on how many there are. The model goes back to
-        w_head itself once that is assigned or written to (writes through ``.data`` are not seen): the 4-bit form is of
-        what it held before, and is made again by another call. ``w_head4 = None`` does the same by hand."""
-        self.w_head4 = w4_quantize(self.w_head)
+    def quantize_head(self, bits=4):
+        """Rounds the head's weights to 4 bits with group scales (ssm.w4_quantize), or to 8 with a scale a vocabulary entry
+        (ssm.i8_quantize): from then on prefill and decode alike read them through hx_linear_w4, or hx_linear_i8 on the last norm's
+        output in 8 bits, whose rows do not depend on how many there are. The model goes back to w_head itself once that is
+        assigned or written to (writes through ``.data`` are not seen): the rounded form is of what it held before, and is made
+        again by another call. ``w_head4 = None`` (``w_head8 = None``) does the same by hand."""
+        if bits == 4:
+            self.w_head4 = w4_quantize(self.w_head)
+        elif bits == 8:
+            self.w_head8 = i8_quantize(self.w_head)
+        else:
+            raise _ffi.InvalidInput(f"quantize_head: {bits} bits, 4 or 8 are there")
+
+    def _rounded_head(self, bits):
+        if self._rounded is None or self._rounded[0] != bits:
+            return None
+        _, pair, of, version = self._rounded
+        return pair if of is self.w_head and version == _version(of) else None
+
+    def _round_head(self, bits, pair):
+        if pair is not None:
+            self._rounded = (bits, pair, self.w_head, _version(self.w_head))
+        elif self._rounded is not None and self._rounded[0] == bits:
+            self._rounded = None
 
     @property
     def w_head4(self):
-        """The 4-bit head (packed, scales), None where there is none of what w_head holds now."""
-        if self._head4 is None:
-            return None
-        pair, of, version = self._head4
-        return pair if of is self.w_head and version == _version(of) else None
+        """The 4-bit head (packed, scales), None where there is none of what w_head holds now. One rounded form is kept at a time."""
+        return self._rounded_head(4)
 
     @w_head4.setter
     def w_head4(self, pair):
-        self._head4 = None if pair is None else (pair, self.w_head, _version(self.w_head))
+        self._round_head(4, pair)
+
+    @property
+    def w_head8(self):
+        """The 8-bit head (packed, scales), as w_head4."""
+        return self._rounded_head(8)
+
+    @w_head8.setter
+    def w_head8(self, pair):
+        self._round_head(8, pair)
 
     def _workspace(self, batch, seqlen):
         need = int(_ffi.lib().hx_mamba_layer_workspace_size(batch, seqlen, self.d_model, self.d_inner,
@@ -256,6 +281,12 @@ class ByteLM:
 
     def _head(self, x, stream):
         rows = x.numel() // self.d_model
+        head8 = self.w_head8
+        if head8 is not None:
+            codes, scales = add_rmsnorm(x.view(rows, self.d_model), self.norm_f, eps=self.eps, stream=stream)
+            logits = torch.empty((*x.shape[:-1], self.vocab), device=self.device, dtype=torch.float32)
+            linear_i8(codes, scales, *head8, out=logits.view(rows, self.vocab), stream=stream)
+            return logits
         xn = rmsnorm(x, self.norm_f, self.eps, out_dtype=torch.bfloat16, stream=stream)
         logits = torch.empty((*x.shape[:-1], self.vocab), device=self.device, dtype=torch.float32)
         head4 = self.w_head4
@@ -348,15 +379,17 @@ class ByteLM:
         # the captured launches hold these tensors' addresses: they live as long as the step, whatever becomes of
         # the caller's dict and of the model
         step.adjust = adjust
-        step.head = self.w_head4
+        step.head = self.w_head4 or self.w_head8
         step.weights = (self.embed, self.norm_f, self.w_head, [dict(p) for p in self.layers])
         return step
 
     def host_params(self):
         """Every parameter as float32 numpy arrays (for the CPU oracle in tests); w_head is the head that the
-        logits come from, so the 4-bit form's values where there is one."""
+        logits come from, so a rounded form's values where there is one (an 8-bit head also takes the last norm's output
+        in 8 bits)."""
         f = lambda t: t.float().cpu().numpy()  # noqa: E731
-        head4 = self.w_head4
-        head = f(self.w_head) if head4 is None else w4_values(*head4, self.d_model)
+        head4, head8 = self.w_head4, self.w_head8
+        head = (w4_values(*head4, self.d_model) if head4 is not None else i8_values(*head8, self.d_model) if head8 is not None
+                else f(self.w_head))
         return dict(embed=f(self.embed), norm_f=f(self.norm_f), w_head=head,
                     layers=[{k: f(v) for k, v in p.items()} for p in self.layers])
