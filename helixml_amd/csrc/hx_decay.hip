@@ -650,21 +650,21 @@ __global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_
 // y[row][h][c] = sum over the heads of a group of x, in their order, rounded once; V neighbouring columns a thread
 template <typename T, int V>
 __global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int group, int n, const float* __restrict__ x, T* __restrict__ y) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
-    if (i >= total) return;
-    const int64_t rh = (uint64_t)i / (uint32_t)n;
-    const float* at = x + rh * (group - 1) * n + i;
-    Run<V, float> s = Run<V, float>::load(at);
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < total; i += (int64_t)gridDim.x * 256 * V) {
+        const int64_t rh = (uint64_t)i / (uint32_t)n;
+        const float* at = x + rh * (group - 1) * n + i;
+        Run<V, float> s = Run<V, float>::load(at);
 #pragma unroll 4
-    for (int k = 1; k < group; ++k) {
-        const Run<V, float> o = Run<V, float>::load(at + (int64_t)k * n);
+        for (int k = 1; k < group; ++k) {
+            const Run<V, float> o = Run<V, float>::load(at + (int64_t)k * n);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s.v[e] += o.v[e];
+            for (int e = 0; e < V; ++e) s.v[e] += o.v[e];
+        }
+        Run<V, T> r;
+#pragma unroll
+        for (int e = 0; e < V; ++e) Storage<T>::store(&r.v[e], s.v[e]);
+        r.store(y + i);
     }
-    Run<V, T> r;
-#pragma unroll
-    for (int e = 0; e < V; ++e) Storage<T>::store(&r.v[e], s.v[e]);
-    r.store(y + i);
 }
 
 // ------------------------------------------------------------------ one token
@@ -819,8 +819,8 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 template <typename T>
 int group_sum(int64_t rows, int64_t H, int64_t heads, int64_t n, const float* x, void* y, hipStream_t s) {
-    const int64_t total = rows * heads * n, each = n % 4 == 0 ? 4 : 1, blocks = (total / each + 255) / 256;
-    HX_REQUIRE(blocks < ((int64_t)1 << 24), HX_ERR_UNSUPPORTED, "decay_attention: too many elements of shared heads");
+    const int64_t total = rows * heads * n, each = n % 4 == 0 ? 4 : 1, most = (int64_t)1 << 23, want = (total / each + 255) / 256;
+    const int64_t blocks = want < most ? want : most;
     hipLaunchKernelGGL((each == 4 ? group_sum_kernel<T, 4> : group_sum_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, s, total, (int)(H / heads), (int)n, x, (T*)y);
     HX_LAUNCH_CHECK();
     return HX_OK;
@@ -922,7 +922,7 @@ extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t hea
         int group;
     };
     const Operand Q{q, ldq, gq}, K{k, ldk, gk}, V{v, ldv, gv}, D{dout, heads * dv, 1};
-    const bool in_place = dinit && dinit == dlast, chained = nseg > kFewSegments || (nseg > 1 && in_place);
+    const bool in_place = dinit && (dinit == dlast || dinit == init_state), chained = nseg > kFewSegments || (nseg > 1 && in_place);
     const auto mixing = [&](const Operand& a, const Operand& b, const Operand& c, bool transposed, bool back, float* last) {
         MixArgs p{};
         p.B = batch, p.L = seqlen, p.H = heads;
@@ -946,7 +946,7 @@ extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t hea
         if (rc != HX_OK) return rc;
     }
     // dq, dk and dv as they are to be, or in 32 bits and head by head where heads share an operand. Passes with the same sizes
-    // and type go out together; where dinit's buffer is dlast's, the pass that writes it goes last.
+    // and type go out together; where dinit's buffer is dlast's or init_state's, the pass that writes it goes last.
     struct Gradient {
         MixArgs p;
         void* out;

@@ -242,6 +242,23 @@ def test_carried_in_place(dev, dtype):
         assert torch.equal(t, want[n]), n
 
 
+@pytest.mark.parametrize("L", [40, 700], ids=["one segment", "segments"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_gradient_in_the_states_place(dev, dtype, L):
+    """dinit may take init_state's buffer, which dq's pass reads."""
+    x = inputs(3, L, 2, 160, 160, seed=9, dtype=dtype)
+    want, d = run(dev, x), on(dev, x)
+    code, ld = ssm._STORAGE[dtype], 2 * 160
+    nbytes = ssm.decay_attention_workspace_size(3, L, 2, 160, 160, dtype, backward=True)
+    ws = torch.empty(max(nbytes, 1), device=dev, dtype=torch.uint8)
+    state, g = d["init"].clone(), [torch.empty_like(d[n]) for n in ("q", "k", "v")]
+    _ffi.call("hx_decay_attention_bwd", 3, L, 2, 2, 2, 2, 160, 160, code, d["q"].data_ptr(), ld, d["k"].data_ptr(), ld, d["v"].data_ptr(), ld,
+              d["log_decay"].data_ptr(), float(x["scale"]), None, state.data_ptr(), d["dout"].data_ptr(), d["dlast"].data_ptr(),
+              *(t.data_ptr() for t in g), state.data_ptr(), ws.data_ptr(), nbytes, None)
+    for t, n in zip((*g, state), ("dq", "dk", "dv", "dinit")):
+        assert torch.equal(t, want[n]), n
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_pieces_and_tokens_agree(dev, dtype):
     """A sequence in pieces of any length, each from the last one's state, and token by token: the whole sequence's result."""
