@@ -335,6 +335,8 @@ extern "C" int hx_add_rmsnorm(int64_t rows, int64_t dim, int dtype, const void* 
     HX_REQUIRE(x && y && (out_dtype != HX_I8 || scales), HX_ERR_INVALID_INPUT, "add_rmsnorm: NULL pointer");
     HX_REQUIRE(ldx >= dim && ldy >= dim && (!delta || ldd >= dim) && (!resid || ldr >= dim), HX_ERR_INVALID_INPUT,
                "add_rmsnorm: a stride is shorter than a row");
+    HX_REQUIRE(!resid || ((resid != x || ldr == ldx) && (resid != delta || (delta_dtype == dtype && ldr == ldd))), HX_ERR_INVALID_INPUT,
+               "add_rmsnorm: resid in the place of x or delta needs its type and stride");
     HX_REQUIRE(rows < (1 << 22) || (dim <= 4096 && rows < (1 << 24)), HX_ERR_UNSUPPORTED,
                "add_rmsnorm: fewer than 2^24 rows of up to 4096 elements, 2^22 of more");
     const NormArgs p{rows, dim, x, delta, ldx, ldd, delta ? delta_dtype : -1, weight, eps, resid, ldr, y, ldy, scales};

@@ -213,7 +213,8 @@ int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, c
  * Tokens are taken in chunks through the matrix cores with fp32 sums (bf16 operands that are not stored
  * as bf16 are split into two or three bf16 parts), the same bits on every call; an infinite value may
  * become NaN, but nothing reaches the tokens before it. dk and dv 1..256, batch * heads < 2^24, heads <
- * 2^16, batch * seqlen < 2^40. workspace: hx_decay_attention_workspace_size(...) bytes of device memory
+ * 2^16, batch * seqlen < 2^40, ldq, ldk, ldv and heads * max(dk, dv) < 2^23 (else HX_ERR_UNSUPPORTED). No
+ * buffer that is written may overlap another one, but for what is named here. workspace: hx_decay_attention_workspace_size(...) bytes of device memory
  * (0 where no sequence is cut into segments), 16-byte aligned; it holds nothing between calls, and one
  * call uses it at a time. */
 size_t hx_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk,
@@ -228,8 +229,8 @@ int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t
  *   dq_i = scale * S_i dout_i;  dk_i = G_i v_i;  dv_i = G_i^T k_i;  dinit = e^g G_0 (dlast for no tokens)
  * dout: [batch, seqlen, heads, dv]; dq, dk_out, dv_out: like q, k and v but contiguous, all of `dtype`
  * (a shared head's gradient is the sum over its group, rounded once; rows behind a length are zero).
- * dlast (nullable: zero), dinit (nullable: not wanted): [batch, heads, dk, dv] fp32, which may be one
- * buffer. The states are formed again. workspace as above. */
+ * dlast (nullable: zero), dinit (nullable: not wanted): [batch, heads, dk, dv] fp32; dinit may be dlast's
+ * or init_state's buffer. The states are formed again. workspace as above. */
 size_t hx_decay_attention_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t heads,
                                              int64_t q_heads, int64_t k_heads, int64_t v_heads,
                                              int64_t dk, int64_t dv, int dtype);
@@ -446,7 +447,8 @@ int hx_rmsnorm_fwd(int64_t rows, int64_t dim, const float* x, const float* weigh
 /* The residual's addition, RMSNorm and rounding to 8 bits in one pass over rows of x [rows, dim]:
  *   r = x + delta (rounded to x's type);  y = r / sqrt(mean(r^2) + eps) * weight
  * dtype: x's and resid's; delta (nullable: none) of delta_dtype; both HX_F32 or HX_BF16. resid (nullable:
- * not wanted) receives r and may be x or delta itself. weight [dim] fp32 (nullable: no norm, y = r).
+ * not wanted) receives r and may be x or delta itself (of its type and stride; else no buffer may
+ * overlap another that is written). weight [dim] fp32 (nullable: no norm, y = r).
  * out_dtype HX_F32 or HX_BF16: y as such. HX_I8: codes of 8 bits with one scale a row, scales [rows]
  * fp32, which stand for code * scale:
  *   code = round(127 p / max|p|), ties to even, p = r * weight (the norm cancels);  scale = max|y| / 127

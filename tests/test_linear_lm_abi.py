@@ -47,6 +47,14 @@ def test_attention_sizes_and_types(call):
         assert call(L=-1) == DIM and call(L=2 ** 62) == UNSUPPORTED
 
 
+@pytest.mark.parametrize("call", [fwd, bwd, step])
+def test_attention_far_tokens(call):
+    """A chunk's offsets are counted in 32 bits."""
+    for name in ("ldq", "ldk", "ldv"):
+        assert call(**{name: 2 ** 23}) == UNSUPPORTED, name
+    assert call(h=2 ** 15, hq=1, hk=1, hv=1, dk=256) == UNSUPPORTED and call(h=2 ** 15, hq=1, hk=1, hv=1, dv=256) == UNSUPPORTED
+
+
 def test_attention_missing_operands():
     for k in ("q", "k", "v", "decay", "out"):
         assert fwd(**{k: None}) == INPUT and step(**{k: None}) == INPUT
@@ -81,6 +89,9 @@ def test_norm_refusals():
     assert norm(rows=0) == 0 and norm(dim=0) == 0
     assert norm(x=None) == INPUT and norm(y=None) == INPUT and norm(scales=None) == INPUT
     assert norm(ldx=7) == INPUT and norm(ldy=7) == INPUT and norm(delta=P, ldd=7) == INPUT and norm(resid=P, ldr=7) == INPUT
+    Q = ctypes.c_void_p(65536)
+    assert norm(resid=P, ldr=9) == INPUT and norm(delta=Q, resid=Q, ldr=9) == INPUT  # in place with another stride
+    assert norm(delta=Q, ddtype=1, resid=Q) == INPUT and norm(dtype=1, delta=Q, resid=Q) == INPUT  # or of another type
     assert norm(rows=1 << 40) == UNSUPPORTED and norm(rows=1 << 23, dim=4100, ldx=4100, ldy=4100) == UNSUPPORTED
 
 
