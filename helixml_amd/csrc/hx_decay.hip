@@ -186,33 +186,18 @@ __device__ inline Frag<float> finite_only(Frag<float> f) {
     for (int e = 0; e < 8; ++e) f.v[e] = not_finite(f.v[e]) ? 0.0f : f.v[e];
     return f;
 }
-// A row's elements from one of them on: 16 bytes moved down by `by` elements, zeros behind them.
-template <typename T>
-__device__ inline u32x4 moved(const u32x4& v, int by) {
-    const uint32_t bits = 8 * sizeof(T) * by;
-    uint32_t w[8] = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = bits & 64 ? w[i + 2] : w[i];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = bits & 32 ? w[i + 1] : w[i];
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], bits & 31);
-    }
-    return u32x4{w[0], w[1], w[2], w[3]};
-}
-
 // Rows by columns of T in LDS, 16 bytes apart from a multiple of all banks, and the registers through which a chunk of them comes
 // from global memory: a thread has the same 16 bytes of every few rows. Loads go out without a branch, rows and columns that are
 // not there reading ones that are; columns behind a row's end are never written to LDS and keep the zeros that it starts with.
-// WHOLE: rows end with a whole 16 bytes. Else the last 16 bytes end with the row and are moved into place.
+// WHOLE: rows end with a whole 16 bytes. Else the last 16 bytes end with the row, and repeat in LDS what stands before them (they
+// were moved into place in registers, for which the compiler took scratch memory: training 2 x 19407 x 15 x 57 bf16 1637 -> 608 us).
 template <typename T, int ROWS, int COLS, int THREADS, bool WHOLE>
 struct Tile {
     static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kPerRow = COLS / E, kStep = THREADS / kPerRow;
     static constexpr int kEach = (ROWS + kStep - 1) / kStep, kBytes = ROWS * kStride * (int)sizeof(T);
     static_assert(THREADS % kPerRow == 0, "a thread's column is the same in all rows");
     u32x4 reg[kEach];
-    int row, col, by, n;  // `by`: elements that what is loaded stands too early
+    int row, col, place, n;
     bool in;
     // columns c0.. of rows of n
     __device__ void begin(int c0, int width) {
@@ -221,7 +206,7 @@ struct Tile {
         const int want = c0 + threadIdx.x % kPerRow * E, most = WHOLE || n >= E ? n - E : 0;
         in = want < n;
         col = want < most ? want : most;
-        by = want - col;
+        place = WHOLE ? threadIdx.x % kPerRow * E : col - c0;
     }
     __device__ void unit(int i, const T* at, uint32_t off) {
         if (WHOLE || n >= E) {
@@ -252,20 +237,21 @@ struct Tile {
         }
     }
     __device__ void store(T* tile, int shift) {
-        if constexpr (!WHOLE) {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) reg[i] = moved<T>(reg[i], by);
-        }
         if (shift) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
                 if (row + i * kStep < shift) reg[i] = u32x4{0, 0, 0, 0};
         }
         if (!in) return;
-        T* const to = tile + row * kStride + threadIdx.x % kPerRow * E;
+        T* const to = tile + row * kStride + place;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            if (ROWS % kStep == 0 || row + i * kStep < ROWS) *reinterpret_cast<u32x4*>(to + i * kStep * kStride) = reg[i];
+            if (ROWS % kStep == 0 || row + i * kStep < ROWS) {
+                if constexpr (WHOLE)
+                    *reinterpret_cast<u32x4*>(to + i * kStep * kStride) = reg[i];
+                else
+                    __builtin_memcpy(to + i * kStep * kStride, &reg[i], 16);
+            }
     }
     // after store(): whether a value that was stored is not finite
     __device__ bool bad() const {
