@@ -193,7 +193,7 @@ __device__ inline Frag<float> finite_only(Frag<float> f) {
 // were moved into place in registers, for which the compiler took scratch memory: training 2 x 19407 x 15 x 57 bf16 1637 -> 608 us).
 template <typename T, int ROWS, int COLS, int THREADS, bool WHOLE>
 struct Tile {
-    static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kPerRow = COLS / E, kStep = THREADS / kPerRow;
+    static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kPerRow = (COLS > 128 ? 256 : COLS) / E, kStep = THREADS / kPerRow;
     static constexpr int kEach = (ROWS + kStep - 1) / kStep, kBytes = ROWS * kStride * (int)sizeof(T);
     static_assert(THREADS % kPerRow == 0, "a thread's column is the same in all rows");
     u32x4 reg[kEach];
@@ -208,31 +208,51 @@ struct Tile {
         col = want < most ? want : most;
         place = WHOLE ? threadIdx.x % kPerRow * E : col - c0;
     }
-    __device__ void unit(int i, const T* at, uint32_t off) {
-        if (WHOLE || n >= E) {
-            __builtin_memcpy(&reg[i], at + off, 16);
-        } else {
-            T v[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = at[off + (e < n ? e : n - 1)];
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = e < n ? v[e] : 0;
-            __builtin_memcpy(&reg[i], v, 16);
+    // A row of fewer than E elements, which only the narrowest tile holds.
+    static constexpr bool kNarrow = !WHOLE && COLS <= 64;
+    __device__ u32x4 narrow(const T* at) const {
+        uint64_t v[2] = {0, 0};
+        int k = 0;
+        if (sizeof(T) == 2 && (n & 4)) {
+            __builtin_memcpy(&v[0], at, 8);
+            k = 8;
         }
+        if (n & 2) {
+            uint64_t x = 0;
+            __builtin_memcpy(&x, at + k / sizeof(T), 2 * sizeof(T));
+            if (k) v[1] = x;
+            else v[0] = x;
+            k += 2 * sizeof(T);
+        }
+        if (n & 1) {
+            T x;
+            __builtin_memcpy(&x, at + k / sizeof(T), sizeof(T));
+            const uint64_t bits = sizeof(T) == 2 ? (uint64_t)x : (uint64_t)__builtin_bit_cast(uint32_t, (float)x);
+            if (k < 8) v[0] |= bits << (8 * k);
+            else v[1] |= bits << (8 * k - 64);
+        }
+        return u32x4{(uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32)};
     }
     // Rows shift.. of the tile are tokens of a chunk, ROWS - shift of them, the first (or, backwards, the last) at `first`.
     __device__ void load(const T* first, int64_t ld, int shift, bool back) {
-        if (shift == 0 && ROWS % kStep == 0) {  // one offset, and places that are the same for all threads
+        if (kNarrow && n < E) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                int k = row + i * kStep - shift;
+                k = k < 0 ? 0 : k >= ROWS - shift ? ROWS - shift - 1 : k;
+                reg[i] = narrow(first + (back ? ROWS - shift - 1 - k : k) * ld);
+            }
+        } else if (shift == 0 && ROWS % kStep == 0) {  // one offset, and places that are the same for all threads
             const uint32_t off = (uint32_t)((back ? kStep - 1 - row : row) * (int)ld + col);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) unit(i, first + (back ? kEach - 1 - i : i) * kStep * ld, off);
+            for (int i = 0; i < kEach; ++i) __builtin_memcpy(&reg[i], first + (back ? kEach - 1 - i : i) * kStep * ld + off, 16);
         } else {
             const int valid = ROWS - shift;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 int k = row + i * kStep - shift;
                 k = k < 0 ? 0 : k >= valid ? valid - 1 : k;
-                unit(i, first, (uint32_t)((back ? valid - 1 - k : k) * (int)ld + col));
+                __builtin_memcpy(&reg[i], first + (uint32_t)((back ? valid - 1 - k : k) * (int)ld + col), 16);
             }
         }
     }
@@ -276,7 +296,7 @@ struct Tile {
 
 template <typename T> constexpr int kPParts = sizeof(T) == 2 ? 2 : 1;
 // waves to a SIMD that a kernel's LDS leaves room for, as its register bound
-template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT ? (MP > 128 ? 2 : 3) : MP > 128 ? (NW == 8 ? 2 : 1) : NW == 8 ? 2 : MP > 64 ? 2 : sizeof(T) == 4 ? 4 : 3;
+template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT ? (MP > 128 ? 2 : 3) : MP > 192 ? (NW == 8 ? 2 : 1) : NW == 8 ? 2 : MP > 64 ? 2 : sizeof(T) == 4 ? 4 : 3;
 
 // One segment of one (sequence, head) through NW waves, 16 columns of the output to each; MP >= m channels of a and b, C tokens
 // a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state. A segment's last chunk that
@@ -710,10 +730,13 @@ constexpr int64_t kMaxStride = 1 << 23;  // elements from one token to the next:
 int chunk_of(int dtype) { return dtype == HX_BF16 ? 64 : 32; }
 
 // Segments that a sequence is cut into where the (sequence, head) pairs leave compute units idle: as many blocks as are
-// resident at once, each of two chunks at least.
+// resident at once, each of two chunks at least, and fewer of large states, which are written and read again for every one. 512, 256
+// and 128 for training: 1 x 65536 x 16 x 128/64 bf16 (q, k shared) 1298, 1602 and 2392 us, 1 x 16384 x 8 x 128 308, 276 and 306,
+// x 192 742, 674 and 700, x 256 1185, 1013 and 937.
 int64_t segments_of(int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv, int dtype, bool backward, int64_t* seglen) {
     const int64_t C = chunk_of(dtype), chunks = (L + C - 1) / C, pairs = B * H, wide = dk > dv ? dk : dv;
-    const int64_t target = wide > 64 ? 512 : dtype == HX_F32 ? 1024 : backward ? 512 : 768;
+    const int64_t area = dk * dv, large = area <= 8192 ? 512 : area <= 40960 ? 256 : 128;
+    const int64_t target = wide > 64 ? large : dtype == HX_F32 ? 1024 : backward ? 512 : 768;
     int64_t want = pairs > 0 ? target / pairs : 1;
     const int64_t most = chunks / 2;
     if (want > most) want = most;
@@ -766,14 +789,13 @@ int launch_mix_of(MixPasses& a, hipStream_t stream) {
 template <typename T, bool WHOLE, bool OUT, typename TO>
 int launch_mix_as(MixPasses& a, hipStream_t s) {
     const MixArgs& p = a.p[0];
-    if (p.n > 64) {
-        if (p.m <= 64) return launch_mix_of<T, 64, 8, WHOLE, OUT, TO>(a, s);
-        if (p.m <= 128) return launch_mix_of<T, 128, 8, WHOLE, OUT, TO>(a, s);
-        return launch_mix_of<T, 256, 8, WHOLE, OUT, TO>(a, s);
-    }
     if (p.m <= 64) return launch_mix_of<T, 64, 4, WHOLE, OUT, TO>(a, s);
     if (p.m <= 128) return launch_mix_of<T, 128, 4, WHOLE, OUT, TO>(a, s);
-    return launch_mix_of<T, 256, 4, WHOLE, OUT, TO>(a, s);
+    if (p.m <= 192) return launch_mix_of<T, 192, 4, WHOLE, OUT, TO>(a, s);
+    // Eight waves share a tile of m > 192, whose memory leaves room for one block a CU. Four do better below: training at 1 x 4096 x 8
+    // x 192 fp32 501 and 606 us, 1 x 16384 x 8 x 128 bf16 311 and 344; 1 x 16384 x 8 x 256 1430 and 1128.
+    if (p.n <= 64) return launch_mix_of<T, 256, 4, WHOLE, OUT, TO>(a, s);
+    return launch_mix_of<T, 256, 8, WHOLE, OUT, TO>(a, s);
 }
 template <typename T, bool OUT, typename TO>
 int launch_mix(MixPasses& a, hipStream_t s) {
