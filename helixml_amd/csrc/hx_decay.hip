@@ -746,9 +746,13 @@ int64_t segments_of(int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv, int
     const int64_t nseg = chunks > 0 ? (chunks + per - 1) / per : 1;
     return nseg >= 8 ? (nseg + 7) / 8 * 8 : nseg;  // whole rounds of dies, the last ones perhaps without tokens
 }
-// Up to this many, an output's block goes through the segments before it by itself (not where the last one's state takes the
-// first one's buffer, which another block may yet read).
-constexpr int kFewSegments = 8;
+// Up to this many, an output's block goes through the segments before it by itself, which saves the chain's launch but reads a part
+// after the other: fewer of large states (training at 2 x 520 x 1 x 168/58 fp32, six segments, 159 us so and 103 chained; 6 x 2048 x 16
+// x 128/64 bf16, five, 278 and 285). Not where the last one's state takes the first one's buffer, which another block may yet read.
+int64_t few_segments(int64_t dk, int64_t dv) {
+    const int64_t few = 40960 / (dk * dv);
+    return few < 8 ? few : 8;
+}
 
 struct Shape {
     int64_t B, L, H, hq, hk, hv, dk, dv;
@@ -876,7 +880,7 @@ extern "C" int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t hea
     p.m = (int)dk, p.n = (int)dv;
     p.log_decay = log_decay, p.lengths = lengths;
     p.init = init_state, p.last = last_state, p.parts = (float*)workspace;
-    p.chained = nseg > kFewSegments || (nseg > 1 && last_state && last_state == init_state);
+    p.chained = nseg > few_segments(dk, dv) || (nseg > 1 && last_state && last_state == init_state);
     p.state = dk * dv, p.sm = (int)dv, p.sn = 1;
     p.ps = p.es = scale, p.cs = 1.0f, p.e0 = 1, p.back = 0;
     p.out = out, p.ldo = heads * dv;
@@ -930,7 +934,7 @@ extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t hea
         int group;
     };
     const Operand Q{q, ldq, gq}, K{k, ldk, gk}, V{v, ldv, gv}, D{dout, heads * dv, 1};
-    const bool in_place = dinit && (dinit == dlast || dinit == init_state), chained = nseg > kFewSegments || (nseg > 1 && in_place);
+    const bool in_place = dinit && (dinit == dlast || dinit == init_state), chained = nseg > few_segments(dk, dv) || (nseg > 1 && in_place);
     const auto mixing = [&](const Operand& a, const Operand& b, const Operand& c, bool transposed, bool back, float* last) {
         MixArgs p{};
         p.B = batch, p.L = seqlen, p.H = heads;
