@@ -880,7 +880,7 @@ extern "C" int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t hea
     p.m = (int)dk, p.n = (int)dv;
     p.log_decay = log_decay, p.lengths = lengths;
     p.init = init_state, p.last = last_state, p.parts = (float*)workspace;
-    p.chained = nseg > few_segments(dk, dv) || (nseg > 1 && last_state && last_state == init_state);
+    p.chained = nseg > 1 && (nseg > few_segments(dk, dv) || (last_state && last_state == init_state));
     p.state = dk * dv, p.sm = (int)dv, p.sn = 1;
     p.ps = p.es = scale, p.cs = 1.0f, p.e0 = 1, p.back = 0;
     p.out = out, p.ldo = heads * dv;
@@ -934,7 +934,7 @@ extern "C" int hx_decay_attention_bwd(int64_t batch, int64_t seqlen, int64_t hea
         int group;
     };
     const Operand Q{q, ldq, gq}, K{k, ldk, gk}, V{v, ldv, gv}, D{dout, heads * dv, 1};
-    const bool in_place = dinit && (dinit == dlast || dinit == init_state), chained = nseg > few_segments(dk, dv) || (nseg > 1 && in_place);
+    const bool in_place = dinit && (dinit == dlast || dinit == init_state), chained = nseg > 1 && (nseg > few_segments(dk, dv) || in_place);
     const auto mixing = [&](const Operand& a, const Operand& b, const Operand& c, bool transposed, bool back, float* last) {
         MixArgs p{};
         p.B = batch, p.L = seqlen, p.H = heads;
