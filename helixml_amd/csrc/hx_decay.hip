@@ -301,6 +301,13 @@ template <typename T, int MP, int NW, bool OUT> constexpr int kOccupancy = !OUT 
 // One segment of one (sequence, head) through NW waves, 16 columns of the output to each; MP >= m channels of a and b, C tokens
 // a chunk. OUT: outputs, of type TO; else only the state that the segment gives from a zero state. A segment's last chunk that
 // is not whole stands at its tile's end, zeros before it, where its weights are a whole chunk's.
+// A wave keeps 16 columns of the state in accumulators, whose layout (rows 4u.. of a column) is the matrix instruction's operand as it is,
+// so the state never passes through LDS. bf16 operands that are formed in fp32 go in as two bf16 parts (scores and the state before a
+// chunk, 2^-17 of the value, below an output's rounding) or three (what a chunk adds to the state, which is carried on): one part's
+// 2^-9 would show. Chunks of 64 bf16 or 32 fp32 tokens: the scores' share grows with the chunk, the state's falls.
+// What bounds it: memory at some 4 TB/s (reading more than writing) for heads of 64 channels, the issue of matrix and LDS instructions of
+// its few waves a SIMD for wider ones. 1 x 65536 x 16 x 64 fp32, 1074 MB: segments' states 126-149 us (537 MB), outputs 315-348; 8 x 2048 x 16 x 64
+// bf16: 19 and 40, its three gradients 94.
 template <typename T, int MP, int C, int NW, bool WHOLE, bool OUT, typename TO>
 __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_kernel(const MixPasses all) {
     constexpr int THREADS = 64 * NW, MT = MP / 16, NT = C / 16, KB = C / 32, E = 16 / sizeof(T);
@@ -615,7 +622,8 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
     }
 }
 
-// Many segments' parts to the states before them, in place: of one or two passes.
+// Many segments' parts to the states before them, in place: of one or two passes. A thread has one element of the state, eight segments'
+// loads on their way at once. Each state is read and written once: 64 x 8 x 256 x 256 fp32 for two passes 63 us, 4.3 TB/s; some 4 us at least.
 struct ChainArgs {
     const float* init[2];
     float* parts[2];
@@ -653,7 +661,8 @@ __global__ __launch_bounds__(256) void chain_kernel(int64_t H, int64_t L, int64_
     }
 }
 
-// y[row][h][c] = sum over the heads of a group of x, in their order, rounded once; V neighbouring columns a thread
+// y[row][h][c] = sum over the heads of a group of x, in their order, rounded once; V neighbouring columns a thread. 65536 rows of 16
+// heads x 128 to one: 537 MB in 96-108 us (5.0-5.6 TB/s).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int group, int n, const float* __restrict__ x, T* __restrict__ y) {
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < total; i += (int64_t)gridDim.x * 256 * V) {
@@ -676,6 +685,7 @@ __global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int group
 // ------------------------------------------------------------------ one token
 // S = e^g S + k v^T, out = scale q S: a state is read and written once. A block takes 64 columns of one (sequence, head): 16
 // threads hold four columns each of a row, 16 rows at a time; the rows' parts of q S are joined in LDS in a fixed order.
+// Memory bounds it: 256 x 16 x 128 x 64, 268 MB, 41.8 us (6.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void step_kernel(int64_t H, int dk, int dv, int gq, int gk, int gv, float* __restrict__ state,
                                                    const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk,

@@ -88,7 +88,8 @@ __device__ inline void store_outputs(const I8Args& p, TO* to, int64_t left, floa
 // A block takes 16 NT outputs of 16 MT rows of X, its waves a run of K each, in windows of 256 columns. Pieces of weights come
 // straight into the matrix instruction's registers, a window ahead. X comes by memory, 16 lanes to a row's 256 bytes, since
 // lanes that each sit in a row of their own cost the L1 a look-up apiece (64 a load), and goes through LDS rows that a wave
-// keeps to itself. Sums are whole numbers: the waves' are added in any order to the same bits.
+// keeps to itself. Sums are whole numbers: the waves' are added in any order to the same bits. Bound by the latency of one round of loads
+// and of the joining (1 x 8192 x 2048 4.5 us, 3.7 TB/s of weights) and by X, which every block reads whole (48 x 2048 x 8192 8.5 us).
 constexpr int kWindow = 256, kWindowPieces = kWindow / kPieceCols, kXRow = kWindow + 16;
 
 template <int NT, int MT, typename TO>
@@ -208,7 +209,8 @@ __global__ __launch_bounds__(512) void linear_i8_rows_kernel(const I8Args p, con
 // straight into a two-stage LDS ring: rows of X as 128 bytes with their 16-byte chunks exchanged by row (chunk c of row r
 // in place c ^ (r & 7)), so that a fragment's 32 rows meet all banks, pieces of weights as they lie in memory, which is the
 // order they are read in. The next fragments are read and a later tile's loads issued between the matrix instructions; the barrier
-// of a K tile stands before its last quarter, whose fragments are in registers by then. Needs rows of X that start at
+// of a K tile stands before its last quarter, whose fragments are in registers by then. 8191 x 8192 x 2048 to bf16 with SiLU: 167-183 us, 1.5
+// to 1.65 POP/s of the 2.1 that a large library product reaches; a K of 2048 leaves a sixth of the time to first loads and outputs. Needs rows of X that start at
 // 16 bytes; columns behind the last whole K tile come straight from memory. Rows behind M and N are the last ones', and not stored.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTileCols = 128;
