@@ -191,6 +191,7 @@ __device__ inline Frag<float> finite_only(Frag<float> f) {
 // not there reading ones that are; columns behind a row's end are never written to LDS and keep the zeros that it starts with.
 // WHOLE: rows end with a whole 16 bytes. Else the last 16 bytes end with the row, and repeat in LDS what stands before them (they
 // were moved into place in registers, for which the compiler took scratch memory: training 2 x 19407 x 15 x 57 bf16 1637 -> 608 us).
+// Where a slice's first columns are a row's last, what repeats falls into the E elements of padding before them.
 template <typename T, int ROWS, int COLS, int THREADS, bool WHOLE>
 struct Tile {
     static constexpr int E = 16 / sizeof(T), kStride = COLS + E, kPerRow = (COLS > 128 ? 256 : COLS) / E, kStep = THREADS / kPerRow;

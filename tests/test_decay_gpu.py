@@ -221,6 +221,18 @@ def test_not_finite_stays_behind(dev, what, value, dtype):
         assert torch.equal(got["dq"][:, :at], want["dq"][:, :at])
 
 
+WIDTHS = [(1, 600, 1, 168, 58), (1, 700, 1, 5, 140), (2, 300, 2, 3, 7), (1, 1000, 2, 190, 190), (1, 330, 2, 193, 70), (1, 520, 1, 6, 2), (2, 200, 1, 256, 193),
+          (1, 1100, 1, 128, 65), (1, 90, 2, 256, 4)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", WIDTHS, ids=lambda s: "x".join(map(str, s)))
+def test_widths_in_segments(dev, shape, dtype):
+    """Rows that end anywhere, narrower than one load among them, in tiles of every width, with lengths, cut and not."""
+    bt, L = shape[:2]
+    check_all(dev, inputs(*shape, seed=sum(shape), dtype=dtype, lengths=[L - 1, L // 2][:bt]))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_carried_in_place(dev, dtype):
     """One buffer for the state before and after; one for its gradient."""
