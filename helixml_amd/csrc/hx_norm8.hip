@@ -118,8 +118,10 @@ struct RowFactor {
         return (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)q[3] << 24;
     }
 };
-// a row's scale; NaN where it holds what is not finite (a NaN among the products is above all numbers in `top`)
+// a row's scale; NaN where it holds what is not finite (a NaN among the products is above all numbers in `top`), 0 where all of its
+// products are zero, also where its squares are and eps is, so that 1 / rms has no value
 __device__ inline float scale_of(const RowSums& s, unsigned long long top, const NormArgs& p) {
+    if (top == 0) return 0.0f;
     const double inv = inverse_rms(s, p);
     return top >= 0x7ff0000000000000ull || !(inv <= 1.7e308) ? __uint_as_float(0x7fc00000u) : (float)(__longlong_as_double((long long)top) * inv / 127.0);
 }

@@ -452,7 +452,8 @@ int hx_rmsnorm_fwd(int64_t rows, int64_t dim, const float* x, const float* weigh
  * out_dtype HX_F32 or HX_BF16: y as such. HX_I8: codes of 8 bits with one scale a row, scales [rows]
  * fp32, which stand for code * scale:
  *   code = round(127 p / max|p|), ties to even, p = r * weight (the norm cancels);  scale = max|y| / 127
- * (0, with codes 0, for a row of zeros; NaN, with codes 0, for one that holds what is not finite). Sums,
+ * (0, with codes 0, for a row whose p are all zero, whatever eps is; NaN, with codes 0, for one that holds
+ * what is not finite). Sums,
  * products and codes are formed in 64 bits, so the codes are the definition's own. ldx, ldd, ldr, ldy:
  * elements from one row to the next. nn::RMSNorm::forward (crates/nn/src/lib.rs:258-285) is its case
  * without delta. Fewer than 2^22 rows (2^24 of up to 4096 elements). */
