@@ -22,7 +22,8 @@ struct NormArgs {
 // With r = x + delta as it is stored and p = r w, a row is p / rms(r). In 8 bits its codes are round(127 p / max |p|), whatever the
 // norm, and its scale is max |p| / (127 rms). The squares are summed in 64 bits, and the codes are those of the definition, not of
 // one order of rounding: 127 p / max |p| in 32 bits is off by less than 4e-5 steps, so what lies further than 1e-4 from a border
-// is decided by it, and the rest (one element in five thousand) by the exact products, which 64 bits hold (two numbers of 24).
+// is decided by it, and the rest (one element in five thousand) by the exact products, which 64 bits hold (two numbers of 24), and
+// the exact sign of their distance from the border.
 // The largest of the exact products is sought among the elements that are the largest in 32 bits. Rows whose products leave 32
 // bits' range take 64 throughout. 32768 x 2048 fp32 with a bf16 delta: 64 bits for every element and a wave a row 207 us,
 // a block of four waves a row, 2 x 4 elements a lane (58 registers for 145), 153 (4.8 TB/s).
@@ -79,6 +80,17 @@ __device__ inline double inverse_rms(const RowSums& s, const NormArgs& p) {
     return p.weight ? 1.0 / sqrt(s.squares / (double)p.dim + (double)p.eps) : 1.0;
 }
 
+// round(127 |p| / top), ties to even, of products of 48 bits; by = 127 / top. 127 |p| has up to 55 bits, so its quotient would be rounded
+// twice, and an element of half the row's largest go either way. The border above a whole part that is right or one off is exact: 254 |p| -
+// (2 whole + 1) top, the second product as a rounded one and its error. Next to a border the difference is a few units of what the
+// products are multiples of; elsewhere its sign is plain.
+__device__ inline int exact_code(float r, float w, double top, double by) {
+    const double rw = (double)r * (double)w, p = fabs(rw), whole = floor(p * by), odd = 2.0 * whole + 1.0, edge = odd * top;
+    const double over = fma(254.0, p, -edge) - fma(odd, top, -edge);
+    const int code = (int)whole + (over > 0.0 || (over == 0.0 && ((int)whole & 1)));
+    return rw < 0.0 ? -code : code;  // (the signs' own bits were held in registers for all elements, 10 more)
+}
+
 enum Kind { kF32 = HX_F32, kBf16 = HX_BF16, kI8 = HX_I8 };
 
 // What four elements become. For codes: the largest |p| exactly and 127 over it in 32 bits (0 where that does not serve).
@@ -112,8 +124,9 @@ struct RowFactor {
             q[e] = (int)whole;
         }
         if (border) {
+            const double by = 127.0 / top;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = zero ? 0 : (int)rint((double)r[e] * (double)w[e] * 127.0 / top);
+            for (int e = 0; e < 4; ++e) q[e] = zero ? 0 : exact_code(r[e], w[e], top, by);
         }
         return (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)q[3] << 24;
     }
@@ -249,9 +262,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void row_kernel(cons
     }
 }
 
-// Rows of any width: passes over the row, the later ones from what the first stored where it stored anything.
+// Rows of any width: passes over the row, the later ones from what the first stored where it stored anything. Two blocks a CU, whose 64
+// registers the 8-bit form passes by two: 4096 x 20000 bf16 with a bf16 delta 224 us, with one block 316.
 template <typename TX, int KIND>
-__global__ __launch_bounds__(1024) void wide_row_kernel(const NormArgs p) {
+__global__ __launch_bounds__(1024, 8) void wide_row_kernel(const NormArgs p) {
     const int64_t row = blockIdx.x;
     RowSums s{0.0, 0};
     const auto weights = [&](int64_t c, float (&w)[4]) {

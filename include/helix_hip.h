@@ -453,10 +453,10 @@ int hx_rmsnorm_fwd(int64_t rows, int64_t dim, const float* x, const float* weigh
  * fp32, which stand for code * scale:
  *   code = round(127 p / max|p|), ties to even, p = r * weight (the norm cancels);  scale = max|y| / 127
  * (0, with codes 0, for a row whose p are all zero, whatever eps is; NaN, with codes 0, for one that holds
- * what is not finite). Sums,
- * products and codes are formed in 64 bits, so the codes are the definition's own. ldx, ldd, ldr, ldy:
- * elements from one row to the next. nn::RMSNorm::forward (crates/nn/src/lib.rs:258-285) is its case
- * without delta. Fewer than 2^22 rows (2^24 of up to 4096 elements). */
+ * what is not finite). Squares are summed in 64 bits, and the codes are those of exact arithmetic, whatever
+ * they are formed in (32 bits far from a border, 64 next to one). ldx, ldd, ldr, ldy: elements from one
+ * row to the next. nn::RMSNorm::forward (crates/nn/src/lib.rs:258-285) is its case without delta. Fewer
+ * than 2^22 rows (2^24 of up to 4096 elements). */
 int hx_add_rmsnorm(int64_t rows, int64_t dim, int dtype, const void* x, int64_t ldx, int delta_dtype,
                    const void* delta, int64_t ldd, const float* weight, float eps, void* resid,
                    int64_t ldr, int out_dtype, void* y, int64_t ldy, float* scales, void* stream);

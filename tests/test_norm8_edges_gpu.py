@@ -1,4 +1,6 @@
-"""The norm to 8 bits (hx_add_rmsnorm) where its arithmetic is at an end: rows of zeros without an eps."""
+"""The norm to 8 bits (hx_add_rmsnorm) where its arithmetic is at an end: rows of zeros without an eps, ties between products that fill
+48 bits. Codes are compared with the definition in whole numbers."""
+import numpy as np
 import pytest
 import torch
 
@@ -27,3 +29,37 @@ def test_rows_of_zeros_without_eps(dev, dim):
         for i in range(5):
             one, s = lm.add_rmsnorm(x[i: i + 1], weight, eps=0.0)
             assert torch.equal(codes[i], one[0]) and torch.equal(scales[i], s[0]) and (i in zero or s[0] > 0)
+
+
+def whole_codes(r, w):
+    """round(127 p / max |p|), ties to even, of whole r and w of at most 24 bits: every step in whole numbers of at most 56 bits."""
+    p = r.astype(np.int64) * w.astype(np.int64)
+    top = np.abs(p).max(1, keepdims=True)
+    code, rest = np.divmod(127 * np.abs(p), top)
+    up = (2 * rest > top) | ((2 * rest == top) & (code % 2 == 1))
+    return (np.sign(p) * (code + up)).astype(np.int8)
+
+
+@pytest.mark.parametrize("dim", DIMS)
+def test_ties_of_products_of_48_bits(dev, dim):
+    """Ties go to the even code also where 127 p does not fit the 53 bits of a double: every border c + 1/2, both signs, and values
+    next to one, in columns with one weight and with weights that make up for their halves."""
+    g = np.random.default_rng(dim)
+    rows = 64
+    a = g.integers(1 << 15, 1 << 16, (rows, 1)) | 1
+    c = np.arange(dim) % 127
+    r = (2 * c + 1) * a * g.choice([-1, 1], (rows, dim))
+    odd = g.random((rows, dim)) < 0.1
+    r = np.where(odd, r + g.integers(-1, 2, r.shape), r)
+    r[:, dim // 3] = 254 * a[:, 0]
+    w = np.full(dim, int(g.integers(1 << 23, 1 << 24)) | 1)
+    half = g.random(dim) < 0.3
+    half[dim // 3] = False
+    w2, r2 = np.where(half, w * 2, w).astype(np.float64) / 2, r  # p / 2 of the others: ties at other borders
+    for weight, x, whole_w in ((w.astype(np.float64), r, w), (w2, r2, np.where(half, 2 * w, w))):
+        want = whole_codes(x, whole_w)
+        for scale in (1.0, 2.0 ** -30, 2.0 ** 60):
+            X, W = torch.from_numpy(x.astype(np.float32) * np.float32(scale)), torch.from_numpy(weight.astype(np.float32))
+            assert np.array_equal(W.double().numpy(), weight) and np.array_equal(X.double().numpy() / scale, x)
+            codes, _ = lm.add_rmsnorm(X.to(dev), W.to(dev))
+            assert np.array_equal(codes.cpu().numpy(), want), int((codes.cpu().numpy() != want).sum())
