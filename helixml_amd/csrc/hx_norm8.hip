@@ -111,7 +111,8 @@ struct RowFactor {
         RowFactor f{};
         f.inv = inverse_rms(s, p);
         f.m32 = (float)f.inv;
-        f.fast = s.common();
+        // (a subnormal product is off by 2^-150, which the factor lifts: to 2^-141 at most, far below half a step of bf16)
+        f.fast = s.common() && f.inv >= 0x1p-100 && f.inv <= 0x1p9;
         return f;
     }
     __device__ uint32_t codes(const float (&r)[4], const float (&w)[4]) const {

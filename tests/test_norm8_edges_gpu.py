@@ -1,11 +1,11 @@
 """The norm to 8 bits (hx_add_rmsnorm) where its arithmetic is at an end: rows of zeros without an eps, ties between products that fill
-48 bits. Codes are compared with the definition in whole numbers."""
+48 bits, factors that 32 bits do not hold. Codes are compared with the definition in whole numbers, outputs with float64."""
 import numpy as np
 import pytest
 import torch
 
 from helixml_amd import lm, ssm
-from tests.test_i8_gpu import F32
+from tests.test_i8_gpu import BF16, F32, HALF, I8, definition
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,25 @@ def test_ties_of_products_of_48_bits(dev, dim):
             assert np.array_equal(W.double().numpy(), weight) and np.array_equal(X.double().numpy() / scale, x)
             codes, _ = lm.add_rmsnorm(X.to(dev), W.to(dev))
             assert np.array_equal(codes.cpu().numpy(), want), int((codes.cpu().numpy() != want).sum())
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, F32, I8], ids=["bf16", "f32", "i8"])
+@pytest.mark.parametrize("dim", DIMS)
+def test_factors_past_32_bits(dev, dim, out_dtype):
+    """Rows so small or large that 1 / rms leaves what 32 bits hold (with an eps of 0), and products that do while the outputs do not."""
+    g = torch.Generator().manual_seed(dim)
+    n = lambda: torch.randn(4, dim, generator=g)  # noqa: E731
+    spread = 10.0 ** (torch.rand(dim, generator=g) * 16 - 13)
+    spread[0] = 1e3
+    for x, w in ((n() * 1e-42, torch.full((dim,), 1e30)), (torch.sign(n()) * 3e38, torch.full((dim,), 1e-30)), (n() * 1e-32, spread),
+                 (n() * 1e30, 1e-6 / spread)):
+        _, p, inv = definition(x, w, None, eps=0.0)
+        y = lm.add_rmsnorm(x.to(dev), w.to(dev), eps=0.0, out_dtype=out_dtype)
+        if out_dtype == I8:
+            top = np.abs(p).max(1)
+            assert np.array_equal(y[0].cpu().numpy(), np.rint(p * 127.0 / top[:, None]).astype(np.int8))
+            got, want, half = y[1], top * inv / 127.0, 2.0 ** -24
+        else:
+            got, want, half = y, p * inv[:, None], HALF[out_dtype]
+        # bf16's products may be formed in 32 bits, whose subnormals are off by 2^-150 before a factor of up to 2^9
+        assert (np.abs(got.double().cpu().numpy() - want) <= half * np.abs(want) * (1 + 2.0 ** -20) + 2.0 ** -134 + 2.0 ** -141).all()
