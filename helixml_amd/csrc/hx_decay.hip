@@ -44,6 +44,7 @@ constexpr int kMaxPasses = 3;
 struct MixPasses {
     MixArgs p[kMaxPasses];
     int count, slices;
+    int64_t b0;  // the first sequence of the launch
 };
 
 // w^x for x >= 0 as 2^(x l2); a decay of nothing (g = -inf) keeps w^0 = 1.
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(64 * NW, (kOccupancy<T, MP, NW, OUT>)) void mix_ker
     const int h = (int)(id % heads);
     id = id / heads * dies + die;
     const int seg = (int)(id % (uint32_t)p.nseg);
-    const int64_t b = id / (uint32_t)p.nseg;
+    const int64_t b = all.b0 + id / (uint32_t)p.nseg;
     int64_t len = p.L;
     if (p.lengths) {
         const int64_t given = p.lengths[b];
@@ -795,10 +796,14 @@ int launch_mix_of(MixPasses& a, hipStream_t stream) {
     HX_REQUIRE(bytes <= 65536 || grant_dynamic_lds((const void*)k, bytes, 16), HX_ERR_BACKEND, "decay_attention: %zu bytes of LDS not granted", bytes);
     const MixArgs& p = a.p[0];
     a.slices = (p.n + 16 * NW - 1) / (16 * NW);
-    const int64_t blocks = p.B * p.H * p.nseg * a.slices * a.count;
-    HX_REQUIRE(blocks < ((int64_t)1 << 32) / (64 * NW), HX_ERR_UNSUPPORTED, "decay_attention: too many blocks");
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * NW), bytes, stream, a);
-    HX_LAUNCH_CHECK();
+    // A launch holds fewer than 2^32 threads: many short sequences take several, whole sequences to each (one has fewer than 2^16 heads by
+    // four slices by three passes, or, cut into segments, some thousand blocks).
+    const int64_t each = p.H * p.nseg * a.slices * a.count, most = (((int64_t)1 << 32) / (64 * NW) - 1) / each;
+    for (a.b0 = 0; a.b0 < p.B; a.b0 += most) {
+        const int64_t count = p.B - a.b0 < most ? p.B - a.b0 : most;
+        hipLaunchKernelGGL(k, dim3((unsigned)(count * each)), dim3(64 * NW), bytes, stream, a);
+        HX_LAUNCH_CHECK();
+    }
     return HX_OK;
 }
 template <typename T, bool WHOLE, bool OUT, typename TO>
