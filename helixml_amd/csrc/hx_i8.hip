@@ -2,6 +2,7 @@
 #include <cmath>
 
 #include "hx_common.h"
+#include "hx_i8_rule.h"
 #include "hx_wave.h"
 
 namespace hx {
@@ -408,23 +409,13 @@ int launch_tiles(const I8Args& p, hipStream_t s) {
 
 template <typename TO>
 int launch_i8(const I8Args& p, hipStream_t s) {
-    const auto tiles = [&](int64_t side) { return ((p.M + side - 1) / side) * ((p.N + side - 1) / side); };
-    // Many rows: tiles of 128 where there are enough for half the chip, two blocks to a CU, so that one's outputs are written while the
-    // other multiplies; tiles of 256 from K 4096 on. 128 and 256 wide, in us: 8192 x 8192 x 2048 177 and 178, x 4096 361 and
-    // 306, 4096 x 4096 x 8192 143 and 118, 13479 x 13976 x 272 to fp32 286 and 357. Tiles of 128 and few rows' kernel: 1024 x 2048 x
-    // 2048 14.6 and 15.7 (128 tiles), 512 x 2048 x 2048 14.1 and 10.5 (64 tiles).
-    if (aligned(p.X, 16) && p.ldx % 16 == 0 && p.ldx < (1 << 22) && tiles(128) < (1 << 23)) {
-        if (p.K >= 4096 && tiles(256) >= 256) return launch_tiles<4, TO>(p, s);
-        if (p.M > 128 && tiles(128) >= 128) return launch_tiles<2, TO>(p, s);
+    switch (i8_kernel(p.M, p.N, p.K, aligned(p.X, 16) && p.ldx % 16 == 0 && p.ldx < (1 << 22))) {
+        case I8Kernel::kTiles256: return launch_tiles<4, TO>(p, s);
+        case I8Kernel::kTiles128: return launch_tiles<2, TO>(p, s);
+        case I8Kernel::kRows64x32: return launch_rows<2, 4, TO>(p, s);
+        case I8Kernel::kRows32x32: return launch_rows<2, 2, TO>(p, s);
+        default: return launch_rows<1, 1, TO>(p, s);
     }
-    // Few rows, a block's outputs by rows: 16 x 16 where blocks are wanting, 32 x 32, 32 x 64 where there are more of them than are
-    // resident. 16 x 16, 32 x 32 and 32 x 64: 48 x 2048 x 8192 9.4, 8.5 and 12.0; 32 x 2048 x 8192 6.8, 8.1 and 11.8; 48 x 8192 x
-    // 2048 8.1, 7.4 and 8.1; 256 x 1024 x 8192 13.9, 9.5 and 12.3; 1024 x 2048 x 2048 23.8, 15.7 and 18.0; 4096 x 4096 x 8192 597,
-    // 320 and 267.
-    const int64_t outs = (p.N + 15) / 16;
-    if (p.M <= 16 || (p.M <= 32 && outs <= 128)) return launch_rows<1, 1, TO>(p, s);
-    if (outs * ((p.M + 63) / 64) < 4096) return launch_rows<2, 2, TO>(p, s);
-    return launch_rows<2, 4, TO>(p, s);
 }
 
 }  // namespace
