@@ -200,12 +200,13 @@ int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, c
  *   S_i = e^g S_{i-1} + k_i v_i^T;   out_i = scale * q_i^T S_i;   g = log_decay[head]
  * the matrix member of the family (the reference's recurrences, crates/nn/src/ssm.rs:138-186, carry a
  * state per channel). g is a constant of the head, -inf (nothing is kept) and 0 (everything is) among
- * them; it has no gradient here.
+ * them; it has no gradient here. A growth (g > 0) is carried as far as e^(64 g) and e^(g seqlen) fit 32
+ * bits, and may give NaN beyond.
  * q: [batch, seqlen, q_heads, dk], k: [batch, seqlen, k_heads, dk], v: [batch, seqlen, v_heads, dv] of
  * `dtype` with ldq, ldk, ldv elements from one token to the next (so they can be slices of one
  * projection's output; a token's heads follow each other). q_heads, k_heads and v_heads each divide
  * `heads`: head h reads head h / (heads / q_heads) of q, and so on (k and v shared by groups of queries,
- * or q and k shared as a state-space block shares B and C). out: [batch, seqlen, heads, dv] of `dtype`.
+ * or q and k by all heads, as a state-space block shares B and C, though that decays by the token). out: [batch, seqlen, heads, dv] of `dtype`.
  * log_decay: [heads] fp32. init_state (nullable: zero), last_state (nullable): [batch, heads, dk, dv]
  * fp32, which may be one buffer. lengths (nullable: seqlen): int32 [batch], clamped to [0, seqlen]; what
  * lies behind a sequence's length is not read, its rows of out are zero, and last_state is the state
@@ -214,9 +215,9 @@ int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, c
  * as bf16 are split into two or three bf16 parts), the same bits on every call; an infinite value may
  * become NaN, but nothing reaches the tokens before it. dk and dv 1..256, batch * heads < 2^24, heads <
  * 2^16, batch * seqlen < 2^40, ldq, ldk, ldv and heads * max(dk, dv) < 2^23 (else HX_ERR_UNSUPPORTED). No
- * buffer that is written may overlap another one, but for what is named here. workspace: hx_decay_attention_workspace_size(...) bytes of device memory
- * (0 where no sequence is cut into segments), 16-byte aligned; it holds nothing between calls, and one
- * call uses it at a time. */
+ * buffer that is written may overlap another one, but for what is named here. workspace:
+ * hx_decay_attention_workspace_size(...) bytes of device memory (0 where no sequence is cut into segments),
+ * 16-byte aligned; it holds nothing between calls, and one call uses it at a time. */
 size_t hx_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk,
                                          int64_t dv, int dtype);
 int hx_decay_attention_fwd(int64_t batch, int64_t seqlen, int64_t heads, int64_t q_heads,
@@ -382,9 +383,9 @@ int hx_i8_quantize(int64_t N, int64_t K, const float* w, void* packed, float* sc
  * (crates/nn/src/lib.rs:120-134): X [M, K] int8 (row stride ldx) with one scale a row x_scales [M] (what
  * hx_add_rmsnorm gives with HX_I8), packed (16-byte aligned) and scales as above, bias [N] fp32
  * (nullable), Y [M, N] of out_dtype HX_F32 or HX_BF16 (row stride ldy); act as in hx_gemm_bf16 (bit 0
- * SiLU, bit 1 Y = Y + result). Products are summed exactly in 32-bit integers and scaled once, so a
- * row's result does not depend on the rows beside it. Any M, N, K and any alignment of X and Y (K < 2^17, N <
- * 2^26, M up to 64 * 65535, else HX_ERR_UNSUPPORTED). */
+ * SiLU, bit 1 Y = Y + result). Products are summed exactly in 32-bit integers and scaled once, by x_scale *
+ * scale in fp32, so a row's result does not depend on the rows beside it. Any M, N, K and any alignment of
+ * X and Y (K < 2^17, N < 2^26, M up to 64 * 65535, else HX_ERR_UNSUPPORTED). */
 int hx_linear_i8(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const float* x_scales,
                  const void* packed, const float* scales, const float* bias, int act, int out_dtype,
                  void* Y, int64_t ldy, void* stream);

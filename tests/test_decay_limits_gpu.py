@@ -1,10 +1,11 @@
-"""Linear attention with a decay a head at the ends of what it takes: more blocks than one launch holds, and states that live for
-hundreds of chunks."""
+"""Linear attention with a decay a head at the ends of what it takes: more blocks than one launch holds, no tokens at all, states that
+grow, and states that live for hundreds of chunks."""
 import numpy as np
 import pytest
 import torch
 
 from helixml_amd import ssm
+from tests.test_decay_gpu import check_all, inputs, on
 
 F32, BF16 = torch.float32, torch.bfloat16
 HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8}
@@ -40,6 +41,36 @@ def test_more_gradients_than_a_launch_holds(dev):
         s, m = (a * b).sum(-1, keepdim=True), (a * b).abs().sum(-1, keepdim=True)
         bound = 0.25 * m * c.abs() * 2 * (d + 8) * 2.0 ** -24
         assert ((got[name] - 0.25 * s * c).abs() <= bound + 1e-30).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("L,decay", [(1, [1.2, 1.0]), (3, [1.2, 0.0]), (65, [1.2, 0.5, -0.1]), (70, [1.0, 0.3]), (200, [0.4, 0.1, -0.4])])
+def test_states_that_grow(dev, L, decay, dtype):
+    """A growth is carried as a decay is, as long as that of 64 tokens and of the sequence fits 32 bits: in one chunk that is not whole, over
+    several, over segments."""
+    check_all(dev, inputs(2, L, len(decay), 24, 20, seed=L, dtype=dtype, decay=decay))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_no_tokens_and_no_sequences(dev, dtype):
+    """The states pass through unchanged, of shared heads too; nothing is launched for a batch or a head count of none."""
+    x = on(dev, inputs(3, 0, 4, 24, 40, seed=0, dtype=dtype, hk=2, hv=1))
+    args = (x["q"], x["k"], x["v"], x["log_decay"])
+    out, last = ssm.decay_attention_fwd(*args, init_state=x["init"], return_last_state=True)
+    assert out.shape == (3, 0, 4, 40) and torch.equal(last, x["init"])
+    dq, dk, dv, dinit = ssm.decay_attention_bwd(*args, x["dout"], init_state=x["init"], dlast=x["dlast"])
+    assert dq.shape == x["q"].shape and dk.shape == x["k"].shape and dv.shape == x["v"].shape and torch.equal(dinit, x["dlast"])
+    assert not ssm.decay_attention_fwd(*args, return_last_state=True)[1].any() and not ssm.decay_attention_bwd(*args, x["dout"])[3].any()
+    for bt, heads in ((0, 4), (3, 0)):
+        x = on(dev, inputs(bt, 7, max(heads, 1), 24, 40, seed=0, dtype=dtype))
+        q, k, v, do = (x[n][:, :, :heads].contiguous() for n in ("q", "k", "v", "dout"))
+        g = x["log_decay"][:heads]
+        out, last = ssm.decay_attention_fwd(q, k, v, g, return_last_state=True)
+        assert out.shape == (bt, 7, heads, 40) and last.shape == (bt, heads, 24, 40)
+        assert [t.shape for t in ssm.decay_attention_bwd(q, k, v, g, do)] == [q.shape, k.shape, v.shape, last.shape]
+        assert ssm.decay_attention_step(last, q[:, 0], k[:, 0], v[:, 0], g).shape == (bt, heads, 40)
 
 
 # ------------------------------------------------------------------ states that live long
