@@ -687,7 +687,8 @@ __global__ __launch_bounds__(256) void group_sum_kernel(int64_t total, int group
 // ------------------------------------------------------------------ one token
 // S = e^g S + k v^T, out = scale q S: a state is read and written once. A block takes 64 columns of one (sequence, head): 16
 // threads hold four columns each of a row, 16 rows at a time; the rows' parts of q S are joined in LDS in a fixed order.
-// Memory bounds it: 256 x 16 x 128 x 64, 268 MB, 41.8 us (6.4 TB/s).
+// Memory bounds it: 256 x 16 x 128 x 64, 268 MB, 42 us (6.4 TB/s). Columns that do not fill a block's 64 leave its threads idle: 128 x 16
+// 17.6 (67 MB, 3.8 TB/s), 128 x 66 63 (4.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void step_kernel(int64_t H, int dk, int dv, int gq, int gk, int gv, float* __restrict__ state,
                                                    const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk,
@@ -742,9 +743,18 @@ constexpr int64_t kMaxStride = 1 << 23;  // elements from one token to the next:
 int chunk_of(int dtype) { return dtype == HX_BF16 ? 64 : 32; }
 
 // Segments that a sequence is cut into where the (sequence, head) pairs leave compute units idle: as many blocks as are
-// resident at once, each of two chunks at least, and fewer of large states, which are written and read again for every one. 512, 256
-// and 128 for training: 1 x 65536 x 16 x 128/64 bf16 (q, k shared) 1298, 1602 and 2392 us, 1 x 16384 x 8 x 128 308, 276 and 306,
-// x 192 742, 674 and 700, x 256 1185, 1013 and 937.
+// resident at once, each of two chunks at least, and fewer of large states, which are written and read again for every one. Blocks aimed at,
+// in us:
+//   64 x 64 channels                   256   512   768  1024  2048
+//   fp32 forward   1 x 65536 x 16      649   440   417   397   409      1 x 16384 x 8    86    71    75    77   100
+//   fp32 backward  1 x 65536 x 16     1035  1004  1031  1010  1016      8 x 2048 x 16   265   257   284   277   295
+//   bf16 forward   1 x 65536 x 16      333   206   208   216   223      8 x 2048 x 16    81    55    54    68    75
+//   bf16 backward  1 x 65536 x 16      471   477   480   475   497      8 x 2048 x 16   105   113   125   143   156
+// so 1024, 768 and 512 stand where the long sequences take them; a few percent are left at shorter ones, most at a single head (1 x 131072 x
+// 1: fp32 forward 172 for 109 with 256). Training, wider heads, 128, 256 and 512 blocks: 1 x 65536 x 16 x 128/64 bf16 (q, k shared) 2342,
+// 1598 and 1268; 1 x 16384 x 8 bf16 x 80 295, 249 and 269, x 96 298, 253 and 277, x 128 304, 265 and 301, x 192 682, 662 and 736, x 200 768, 844
+// and 983, x 256 822, 899 and 1061. The rule goes by a state's elements: 512 up to 8192, 256 up to 40960 (192 x 192 are
+// 36864; 200 x 200, 40000, would do better with 128, as every tile of more than 192 channels does), 128 beyond.
 int64_t segments_of(int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv, int dtype, bool backward, int64_t* seglen) {
     const int64_t C = chunk_of(dtype), chunks = (L + C - 1) / C, pairs = B * H, wide = dk > dv ? dk : dv;
     const int64_t area = dk * dv, large = area <= 8192 ? 512 : area <= 40960 ? 256 : 128;
@@ -812,8 +822,9 @@ int launch_mix_as(MixPasses& a, hipStream_t s) {
     if (p.m <= 64) return launch_mix_of<T, 64, 4, WHOLE, OUT, TO>(a, s);
     if (p.m <= 128) return launch_mix_of<T, 128, 4, WHOLE, OUT, TO>(a, s);
     if (p.m <= 192) return launch_mix_of<T, 192, 4, WHOLE, OUT, TO>(a, s);
-    // Eight waves share a tile of m > 192, whose memory leaves room for one block a CU. Four do better below: training at 1 x 4096 x 8
-    // x 192 fp32 501 and 606 us, 1 x 16384 x 8 x 128 bf16 311 and 344; 1 x 16384 x 8 x 256 1430 and 1128.
+    // Eight waves share a tile of m > 192, whose memory leaves room for one block a CU. Training, four and eight waves: 1 x 16384 x 8 x 256 bf16
+    // 1132 and 817, 1 x 4096 x 8 x 256 fp32 721 and 588; four do as well or better below: 1 x 16384 x 8 x 192 bf16 664 and 678, 1 x 4096 x
+    // 8 x 192 fp32 415 and 502, 1 x 16384 x 8 x 128 bf16 265 and 280 (fp32, 4096 tokens, 205 and 200).
     if (p.n <= 64) return launch_mix_of<T, 256, 4, WHOLE, OUT, TO>(a, s);
     return launch_mix_of<T, 256, 8, WHOLE, OUT, TO>(a, s);
 }

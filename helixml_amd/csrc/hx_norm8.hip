@@ -25,8 +25,9 @@ struct NormArgs {
 // is decided by it, and the rest (one element in five thousand) by the exact products, which 64 bits hold (two numbers of 24), and
 // the exact sign of their distance from the border.
 // The largest of the exact products is sought among the elements that are the largest in 32 bits. Rows whose products leave 32
-// bits' range take 64 throughout. 32768 x 2048 fp32 with a bf16 delta: 64 bits for every element and a wave a row 207 us,
-// a block of four waves a row, 2 x 4 elements a lane (58 registers for 145), 153 (4.8 TB/s).
+// bits' range take 64 throughout. Memory bounds it. 32768 x 2048 fp32 with a bf16 delta: 64 bits for every element and a wave a row 207 us,
+// a block of four waves a row, 2 x 4 elements a lane (60 registers for 145), 146 (5.1 TB/s); to fp32, every element in 64 bits, 181 (5.2), to
+// bf16 151 (5.3). A bf16 stream has fewer bytes for the same arithmetic: with a bf16 delta 111 (4.2 TB/s), without a delta 62 to 65 (3.1).
 struct RowSums {
     double squares;
     uint32_t top;  // the largest |p| in 32 bits: the bits of numbers without a sign order as they do, with NaN above all

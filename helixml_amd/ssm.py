@@ -376,9 +376,9 @@ def _scratch(name, given, device, *sizes):
 def decay_attention_fwd(q, k, v, log_decay, scale=1.0, lengths=None, init_state=None, return_last_state=False, out=None,
                         workspace=None, stream=None):
     """Linear attention with one decay a head (hx_decay_attention_fwd): S_i = e^g S_{i-1} + k_i v_i^T, out_i = scale q_i^T S_i,
-    g = log_decay[head], a constant of the head (a growth, g > 0, as far as e^(64 g) and e^(g L) fit 32 bits). q: [batch, L, q_heads, dk], k: [batch, L, k_heads, dk], v: [batch, L, v_heads, dv]
-    fp32 or bf16, each with heads that divide log_decay's (fp32 [heads]) and are shared by groups of them; tokens may be
-    strided. lengths: int32 [batch], tokens of each sequence (all when None; rows of ``out`` behind them are zero).
+    g = log_decay[head], a constant of the head (a growth, g > 0, as far as e^(64 g) and e^(g L) fit 32 bits).
+    q: [batch, L, q_heads, dk], k: [batch, L, k_heads, dk], v: [batch, L, v_heads, dv] fp32 or bf16, each with heads that
+    divide log_decay's (fp32 [heads]) and are shared by groups of them; tokens may be strided. lengths: int32 [batch], tokens of each sequence (all when None; rows of ``out`` behind them are zero).
     init_state: [batch, heads, dk, dv] fp32. Returns out [batch, L, heads, dv], followed by the last state where asked for.
     Nothing is recorded for autograd: decay_attention_bwd gives the gradients. ``workspace``: a uint8 device
     tensor of at least decay_attention_workspace_size(...) bytes; allocated here when not given."""

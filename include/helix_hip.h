@@ -206,7 +206,8 @@ int hx_gated_state_update(int64_t batch, int64_t dim, int dtype, float* state, c
  * `dtype` with ldq, ldk, ldv elements from one token to the next (so they can be slices of one
  * projection's output; a token's heads follow each other). q_heads, k_heads and v_heads each divide
  * `heads`: head h reads head h / (heads / q_heads) of q, and so on (k and v shared by groups of queries,
- * or q and k by all heads, as a state-space block shares B and C, though that decays by the token). out: [batch, seqlen, heads, dv] of `dtype`.
+ * or q and k by all heads, as a state-space block shares B and C, though that decays by the token).
+ * out: [batch, seqlen, heads, dv] of `dtype`.
  * log_decay: [heads] fp32. init_state (nullable: zero), last_state (nullable): [batch, heads, dk, dv]
  * fp32, which may be one buffer. lengths (nullable: seqlen): int32 [batch], clamped to [0, seqlen]; what
  * lies behind a sequence's length is not read, its rows of out are zero, and last_state is the state
